@@ -394,6 +394,7 @@ GQA_API int gqa_lm_head_q8_0(gqa_ctx *ctx, gqa_stream_t stream, const void *pack
 #define GQA_STATUS_BAD_LENGTH 1   /* a device-side pos / seq_len was out of range */
 #define GQA_STATUS_WAIT_TIMEOUT 2 /* a bounded device wait gave up */
 #define GQA_STATUS_BAD_TOKEN 8    /* a device-side token id was outside the vocabulary */
+#define GQA_STATUS_BAD_PAGE 16    /* a page table entry was outside the pool */
 
 /* gqa_model.lm_head_type */
 #define GQA_HEAD_Q6_K 0  /* gqa_lm_head_pack layout (Qwen2.5-1.5B, d_model 1536) */
@@ -521,6 +522,88 @@ GQA_API int gqa_session_status(const gqa_session *s, int *base_pos,
 GQA_API int gqa_prefill_bf16(gqa_ctx *ctx, gqa_stream_t stream, int n_seq, int seq_len,
                              const float *qkv, float *out, float *const *k_caches,
                              float *const *v_caches);
+
+/* ---- paged KV cache ----------------------------------------------------- */
+
+/* Types of the paged cache, of the rows that go with it and of logits. */
+#define GQA_F32 0
+#define GQA_BF16 1
+#define GQA_F16 2
+
+/* One layer's cache of many sequences as a pool of pages (device pointers).
+ * Row r of sequence s is row r % page_size of page
+ * page_table[s * table_stride + r / page_size]; element (page, head, row, i)
+ * of either pool is at page * page_stride + head * head_stride +
+ * row * row_stride + i, so a page may be [n_heads_kv][page_size][head_dim] or
+ * [page_size][n_heads_kv][head_dim], dense or padded.  K is stored after RoPE,
+ * as in gqa_layer_kv.  Table entries past a sequence's last row are not read.
+ * An entry outside [0, n_pages) sets GQA_STATUS_BAD_PAGE; its rows are neither
+ * written nor attended.  Pages may be shared by sequences that only read them. */
+typedef struct {
+    int dtype;      /* GQA_F32, GQA_BF16 or GQA_F16; the calls' qkv and out are of it too */
+    int page_size;  /* rows: 16, 32, 64, 128 or 256 */
+    int n_pages;    /* pages in each pool */
+    int max_pages;  /* entries of a sequence's page table row */
+    void *k_pages, *v_pages;                       /* 16-byte aligned */
+    long long page_stride, head_stride, row_stride; /* elements, multiples of 16 bytes */
+    const int *page_table;                         /* [n_seq][max_pages] */
+    long long table_stride;                        /* elements, >= max_pages */
+} gqa_paged_kv;
+
+/* RoPE on the new tokens' keys and append of rotated k and raw v to the pages:
+ * gqa_rope_kv_append for any number of new tokens of many sequences.  The rows
+ * of qkv (q | k | v before RoPE, qkv_stride elements apart) of sequence s are
+ * [q_starts[s], q_starts[s + 1]); they are the last rows of the seq_lens[s]
+ * rows that the sequence has with them (q_starts [n_seq + 1] ascending,
+ * seq_lens [n_seq], both device).  q_starts NULL: one token per sequence, row
+ * s.  Rows past the last sequence are left alone.  A length below the new
+ * tokens' number or past the table sets GQA_STATUS_BAD_LENGTH and skips the
+ * sequence.  The angle pos * theta^(-2i/d) is formed in 64 bits (the decode
+ * calls above form it in fp32, as the reference does), so that far positions
+ * keep their place; q is not touched.  Two tokens of one call must not be
+ * given the same cache row.  Both shapes of gqa_create. */
+GQA_API int gqa_paged_append(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_kv *kv, int n_seq,
+                             int n_tokens, const int *q_starts, const int *seq_lens,
+                             const void *qkv, long long qkv_stride);
+
+/* Causal attention of the new tokens over their sequences' pages, which hold
+ * the new rows already (gqa_paged_append before it): the token at position p
+ * attends rows [0, p].  q of each row is rotated for its position on the way;
+ * arguments as in gqa_paged_append.  max_new bounds the new tokens and max_len
+ * the rows of every sequence (a sequence beyond either sets
+ * GQA_STATUS_BAD_LENGTH and is skipped: its rows of out are left as they
+ * were).  Results go to out + row * out_stride (n_heads_q * head_dim
+ * elements); out may equal qkv with the same stride.  A token with no
+ * readable row gets zeros.  Rows of the cache past a token's position, and
+ * whatever stands in a page past the sequence's end, do not reach its output. */
+GQA_API int gqa_paged_attention(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_kv *kv,
+                                int n_seq, int n_tokens, const int *q_starts,
+                                const int *seq_lens, int max_new, int max_len, const void *qkv,
+                                long long qkv_stride, void *out, long long out_stride);
+
+/* ---- sampling ------------------------------------------------------------- */
+
+#define GQA_SAMPLE_MAX_VOCAB (1 << 20)
+
+/* One token per row of logits (n_rows rows of vocab, logits_stride elements
+ * apart, of type dtype), next to the greedy pick of gqa_lm_head.  Per row:
+ * weights exp((x - max) / temperature); tokens in descending order of logit,
+ * equal logits by ascending id; top_k keeps the first k; top_p the shortest
+ * prefix of those whose weight is at least top_p of theirs (at least one);
+ * min_p those of weight at least min_p (the largest is 1; the first token
+ * always stays).  tokens[row] is the first id, in ascending order of id, at
+ * which the cumulative kept weight exceeds uniform[row] (in [0, 1)) times the
+ * kept total.  Weights are added as 62-bit integers, exact in any order: equal
+ * inputs give equal tokens.  All arrays are device arrays of n_rows;
+ * temperature NULL means 1, top_k / top_p / min_p NULL leave that filter out.
+ * In a row, top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 leave it out
+ * too, and temperature <= 0 takes the first largest logit.  A NaN logit counts
+ * as -infinity, which is never drawn; a row with nothing above -infinity gives
+ * 0; if the largest is +infinity, only such logits are drawn. */
+GQA_API int gqa_sample(gqa_ctx *ctx, gqa_stream_t stream, int n_rows, int vocab, int dtype,
+                       const void *logits, long long logits_stride, const float *temperature,
+                       const int *top_k, const float *top_p, const float *min_p,
+                       const float *uniform, int *tokens);
 
 /* ---- layer call without allocation ------------------------------------ */
 

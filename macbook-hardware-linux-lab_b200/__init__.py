@@ -13,5 +13,6 @@ The directory name contains hyphens, so it is loaded by path (see
 """
 from . import seeded, shard  # noqa: F401
 from .gqa import (BlockWeights, Context, Exchange, FfnWeights, Gguf, GqaError,  # noqa: F401
-                  Graph, LayerKV, LoadedModel, Model, ModelHandle, Session, block_weights_of,
-                  ffn_weights_of, header_functions, kv_of, last_error, lib)
+                  Graph, LayerKV, LoadedModel, Model, ModelHandle, PagedKV, Session,
+                  block_weights_of, ffn_weights_of, header_functions, kv_of, last_error, lib,
+                  paged_kv_of)

@@ -18,8 +18,14 @@
 #include "gqa.h"
 #include "gqa_common.cuh"
 #include "gqa_merge.cuh"
+#include "gqa_paged.cuh"
+#include "gqa_sample.cuh"
 
 namespace gqa {
+cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int head_dim,
+                                cudaStream_t st, bool pdl);
+cudaError_t launch_paged_attention(const PagedAttnParams& p, int dtype, int head_dim,
+                                   cudaStream_t st, bool pdl);
 size_t decode_smem_bytes();
 cudaError_t prepare_decode_kernels();
 cudaError_t launch_decode_split(const DecodeParams& p, int n_seq, bool fused, cudaStream_t st,
@@ -152,6 +158,7 @@ struct gqa_ctx {
   size_t prefill_cap = 0;                // elements
   float2* rope_cs = nullptr;             // prefill RoPE table [rope_cap][64] (cos, sin)
   int rope_cap = 0;                      // positions in the table
+  double* rope_turns = nullptr;          // [head_dim / 2] theta^(-2i/d) / (2 pi) (paged ops)
 };
 
 struct gqa_graph {
@@ -607,6 +614,65 @@ int shard_partials(gqa_ctx* c, cudaStream_t st, const gqa_layer_kv* kv, const fl
   return GQA_OK;
 }
 
+// ---- paged operators: argument checks ----
+
+constexpr long long kPagedMaxStride = 1LL << 40;  // elements
+
+int dtype_size(int dtype) {
+  return dtype == GQA_F32 ? 4 : dtype == GQA_BF16 || dtype == GQA_F16 ? 2 : 0;
+}
+
+int check_paged(const gqa_ctx* c, const gqa_paged_kv* kv, int n_seq, int n_tokens,
+                const int* q_starts, const int* seq_lens, const void* qkv, long long qkv_stride) {
+  if (!kv || !kv->k_pages || !kv->v_pages || !kv->page_table)
+    return fail(GQA_ERR_INVALID_ARG, "null paged cache, pages or page table");
+  const long long size = dtype_size(kv->dtype);
+  if (!size) return fail(GQA_ERR_INVALID_ARG, "unknown dtype %d", kv->dtype);
+  const int ps = kv->page_size;
+  if (ps < 16 || ps > 256 || (ps & (ps - 1)))
+    return fail(GQA_ERR_INVALID_ARG, "page_size %d: must be 16, 32, 64, 128 or 256", ps);
+  if (kv->n_pages < 1 || kv->max_pages < 1 || kv->max_pages > (1 << 30) / ps)
+    return fail(GQA_ERR_INVALID_ARG, "n_pages %d or max_pages %d out of range", kv->n_pages,
+                kv->max_pages);
+  if (kv->table_stride < kv->max_pages || kv->table_stride > kPagedMaxStride)
+    return fail(GQA_ERR_INVALID_ARG, "table_stride smaller than max_pages");
+  const int hd = c->cfg.head_dim, nkv = c->cfg.n_heads_kv;
+  const auto bad = [&](long long s) { return s < hd || s > kPagedMaxStride || (s * size & 15); };
+  if (bad(kv->page_stride) || bad(kv->head_stride) || bad(kv->row_stride))
+    return fail(GQA_ERR_INVALID_ARG, "page, head and row strides must be multiples of 16 bytes of "
+                "at least head_dim elements");
+  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
+    return fail(GQA_ERR_INVALID_ARG, "pages must be 16-byte aligned");
+  if (n_seq < 0 || n_seq > 65535 || n_tokens < 0 || n_tokens > (1 << 24))
+    return fail(GQA_ERR_INVALID_ARG, "n_seq %d or n_tokens %d out of range", n_seq, n_tokens);
+  if (n_tokens == 0) return GQA_OK;
+  if (n_seq == 0) return fail(GQA_ERR_INVALID_ARG, "%d tokens of no sequence", n_tokens);
+  if (!q_starts && n_tokens != n_seq)
+    return fail(GQA_ERR_INVALID_ARG, "without q_starts every sequence has one token (%d of %d)",
+                n_tokens, n_seq);
+  if (!seq_lens || !qkv) return fail(GQA_ERR_INVALID_ARG, "null seq_lens or qkv");
+  if (!aligned16(qkv) || (qkv_stride * size & 15))
+    return fail(GQA_ERR_INVALID_ARG, "qkv and its stride must be 16-byte aligned");
+  if (qkv_stride < (long long)(c->cfg.n_heads_q + 2 * nkv) * hd || qkv_stride > kPagedMaxStride)
+    return fail(GQA_ERR_INVALID_ARG, "qkv stride smaller than one token's row");
+  return GQA_OK;
+}
+
+PagedView paged_view(const gqa_paged_kv* kv) {
+  PagedView v{};
+  v.k = kv->k_pages;
+  v.v = kv->v_pages;
+  v.page_stride = kv->page_stride;
+  v.head_stride = kv->head_stride;
+  v.row_stride = kv->row_stride;
+  v.table = kv->page_table;
+  v.table_stride = kv->table_stride;
+  while ((1 << v.page_shift) < kv->page_size) ++v.page_shift;
+  v.n_pages = kv->n_pages;
+  v.max_pages = kv->max_pages;
+  return v;
+}
+
 }  // namespace
 
 namespace gqa {
@@ -672,6 +738,14 @@ int gqa_create(const gqa_config* cfg, int device, gqa_ctx** out) {
   if (e == cudaSuccess) e = prepare_prefill_kernels();
   if (e == cudaSuccess) e = cudaMalloc(&c->inv_freq, sizeof(float) * kHalf);
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(int));
+  if (e == cudaSuccess) e = cudaMalloc(&c->rope_turns, sizeof(double) * kHalf);
+  if (e == cudaSuccess) {
+    // rotations per position, in 64 bits (the paged operators reach far positions)
+    double turns[kHalf] = {};
+    for (int i = 0; i < cfg->head_dim / 2; ++i)
+      turns[i] = pow((double)cfg->rope_theta, -2.0 * i / cfg->head_dim) / 6.283185307179586477;
+    e = cudaMemcpy(c->rope_turns, turns, sizeof(turns), cudaMemcpyHostToDevice);
+  }
   if (e == cudaSuccess)
     e = cudaMalloc(&c->blk_qkv, sizeof(float) * (cfg->n_heads_q + 2 * cfg->n_heads_kv) * kHeadDim);
   if (e == cudaSuccess) e = cudaMalloc(&c->blk_attn, sizeof(float) * cfg->n_heads_q * kHeadDim);
@@ -719,6 +793,7 @@ int gqa_destroy(gqa_ctx* c) {
   if (c->head_best) cudaFree(c->head_best);
   if (c->prefill_img) cudaFree(c->prefill_img);
   if (c->rope_cs) cudaFree(c->rope_cs);
+  if (c->rope_turns) cudaFree(c->rope_turns);
   if (c->part_o) cudaFree(c->part_o);
   if (c->part_ml) cudaFree(c->part_ml);
   delete c;
@@ -1573,6 +1648,110 @@ int gqa_prefill_bf16(gqa_ctx* c, gqa_stream_t stream, int n_seq, int seq_len, co
   GQA_CUDA(launch_prefill(qkv, (long long)seq_len * (nq + 2 * nkv) * kHeadDim, n_seq, seq_len, nq,
                           nkv, c->rope_cs, qimg, kimg, vimg, k_caches, v_caches, c->cfg.t_max,
                           out, c->status, c->counters + kPrefillSchedSlot, c->n_sm, st));
+  return GQA_OK;
+}
+
+/* ---- paged KV cache and sampling ---------------------------------------- */
+
+int gqa_paged_append(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv, int n_seq,
+                     int n_tokens, const int* q_starts, const int* seq_lens, const void* qkv,
+                     long long qkv_stride) {
+  GQA_RANGE("gqa_paged_append");
+  if (!c) return fail(GQA_ERR_INVALID_ARG, "null context");
+  int rc = check_paged(c, kv, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride);
+  if (rc != GQA_OK || n_tokens == 0) return rc;
+  DeviceGuard g(c->device);
+  PagedAppendParams p{};
+  p.kv = paged_view(kv);
+  p.plan = TokenPlan{q_starts, seq_lens, n_seq, n_tokens};
+  p.qkv = qkv;
+  p.qkv_stride = qkv_stride;
+  p.turns = c->rope_turns;
+  p.n_q = c->cfg.n_heads_q;
+  p.n_kv = c->cfg.n_heads_kv;
+  p.status = c->status;
+  GQA_CUDA(launch_paged_append(p, kv->dtype, c->cfg.head_dim, (cudaStream_t)stream, c->pdl != 0));
+  return GQA_OK;
+}
+
+int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv, int n_seq,
+                        int n_tokens, const int* q_starts, const int* seq_lens, int max_new,
+                        int max_len, const void* qkv, long long qkv_stride, void* out,
+                        long long out_stride) {
+  GQA_RANGE("gqa_paged_attention");
+  if (!c) return fail(GQA_ERR_INVALID_ARG, "null context");
+  int rc = check_paged(c, kv, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride);
+  if (rc != GQA_OK || n_tokens == 0) return rc;
+  const int nq = c->cfg.n_heads_q, hd = c->cfg.head_dim;
+  const long long size = dtype_size(kv->dtype);
+  if (!out || !aligned16(out) || (out_stride * size & 15))
+    return fail(GQA_ERR_INVALID_ARG, "out and its stride must be 16-byte aligned");
+  if (out_stride < (long long)nq * hd || out_stride > kPagedMaxStride)
+    return fail(GQA_ERR_INVALID_ARG, "out stride outside [%d, %lld]", nq * hd, kPagedMaxStride);
+  if (max_len < 1) return fail(GQA_ERR_INVALID_ARG, "max_len %d below 1", max_len);
+  // (no length beyond the table's rows is accepted by the kernels)
+  max_len = std::min(max_len, kv->max_pages * kv->page_size);
+  if (max_new < 1 || (!q_starts && max_new != 1))
+    return fail(GQA_ERR_INVALID_ARG, "max_new %d below 1, or not 1 without q_starts", max_new);
+  max_new = std::min(max_new, std::min(max_len, n_tokens));
+  const char* q0 = static_cast<const char*>(qkv);
+  const char* o0 = static_cast<const char*>(out);
+  if ((o0 != q0 || out_stride != qkv_stride) && o0 < q0 + qkv_stride * size * n_tokens &&
+      q0 < o0 + out_stride * size * n_tokens)
+    return fail(GQA_ERR_INVALID_ARG, "out overlaps qkv without being equal to it");
+  DeviceGuard g(c->device);
+  PagedAttnParams p{};
+  p.kv = paged_view(kv);
+  p.plan = TokenPlan{q_starts, seq_lens, n_seq, n_tokens};
+  p.qkv = qkv;
+  p.qkv_stride = qkv_stride;
+  p.out = out;
+  p.out_stride = out_stride;
+  p.turns = c->rope_turns;
+  p.n_q = nq;
+  p.n_kv = c->cfg.n_heads_kv;
+  p.max_new = max_new;
+  p.max_len = max_len;
+  p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
+  p.status = c->status;
+  GQA_CUDA(launch_paged_attention(p, kv->dtype, hd, (cudaStream_t)stream, c->pdl != 0));
+  return GQA_OK;
+}
+
+int gqa_sample(gqa_ctx* c, gqa_stream_t stream, int n_rows, int vocab, int dtype,
+               const void* logits, long long logits_stride, const float* temperature,
+               const int* top_k, const float* top_p, const float* min_p, const float* uniform,
+               int* tokens) {
+  GQA_RANGE("gqa_sample");
+  if (!c) return fail(GQA_ERR_INVALID_ARG, "null context");
+  if (!dtype_size(dtype)) return fail(GQA_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  if (n_rows < 0 || n_rows > (1 << 20))
+    return fail(GQA_ERR_INVALID_ARG, "n_rows %d outside [0, %d]", n_rows, 1 << 20);
+  if (vocab < 1 || vocab > GQA_SAMPLE_MAX_VOCAB)
+    return fail(GQA_ERR_INVALID_ARG, "vocab %d outside [1, %d]", vocab, GQA_SAMPLE_MAX_VOCAB);
+  if (n_rows == 0) return GQA_OK;
+  if (!logits || !uniform || !tokens)
+    return fail(GQA_ERR_INVALID_ARG, "gqa_sample: null logits, uniform or tokens");
+  if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype))
+    return fail(GQA_ERR_INVALID_ARG, "logits not aligned to their type");
+  if (logits_stride < vocab || logits_stride > kPagedMaxStride)
+    return fail(GQA_ERR_INVALID_ARG, "logits stride outside [vocab, %lld]", kPagedMaxStride);
+  DeviceGuard g(c->device);
+  SampleParams p{};
+  p.logits = logits;
+  p.logits_stride = logits_stride;
+  p.n_rows = n_rows;
+  p.vocab = vocab;
+  int bits = 0;
+  while ((1 << bits) < vocab) ++bits;
+  p.wshift = 62 - bits;  // a row's weights add up to at most 2^62
+  p.temperature = temperature;
+  p.top_k = top_k;
+  p.top_p = top_p;
+  p.min_p = min_p;
+  p.uniform = uniform;
+  p.tokens = tokens;
+  GQA_CUDA(launch_sample(p, dtype, (cudaStream_t)stream, c->pdl != 0));
   return GQA_OK;
 }
 

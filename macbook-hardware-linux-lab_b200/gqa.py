@@ -49,6 +49,10 @@ VARIANT_QUANT = {0: 32, 1: 32, 2: 32, 3: 64, 4: 32, 5: 64, 6: 32}
 STATUS_BAD_LENGTH = 1
 STATUS_WAIT_TIMEOUT = 2
 STATUS_BAD_TOKEN = 8
+STATUS_BAD_PAGE = 16
+
+F32, BF16, F16 = 0, 1, 2   # GQA_F32, GQA_BF16, GQA_F16
+SAMPLE_MAX_VOCAB = 1 << 20
 
 HEAD_Q6_K = 0   # gqa_model.lm_head_type: gqa_lm_head_pack layout (Qwen2.5-1.5B)
 HEAD_Q8_0 = 1   # gqa_lm_head_q8_0_pack layout (Qwen2.5-0.5B)
@@ -79,6 +83,15 @@ class FfnWeights(ctypes.Structure):
 class LayerKV(ctypes.Structure):
     """One layer's cache: the reference's LayerKVDevice {k_cache, v_cache}."""
     _fields_ = [("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p)]
+
+
+class PagedKV(ctypes.Structure):
+    """One layer's paged cache of many sequences (gqa_paged_kv); see paged_kv_of."""
+    _fields_ = [("dtype", ctypes.c_int), ("page_size", ctypes.c_int), ("n_pages", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("k_pages", ctypes.c_void_p),
+                ("v_pages", ctypes.c_void_p), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong),
+                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong)]
 
 
 class GgufTensor(ctypes.Structure):
@@ -167,6 +180,10 @@ _SIGNATURES = {
     "gqa_session_status": [_vp, ctypes.POINTER(_i), ctypes.POINTER(_ull), ctypes.POINTER(_i),
                            ctypes.POINTER(_i)],
     "gqa_prefill_bf16": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp],
+    "gqa_paged_append": [_vp, _vp, ctypes.POINTER(PagedKV), _i, _i, _vp, _vp, _vp, _ll],
+    "gqa_paged_attention": [_vp, _vp, ctypes.POINTER(PagedKV), _i, _i, _vp, _vp, _i, _i, _vp, _ll,
+                            _vp, _ll],
+    "gqa_sample": [_vp, _vp, _i, _i, _i, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp],
     "gqa_fill_normal": [_vp, _vp, _vp, _ll, _ull, _ull, _ll],
     "gqa_inv_freq": [_vp, ctypes.POINTER(ctypes.c_float)],
     "gqa_version": [],
@@ -248,6 +265,80 @@ def block_weights_of(w_qkv, b_qkv, w_o, gamma) -> BlockWeights:
 def ffn_weights_of(w_gate, w_up, w_down, gamma) -> FfnWeights:
     """FfnWeights of device tensors (Q4_0 byte tensors and a float tensor)."""
     return FfnWeights(_ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(gamma))
+
+
+def _dtype_of(x) -> int:
+    """GQA_F32 / GQA_BF16 / GQA_F16 of a torch tensor or a numpy array."""
+    name = str(x.dtype).removeprefix("torch.")
+    codes = {"float32": F32, "bfloat16": BF16, "float16": F16}
+    if name not in codes:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"type {name} is not float32, bfloat16 or float16")
+    return codes[name]
+
+
+def _expect(x, what: str, device: int, dtype: int | str | None = None) -> None:
+    """Refuses a tensor argument of another type, on another device, or whose last dimension is
+    not dense (plain pointers are taken as they are)."""
+    if x is None or not hasattr(x, "data_ptr"):
+        return
+    if not x.is_cuda or x.device.index != device:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is on {x.device}, not on cuda:{device}")
+    if dtype == "int32":
+        if str(x.dtype) != "torch.int32":
+            raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is {x.dtype}, not int32")
+    elif dtype is not None and _dtype_of(x) != dtype:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is {x.dtype}, not the cache's or float32")
+    if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is not dense in its last dimension")
+
+
+def _count(x, what: str, need: int) -> None:
+    if x is not None and hasattr(x, "numel") and x.numel() < need:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} holds {x.numel()} elements, {need} needed")
+
+
+def _row_stride(x, what: str, rows: int, width: int, stride: int | None) -> int:
+    """Elements between the rows of a [rows, width] argument: as given, or the tensor's own."""
+    if hasattr(x, "data_ptr") and x.dim() == 2:
+        if x.shape[0] < rows or x.shape[1] < width:
+            raise GqaError(GQA_ERR_INVALID_ARG,
+                           f"{what} is {tuple(x.shape)}, needs {rows} rows of {width}")
+        if stride is None:
+            return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    return width if stride is None else stride
+
+
+def paged_kv_of(k_pages, v_pages, page_table, layout: str = "hnd") -> PagedKV:
+    """PagedKV of device tensors: pools [n_pages, n_heads_kv, page_size, head_dim] ("hnd") or
+    [n_pages, page_size, n_heads_kv, head_dim] ("nhd"), both with the same strides, and an int32
+    page table [n_seq, max_pages]."""
+    if layout not in ("hnd", "nhd"):
+        raise GqaError(GQA_ERR_INVALID_ARG, f"layout {layout!r} is not 'hnd' or 'nhd'")
+    if (k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype
+            or k_pages.stride() != v_pages.stride() or k_pages.device != v_pages.device):
+        raise GqaError(GQA_ERR_INVALID_ARG, "the pools must be two 4-d tensors alike")
+    if page_table.dim() != 2:
+        raise GqaError(GQA_ERR_INVALID_ARG, "the page table must be [n_seq, max_pages]")
+    device = k_pages.device.index
+    _expect(k_pages, "k_pages", device)
+    _expect(v_pages, "v_pages", device)
+    _expect(page_table, "page_table", device, "int32")
+    rows, heads = (2, 1) if layout == "hnd" else (1, 2)
+
+    def stride(dim, dense):
+        return k_pages.stride(dim) if k_pages.shape[dim] > 1 else dense
+
+    d = k_pages.shape[3]
+    row = stride(rows, d)
+    head = stride(heads, d * k_pages.shape[2] if layout == "hnd" else d)
+    kv = PagedKV(_dtype_of(k_pages), k_pages.shape[rows], k_pages.shape[0], page_table.shape[1],
+                 _ptr(k_pages), _ptr(v_pages),
+                 stride(0, d * k_pages.shape[1] * k_pages.shape[2]), head, row,
+                 _ptr(page_table),
+                 page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1])
+    kv.keep = (k_pages, v_pages, page_table)
+    kv.sizes = (k_pages.shape[heads], d, page_table.shape[0], device)
+    return kv
 
 
 def _kv_array(kvs) -> ctypes.Array:
@@ -684,6 +775,68 @@ class Context:
                      stream=None) -> None:
         _check(lib().gqa_prefill_bf16(self._h, _stream(stream), n_seq, seq_len, _ptr(qkv),
                                       _ptr(out), _ptr(k_ptrs), _ptr(v_ptrs)))
+
+    # ---- paged cache and sampling ----
+
+    def _stream_of(self, stream) -> int | None:
+        if stream is None:  # torch's current stream on this context's device
+            import torch
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return _stream(stream)
+
+    def _paged_args(self, kv: PagedKV, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride):
+        width = (self.n_heads_q + 2 * self.cfg.n_heads_kv) * self.head_dim
+        if hasattr(kv, "sizes"):
+            heads, d, seqs, device = kv.sizes
+            if heads != self.n_heads_kv or d != self.head_dim or device != self.device:
+                raise GqaError(GQA_ERR_INVALID_ARG,
+                               f"the pools hold {heads} heads of {d} on cuda:{device}; the context "
+                               f"has {self.n_heads_kv} of {self.head_dim} on cuda:{self.device}")
+            if n_seq > seqs:
+                raise GqaError(GQA_ERR_INVALID_ARG, f"the page table has {seqs} rows of {n_seq}")
+        _expect(qkv, "qkv", self.device, kv.dtype)
+        _expect(q_starts, "q_starts", self.device, "int32")
+        _expect(seq_lens, "seq_lens", self.device, "int32")
+        _count(q_starts, "q_starts", n_seq + 1)
+        _count(seq_lens, "seq_lens", n_seq)
+        return _row_stride(qkv, "qkv", n_tokens, width, qkv_stride)
+
+    def paged_append(self, kv: PagedKV, n_seq: int, n_tokens: int, q_starts, seq_lens, qkv,
+                     qkv_stride: int | None = None, stream=None) -> None:
+        """Rotated k and raw v of the new tokens into the pages (gqa_paged_append)."""
+        qkv_stride = self._paged_args(kv, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride)
+        _check(lib().gqa_paged_append(self._h, self._stream_of(stream), ctypes.byref(kv), n_seq,
+                                      n_tokens, _ptr(q_starts), _ptr(seq_lens), _ptr(qkv),
+                                      qkv_stride))
+
+    def paged_attention(self, kv: PagedKV, n_seq: int, n_tokens: int, q_starts, seq_lens,
+                        max_new: int, max_len: int, qkv, out, qkv_stride: int | None = None,
+                        out_stride: int | None = None, stream=None) -> None:
+        """Attention of the new tokens over their pages (gqa_paged_attention)."""
+        qkv_stride = self._paged_args(kv, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride)
+        _expect(out, "out", self.device, kv.dtype)
+        out_stride = _row_stride(out, "out", n_tokens, self.n_heads_q * self.head_dim, out_stride)
+        _check(lib().gqa_paged_attention(self._h, self._stream_of(stream), ctypes.byref(kv), n_seq,
+                                         n_tokens, _ptr(q_starts), _ptr(seq_lens), max_new,
+                                         max_len, _ptr(qkv), qkv_stride, _ptr(out), out_stride))
+
+    def sample(self, n_rows: int, vocab: int, logits, temperature, top_k, top_p, min_p, uniform,
+               tokens, logits_stride: int | None = None, dtype: int | None = None,
+               stream=None) -> None:
+        """A token per row of logits (gqa_sample); temperature, top_k, top_p and min_p may be
+        None.  dtype is the logits tensor's unless given."""
+        if dtype is None:
+            dtype = _dtype_of(logits)
+        _expect(logits, "logits", self.device, dtype)
+        logits_stride = _row_stride(logits, "logits", n_rows, vocab, logits_stride)
+        for x, what, t in ((temperature, "temperature", F32), (top_k, "top_k", "int32"),
+                           (top_p, "top_p", F32), (min_p, "min_p", F32),
+                           (uniform, "uniform", F32), (tokens, "tokens", "int32")):
+            _expect(x, what, self.device, t)
+            _count(x, what, n_rows)
+        _check(lib().gqa_sample(self._h, self._stream_of(stream), n_rows, vocab, dtype,
+                                _ptr(logits), logits_stride, _ptr(temperature), _ptr(top_k),
+                                _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens)))
 
     def fill_normal(self, dst, n: int, seed: int, stream_id: int, offset: int = 0,
                     stream=None) -> None:
