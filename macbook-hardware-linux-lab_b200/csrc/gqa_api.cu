@@ -18,14 +18,10 @@
 #include "gqa.h"
 #include "gqa_common.cuh"
 #include "gqa_merge.cuh"
-#include "gqa_paged.cuh"
+#include "gqa_paged_launch.cuh"
 #include "gqa_sample.cuh"
 
 namespace gqa {
-cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int head_dim,
-                                cudaStream_t st, bool pdl);
-cudaError_t launch_paged_attention(const PagedAttnParams& p, int dtype, int head_dim,
-                                   cudaStream_t st, bool pdl);
 size_t decode_smem_bytes();
 cudaError_t prepare_decode_kernels();
 cudaError_t launch_decode_split(const DecodeParams& p, int n_seq, bool fused, cudaStream_t st,
@@ -158,6 +154,7 @@ struct gqa_ctx {
   size_t prefill_cap = 0;                // elements
   float2* rope_cs = nullptr;             // prefill RoPE table [rope_cap][64] (cos, sin)
   int rope_cap = 0;                      // positions in the table
+  PagedPartials paged{};                 // parts of split pairs (paged attention)
   double* rope_turns = nullptr;          // [head_dim / 2] theta^(-2i/d) / (2 pi) (paged ops)
 };
 
@@ -739,6 +736,14 @@ int gqa_create(const gqa_config* cfg, int device, gqa_ctx** out) {
   if (e == cudaSuccess) e = cudaMalloc(&c->inv_freq, sizeof(float) * kHalf);
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(int));
   if (e == cudaSuccess) e = cudaMalloc(&c->rope_turns, sizeof(double) * kHalf);
+  // Slots of the paged attention, two per CTA of its grids: sized once, so that captured
+  // graphs never see them move.
+  c->paged.n_ctas = 2 * c->n_sm;
+  const size_t paged_rows = (size_t)2 * c->paged.n_ctas * group;
+  if (e == cudaSuccess) e = prepare_paged_decode();
+  if (e == cudaSuccess) e = cudaMalloc(&c->paged.o, sizeof(float) * paged_rows * cfg->head_dim);
+  if (e == cudaSuccess) e = cudaMalloc(&c->paged.ml, sizeof(float2) * paged_rows);
+  if (e == cudaSuccess) e = cudaMalloc(&c->paged.jobs, sizeof(PagedJob) * c->paged.n_ctas);
   if (e == cudaSuccess) {
     // rotations per position, in 64 bits (the paged operators reach far positions)
     double turns[kHalf] = {};
@@ -794,6 +799,9 @@ int gqa_destroy(gqa_ctx* c) {
   if (c->prefill_img) cudaFree(c->prefill_img);
   if (c->rope_cs) cudaFree(c->rope_cs);
   if (c->rope_turns) cudaFree(c->rope_turns);
+  if (c->paged.o) cudaFree(c->paged.o);
+  if (c->paged.ml) cudaFree(c->paged.ml);
+  if (c->paged.jobs) cudaFree(c->paged.jobs);
   if (c->part_o) cudaFree(c->part_o);
   if (c->part_ml) cudaFree(c->part_ml);
   delete c;
@@ -1714,7 +1722,9 @@ int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv,
   p.max_len = max_len;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
   p.status = c->status;
-  GQA_CUDA(launch_paged_attention(p, kv->dtype, hd, (cudaStream_t)stream, c->pdl != 0));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (max_new > 1) GQA_CUDA(launch_paged_chunks(p, kv->dtype, hd, st, c->pdl != 0));
+  GQA_CUDA(launch_paged_decode(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));
   return GQA_OK;
 }
 

@@ -6,6 +6,7 @@
 #include <math_constants.h>
 
 #include "gqa_paged.cuh"
+#include "gqa_paged_launch.cuh"
 
 namespace gqa {
 
@@ -69,22 +70,6 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Page
   *reinterpret_cast<V*>(v_out + D / 2) = v1;
 }
 
-template <typename K, typename P>
-static cudaError_t launch_with_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t st,
-                                   bool pdl, const P& p) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int head_dim,
                                 cudaStream_t st, bool pdl) {
   const int vec = dtype == kDtypeF32 ? 4 : 8;
@@ -122,7 +107,7 @@ __global__ void __launch_bounds__(kSimpleWarps * 32)
   const int s = p.plan.q_starts ? find_sequence(p.plan.q_starts, p.plan.n_seq, tok) : tok;
   int pos, n_new, len;
   const Placed placed = place_token(p.plan, p.kv, s, tok, pos, n_new, len);
-  if (placed == kNoSequence) return;
+  if (placed == kNoSequence || (placed == kPlaced && n_new == 1)) return;
   if (placed == kImpossible || len > p.max_len || n_new > p.max_new) {
     if (threadIdx.x == 0) atomicOr(p.status, kStatusBadLength);
     return;
@@ -213,8 +198,8 @@ static cudaError_t launch_simple(const PagedAttnParams& p, int head_dim, cudaStr
                          p);
 }
 
-cudaError_t launch_paged_attention(const PagedAttnParams& p, int dtype, int head_dim,
-                                   cudaStream_t st, bool pdl) {
+cudaError_t launch_paged_chunks(const PagedAttnParams& p, int dtype, int head_dim,
+                                cudaStream_t st, bool pdl) {
   if (dtype == kDtypeF32) return launch_simple<float>(p, head_dim, st, pdl);
   if (dtype == kDtypeBf16) return launch_simple<__nv_bfloat16>(p, head_dim, st, pdl);
   return launch_simple<__half>(p, head_dim, st, pdl);

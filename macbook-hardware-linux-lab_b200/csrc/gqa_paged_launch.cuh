@@ -1,0 +1,50 @@
+// Launches of the paged operators' kernels.
+#pragma once
+
+#include <algorithm>
+
+#include <cuda_runtime.h>
+
+#include "gqa_paged.cuh"
+
+namespace gqa {
+
+// Parts of (token, KV head) pairs whose rows were split over CTAs: two slots per CTA, each
+// [G][D] un-normalised outputs and [G] (m in log2 units, l), and under the CTA that holds a
+// pair's first part what is to be merged.
+struct PagedJob {
+  int tok, head, slot;
+  int n_parts;  // CTAs from this one on (0: nothing to merge)
+};
+struct PagedPartials {
+  float* o;
+  float2* ml;
+  PagedJob* jobs;
+  int n_ctas;  // that there are slots for
+};
+
+template <typename... P, typename... A>
+cudaError_t launch_with_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                            cudaStream_t st, bool pdl, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+cudaError_t prepare_paged_decode();
+cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int head_dim,
+                                cudaStream_t st, bool pdl);
+cudaError_t launch_paged_decode(const PagedAttnParams& p, const PagedPartials& part, int dtype,
+                                int head_dim, int n_sm, cudaStream_t st, bool pdl);
+cudaError_t launch_paged_chunks(const PagedAttnParams& p, int dtype, int head_dim,
+                                cudaStream_t st, bool pdl);
+
+}  // namespace gqa
