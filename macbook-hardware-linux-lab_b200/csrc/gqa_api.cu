@@ -655,6 +655,29 @@ int check_paged(const gqa_ctx* c, const gqa_paged_kv* kv, int n_seq, int n_token
   return GQA_OK;
 }
 
+// The slots of the paged attention, two per CTA of its grids, in one allocation.
+cudaError_t alloc_paged(gqa_ctx* c, int group) {
+  PagedPartials& w = c->paged;
+  const size_t d = c->cfg.head_dim;
+  w.n_ctas = 2 * c->n_sm;
+  w.n_chunk_ctas = c->n_sm;
+  const size_t rows = (size_t)2 * w.n_ctas * group;
+  const size_t chunk_rows = (size_t)2 * w.n_chunk_ctas * kChunkSlotRows;
+  const size_t o = sizeof(float) * rows * d, co = sizeof(float) * chunk_rows * d;
+  const size_t ml = sizeof(float2) * rows, cml = sizeof(float2) * chunk_rows;
+  const size_t jobs = sizeof(PagedJob) * w.n_ctas, cjobs = sizeof(PagedChunkJob) * w.n_chunk_ctas;
+  char* base = nullptr;
+  const cudaError_t e = cudaMalloc(&base, o + co + ml + cml + jobs + cjobs);
+  if (e != cudaSuccess) return e;
+  w.o = reinterpret_cast<float*>(base);
+  w.chunk_o = reinterpret_cast<float*>(base += o);
+  w.ml = reinterpret_cast<float2*>(base += co);
+  w.chunk_ml = reinterpret_cast<float2*>(base += ml);
+  w.jobs = reinterpret_cast<PagedJob*>(base += cml);
+  w.chunk_jobs = reinterpret_cast<PagedChunkJob*>(base += jobs);
+  return cudaSuccess;
+}
+
 PagedView paged_view(const gqa_paged_kv* kv) {
   PagedView v{};
   v.k = kv->k_pages;
@@ -738,12 +761,9 @@ int gqa_create(const gqa_config* cfg, int device, gqa_ctx** out) {
   if (e == cudaSuccess) e = cudaMalloc(&c->rope_turns, sizeof(double) * kHalf);
   // Slots of the paged attention, two per CTA of its grids: sized once, so that captured
   // graphs never see them move.
-  c->paged.n_ctas = 2 * c->n_sm;
-  const size_t paged_rows = (size_t)2 * c->paged.n_ctas * group;
   if (e == cudaSuccess) e = prepare_paged_decode();
-  if (e == cudaSuccess) e = cudaMalloc(&c->paged.o, sizeof(float) * paged_rows * cfg->head_dim);
-  if (e == cudaSuccess) e = cudaMalloc(&c->paged.ml, sizeof(float2) * paged_rows);
-  if (e == cudaSuccess) e = cudaMalloc(&c->paged.jobs, sizeof(PagedJob) * c->paged.n_ctas);
+  if (e == cudaSuccess) e = prepare_paged_chunk16();
+  if (e == cudaSuccess) e = alloc_paged(c, group);
   if (e == cudaSuccess) {
     // rotations per position, in 64 bits (the paged operators reach far positions)
     double turns[kHalf] = {};
@@ -799,9 +819,7 @@ int gqa_destroy(gqa_ctx* c) {
   if (c->prefill_img) cudaFree(c->prefill_img);
   if (c->rope_cs) cudaFree(c->rope_cs);
   if (c->rope_turns) cudaFree(c->rope_turns);
-  if (c->paged.o) cudaFree(c->paged.o);
-  if (c->paged.ml) cudaFree(c->paged.ml);
-  if (c->paged.jobs) cudaFree(c->paged.jobs);
+  if (c->paged.o) cudaFree(c->paged.o);  // (the one allocation of all of it)
   if (c->part_o) cudaFree(c->part_o);
   if (c->part_ml) cudaFree(c->part_ml);
   delete c;
@@ -1723,7 +1741,10 @@ int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv,
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
   p.status = c->status;
   cudaStream_t st = (cudaStream_t)stream;
-  if (max_new > 1) GQA_CUDA(launch_paged_chunks(p, kv->dtype, hd, st, c->pdl != 0));
+  if (max_new > 1 && kv->dtype == GQA_F32)
+    GQA_CUDA(launch_paged_chunks(p, kv->dtype, hd, st, c->pdl != 0));
+  else if (max_new > 1)
+    GQA_CUDA(launch_paged_chunk16(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));
   GQA_CUDA(launch_paged_decode(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));
   return GQA_OK;
 }

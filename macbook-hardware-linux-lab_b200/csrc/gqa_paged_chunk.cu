@@ -1,0 +1,935 @@
+// Attention of chunks of new tokens over a paged KV cache, 16-bit types, on the
+// 5th-generation tensor cores.
+//
+// S = Q K^T and O = P V over tiles of 128 keys with the running maximum and sum of a
+// softmax, causal by position.  4 G d operations a key and token against 4 d bytes a
+// key: for chunks of more than a few tokens the tensor cores and the exponential unit
+// bound it, not memory.
+//
+// Rows: the G query heads of a KV head are rows of one tile beside each other (row =
+// token * G + head, 21 tokens x 6 or 18 x 7 = 126 of 128 rows), so a chunk reads
+// its keys once for all of them and the causal edge is 21 tokens wide.  A unit is
+// two such tiles (A and B) over the same keys: the softmax of one runs while the tensor
+// cores work on the other.
+//
+// Work: the key tiles of all units are laid end to end and cut into equal shares, one
+// per CTA, as in the decode kernel (gqa_paged_decode.cu); a unit that crosses shares
+// leaves its parts in two slots per CTA, merged by a second kernel.  So a short chunk
+// over a long cache uses every SM, and the triangle of a whole prompt is balanced.
+//
+// q is rotated for its position by a first kernel, which puts it where the result of the
+// same token will be (every unit reads its q before it writes its output, and parts are
+// merged after all units), so no workspace grows with the batch.  Rounding it to the type
+// there is what the projection before it would do with a rotated q; scores and sums are
+// fp32, weights are rounded to the type for the second product.
+//
+// Warps 0-3 / 4-7: softmax of tile A / B, a row per thread; 8: loader (TMA of the pages);
+// 9: MMA.  Tensor memory: S_A | S_B | O_A | O_B, P over the first half of its S.
+// Every wait is bounded; a wait that runs out sets the status bit, and the CTA drains
+// what it issued and returns its tensor memory.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <math_constants.h>
+
+#include "gqa_paged.cuh"
+#include "gqa_paged_launch.cuh"
+#include "gqa_tc.cuh"
+
+namespace gqa {
+
+namespace {
+
+constexpr int kKeys = 128;
+constexpr int kThreads = 320;
+constexpr int kRowsTile = 128;
+
+template <int G>
+__host__ __device__ constexpr int tile_tokens() { return kRowsTile / G; }
+template <int G>
+__host__ __device__ constexpr int unit_tokens() { return 2 * tile_tokens<G>(); }
+
+// One piece of a CTA's share: key tiles [kt0, kt1) of a unit.
+struct Piece {
+  int seq, head;
+  int tok, n_tok;  // the unit's first token row and its tokens
+  int pos;         // position of the first
+  int len;         // rows of the sequence
+  int kt0, kt1;
+  int slot;        // -1: the unit is whole here
+};
+
+template <int D>
+struct alignas(1024) Smem {
+  uint16_t q[2][kRowsTile * D];
+  uint16_t k[2][kKeys * D];
+  uint16_t v[2][kKeys * D];
+  uint8_t stage[8][4096];
+  Piece ring[4];
+  int poison[4];         // number of the last piece of this ring place with a non-finite V
+  // per key tile: its 16-row parts without a page (four tiles: the softmax of a tile may
+  // still be due when the second tile after it is loaded)
+  unsigned bad_rows[4];
+  uint64_t item_full[4], item_empty[4];
+  uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_final[2], drain;
+  long long scan[kThreads / 32];
+  long long found_before;
+  int found_seq;
+  uint32_t tmem_base;
+  int err;
+};
+
+struct ChunkMaps {
+  CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) { return umma_smem_desc(addr); }
+
+// V as an operand whose rows are keys: [64-column block][key][64], 128-byte swizzle;
+// leading offset between the blocks, stride offset between groups of 8 keys.
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
+  uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((kKeys * 128) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
+  const uint32_t t = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)b_mn_major << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc));
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc));
+}
+
+__device__ __forceinline__ void tma_load4(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                          int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2),
+        "r"(c3), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2),
+        "r"(smem_addr(bar)) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, __nv_bfloat16)) {
+    return pack_bf16(a, b);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return reinterpret_cast<const uint32_t&>(h);
+  }
+}
+
+// A pair of 16-bit values with an infinity or a NaN among them.
+template <typename T>
+__device__ __forceinline__ bool non_finite2(uint32_t x) {
+  const uint32_t e = __is_same(T, __nv_bfloat16) ? 0x7f80u : 0x7c00u;
+  return (x & e) == e || ((x >> 16) & e) == e;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t drop_non_finite2(uint32_t x) {
+  const uint32_t e = __is_same(T, __nv_bfloat16) ? 0x7f80u : 0x7c00u;
+  if ((x & e) == e) x &= 0xffff0000u;
+  if (((x >> 16) & e) == e) x &= 0xffffu;
+  return x;
+}
+
+// The new tokens of sequence s and its rows, when this kernel takes them (two or more).
+__device__ __forceinline__ bool chunk_of(const PagedAttnParams& p, int s, int& tok, int& n_new,
+                                         int& len) {
+  tok = p.plan.q_starts[s];
+  const long long n = p.plan.q_starts[s + 1] - (long long)tok;
+  if (n < 2 || n > p.max_new || tok < 0 || tok + n > p.plan.n_tokens) return false;
+  int pos;
+  return place_token(p.plan, p.kv, s, tok, pos, n_new, len) == kPlaced && len <= p.max_len;
+}
+
+// Key tiles of a unit of the chunk.
+template <int G>
+__device__ __forceinline__ int unit_tiles(int n_new, int len, int unit) {
+  return (len - n_new + min(n_new, (unit + 1) * unit_tokens<G>()) + kKeys - 1) / kKeys;
+}
+template <int G>
+__device__ __forceinline__ long long chunk_tiles(int n_new, int len) {
+  long long sum = 0;
+  for (int u = 0; u * unit_tokens<G>() < n_new; ++u) sum += unit_tiles<G>(n_new, len, u);
+  return sum;
+}
+
+// q rotated into the rows of out: one thread per (token, KV head, 16-byte chunk of the
+// first half of a row), all heads of the group.
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(256) rotate_q_kernel(const PagedAttnParams p) {
+  using V = Vec16<T>;
+  constexpr int kChunks = D / 2 / V::n;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int per_token = p.n_kv * kChunks;
+  const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long last = (long long)p.plan.n_tokens * per_token - 1;
+  const int tok = (int)(min(item, last) / per_token);
+  const int tok0 = __shfl_sync(0xffffffffu, tok, 0);
+  int s = find_sequence(p.plan.q_starts, p.plan.n_seq, tok0);
+  while (s + 1 < p.plan.n_seq && p.plan.q_starts[s + 1] <= tok) ++s;
+  if (item > last) return;
+  int first, n_new, len;
+  if (!chunk_of(p, s, first, n_new, len) || tok < first || tok >= first + n_new) {
+    return;  // (another kernel's sequence, or one that is reported there)
+  }
+  const int pos = len - n_new + tok - first;
+  const int rem = (int)(item - (long long)tok * per_token);
+  const int h = rem / kChunks, c = rem % kChunks;
+  float co[V::n], si[V::n];
+#pragma unroll
+  for (int e = 0; e < V::n; ++e) rope_cos_sin(pos, p.turns[c * V::n + e], co[e], si[e]);
+  const T* src = static_cast<const T*>(p.qkv) + (long long)tok * p.qkv_stride +
+                 (long long)h * G * D + c * V::n;
+  T* dst = static_cast<T*>(p.out) + (long long)tok * p.out_stride + (long long)h * G * D +
+           c * V::n;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const V a = *reinterpret_cast<const V*>(src + g * D);
+    const V b = *reinterpret_cast<const V*>(src + g * D + D / 2);
+    V y0, y1;
+#pragma unroll
+    for (int e = 0; e < V::n; ++e) {
+      const float x = Elem<T>::get(a.e[e]), y = Elem<T>::get(b.e[e]);
+      y0.e[e] = Elem<T>::put(x * co[e] - y * si[e]);
+      y1.e[e] = Elem<T>::put(x * si[e] + y * co[e]);
+    }
+    *reinterpret_cast<V*>(dst + g * D) = y0;
+    *reinterpret_cast<V*>(dst + g * D + D / 2) = y1;
+  }
+}
+
+// The pieces of a CTA's share, in order.
+template <int G>
+struct Walk {
+  long long tile, first, last, total, n;
+  long long seq_first;  // first tile of sequence seq
+  int seq;
+
+  __device__ bool next(const PagedAttnParams& p, const PagedPartials& part, Piece& out) {
+    while (tile < last && seq < p.plan.n_seq) {
+      int tok, n_new, len;
+      if (!chunk_of(p, seq, tok, n_new, len)) {
+        ++seq;
+        continue;
+      }
+      const long long per_head = chunk_tiles<G>(n_new, len);
+      if (tile >= seq_first + per_head * p.n_kv) {
+        seq_first += per_head * p.n_kv;
+        ++seq;
+        continue;
+      }
+      const int h = (int)((tile - seq_first) / per_head);
+      long long at = seq_first + h * per_head;  // first tile of the unit
+      int u = 0, tiles = unit_tiles<G>(n_new, len, 0);
+      while (tile >= at + tiles) {
+        at += tiles;
+        tiles = unit_tiles<G>(n_new, len, ++u);
+      }
+      out.seq = seq;
+      out.head = h;
+      out.tok = tok + u * unit_tokens<G>();
+      out.n_tok = min(unit_tokens<G>(), n_new - u * unit_tokens<G>());
+      out.pos = len - n_new + u * unit_tokens<G>();
+      out.len = len;
+      out.kt0 = (int)(tile - at);
+      out.kt1 = (int)min((long long)tiles, last - at);
+      const bool whole = out.kt0 == 0 && out.kt1 == tiles;
+      out.slot = whole ? -1 : 2 * (int)blockIdx.x + (tile == first ? 0 : 1);
+      if (!whole && out.kt0 == 0) {
+        const int last_cta = (int)(((at + tiles) * n + total - 1) / total) - 1;
+        part.chunk_jobs[blockIdx.x] = PagedChunkJob{out.tok, out.n_tok, h, out.slot,
+                                                    last_cta - (int)blockIdx.x + 1};
+      }
+      tile = at + out.kt1;
+      return true;
+    }
+    return false;
+  }
+};
+
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_chunk_kernel(const __grid_constant__ PagedAttnParams p,
+                       const __grid_constant__ PagedPartials part,
+                       const __grid_constant__ ChunkMaps maps, const int hnd, const int box_rows) {
+  extern __shared__ unsigned char smem_raw[];
+  using S = Smem<D>;
+  S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                ~static_cast<uintptr_t>(1023));
+  constexpr int kTok = tile_tokens<G>();
+  constexpr int kBlocks = D / 64;               // 64-column blocks of a row
+  constexpr uint32_t kTileBytes = kKeys * D * 2;
+  constexpr uint32_t kQBytes = kTok * G * D * 2;
+  constexpr uint32_t kIdS = idesc<T>(128, false), kIdO = idesc<T>(D, true);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* err = &sm.err;
+
+  if (tid == 0) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&sm.item_full[s], 1);
+      mbar_init(&sm.item_empty[s], 9);  // the MMA thread and the softmax warps
+      sm.poison[s] = -1;
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sm.q_full[s], 1);
+      mbar_init(&sm.q_empty[s], 1);
+      mbar_init(&sm.k_full[s], 1);
+      mbar_init(&sm.k_empty[s], 1);
+      mbar_init(&sm.v_full[s], 1);
+      mbar_init(&sm.v_empty[s], 1);
+      mbar_init(&sm.s_full[s], 1);
+      mbar_init(&sm.p_full[s], 4);
+      mbar_init(&sm.o_final[s], 1);
+    }
+    mbar_init(&sm.drain, 1);
+    sm.err = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_addr(&sm.tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // the two rows of a Q tile that no copy fills
+  for (int i = tid; i < 2 * kBlocks * (kRowsTile - kTok * G) * 64; i += kThreads) {
+    const int x = i % 64, r = i / 64 % (kRowsTile - kTok * G), b = i / 64 / (kRowsTile - kTok * G);
+    sm.q[b / kBlocks][(b % kBlocks) * kRowsTile * 64 + (kTok * G + r) * 64 + x] = 0;
+  }
+  fence_proxy_async_smem();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // Tiles of all units, and this CTA's share of them.
+  Walk<G> walk{};
+  {
+    long long mine = 0;
+    for (int s = tid; s < p.plan.n_seq; s += kThreads) {
+      int tok, n_new, len;
+      if (chunk_of(p, s, tok, n_new, len))
+        mine += chunk_tiles<G>(n_new, len);
+      else if (blockIdx.x == 0 && p.plan.q_starts[s + 1] - (long long)p.plan.q_starts[s] > 1)
+        atomicOr(p.status, kStatusBadLength);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0) sm.scan[warp] = mine;
+    if (tid == 0) part.chunk_jobs[blockIdx.x].n_parts = 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    long long total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) total += sm.scan[w];
+    walk.total = total * p.n_kv;
+    walk.n = min((long long)gridDim.x, walk.total);
+    if (blockIdx.x < walk.n) {
+      walk.first = blockIdx.x * walk.total / walk.n;
+      walk.last = (blockIdx.x + 1) * walk.total / walk.n;
+    }
+    walk.tile = walk.first;
+  }
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 8) {
+    // ---- loader ----
+    const bool some = walk.first < walk.last;
+    Piece pc{};
+    int kv = 0, rd = 0, nq[2] = {0, 0};
+    bool ok = true;
+    const CUtensorMap *km = &maps.k, *vm = &maps.v;
+    for (;; ++rd) {
+      const int place = rd & 3;
+      if (rd >= 4) ok = wait_or_abort(&sm.item_empty[place], ((rd >> 2) - 1) & 1, err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      int more = 0;
+      if (lane == 0) {
+        more = some && walk.next(p, part, pc);
+        if (!more) pc.n_tok = 0;
+        sm.ring[place] = pc;
+        mbar_arrive(&sm.item_full[place]);
+      }
+      __syncwarp();
+      more = __shfl_sync(0xffffffffu, more, 0);
+      if (!more) break;
+      const int seq = __shfl_sync(0xffffffffu, pc.seq, 0);
+      const int head = __shfl_sync(0xffffffffu, pc.head, 0);
+      const int tok = __shfl_sync(0xffffffffu, pc.tok, 0);
+      const int n_tok = __shfl_sync(0xffffffffu, pc.n_tok, 0);
+      const int len = __shfl_sync(0xffffffffu, pc.len, 0);
+      const int kt0 = __shfl_sync(0xffffffffu, pc.kt0, 0);
+      const int kt1 = __shfl_sync(0xffffffffu, pc.kt1, 0);
+      for (int g = 0; g < (n_tok > kTok ? 2 : 1) && ok; ++g, __syncwarp()) {
+        if (nq[g] > 0) ok = wait_or_abort(&sm.q_empty[g], (nq[g] - 1) & 1, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sm.q_full[g], kQBytes);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b)
+            tma_load3(sm.q[g] + b * kRowsTile * 64, &maps.q, b * 64, head * G, tok + g * kTok,
+                      &sm.q_full[g]);
+        }
+        ++nq[g];
+      }
+      if (!ok) break;
+      const int boxes = kKeys / box_rows;
+      for (int kt = kt0; kt < kt1; ++kt, ++kv) {
+        const int st = kv & 1;
+        // the pages of the tile: one per lane
+        int row = kt * kKeys + lane * box_rows, page = p.kv.n_pages;  // (no such page: zeros)
+        bool bad = false;
+        if (lane < boxes && row < len) {
+          page = page_of(p.kv, seq, row);
+          bad = page < 0;
+          if (bad) {
+            page = p.kv.n_pages;
+            atomicOr(p.status, kStatusBadPage);
+          }
+        }
+        const unsigned bad_boxes = __ballot_sync(0xffffffffu, bad);
+        row &= (1 << p.kv.page_shift) - 1;
+        const int c1 = hnd ? row : head, c2 = hnd ? head : row;
+        const uint32_t reuse = ((kv >> 1) - 1) & 1;
+        if (kv >= 2) ok = wait_or_abort(&sm.k_empty[st], reuse, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          unsigned rows16 = 0;  // 16-row parts without a page
+          for (int i = 0; i < 8; ++i)
+            if (bad_boxes >> (i * 16 / box_rows) & 1) rows16 |= 1u << i;
+          sm.bad_rows[kv & 3] = rows16;
+          mbar_arrive_expect_tx(&sm.k_full[st], kTileBytes);
+        }
+        __syncwarp();
+        if (lane < boxes)
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b)
+            tma_load4(sm.k[st] + b * kKeys * 64 + lane * box_rows * 64, km, b * 64, c1, c2, page,
+                      &sm.k_full[st]);
+        __syncwarp();
+        if (kv >= 2) ok = wait_or_abort(&sm.v_empty[st], reuse, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&sm.v_full[st], kTileBytes);
+        __syncwarp();
+        if (lane < boxes)
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b)
+            tma_load4(sm.v[st] + b * kKeys * 64 + lane * box_rows * 64, vm, b * 64, c1, c2, page,
+                      &sm.v_full[st]);
+        __syncwarp();
+      }
+      if (!ok) break;
+    }
+    if (*err && lane == 0) {
+      // Let the copies already issued land before the CTA's shared memory is handed on
+      // (a phase that was never armed runs into the wait's bound).
+      for (int s = 0; s < 2; ++s) {
+        if (nq[s] > 0) mbar_wait_bounded(&sm.q_full[s], (nq[s] - 1) & 1, kWaitBudget);
+        for (int i = max(0, kv - 1); i <= kv; ++i)
+          if ((i & 1) == s) {
+            mbar_wait_bounded(&sm.k_full[s], (i >> 1) & 1, kWaitBudget / 16);
+            mbar_wait_bounded(&sm.v_full[s], (i >> 1) & 1, kWaitBudget / 16);
+          }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---- MMA issuer ----
+    if (lane == 0) {
+      const auto issue_s = [&](int g, int kv) {
+        const uint32_t q = smem_addr(sm.q[g]), k = smem_addr(sm.k[kv & 1]);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
+          umma_ss(tmem + 128 * g, desc_k_major(q + off), desc_k_major(k + off), kIdS, ks > 0);
+        }
+        umma_commit(&sm.s_full[g]);
+      };
+      const auto issue_pv = [&](int g, int kv, bool acc) {
+        const uint32_t v = smem_addr(sm.v[kv & 1]);
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          umma_ts(tmem + 256 + 128 * g, tmem + 128 * g + ks * 8, desc_mn_major(v + ks * 2048), kIdO,
+                  acc || ks > 0);
+      };
+      const auto take = [&](int n, Piece& pc) {
+        if (!wait_or_abort(&sm.item_full[n & 3], (n >> 2) & 1, err)) return false;
+        pc = sm.ring[n & 3];
+        mbar_arrive(&sm.item_empty[n & 3]);
+        return true;
+      };
+      Piece pc{};
+      int rd = 0, kv = 0, nq[2] = {0, 0}, nt[2] = {0, 0};  // Q tiles, S tiles of A and B
+      bool ok = take(0, pc);
+      bool two = pc.n_tok > kTok;
+      // S of the first key tile of a piece or of the next one
+      const auto first_s = [&](int g, bool start) {
+        if (start) {
+          if (!wait_or_abort(&sm.q_full[g], nq[g] & 1, err)) return false;
+          ++nq[g];
+        }
+        return true;
+      };
+      if (ok && pc.n_tok > 0) {
+        const bool lone = pc.kt1 - pc.kt0 == 1;
+        ok = wait_or_abort(&sm.k_full[0], 0, err) && first_s(0, true);
+        if (ok) {
+          tc_fence_after();
+          issue_s(0, 0);
+          if (lone) umma_commit(&sm.q_empty[0]);
+          if (two) ok = first_s(1, true);
+        }
+        if (ok && two) {
+          tc_fence_after();
+          issue_s(1, 0);
+          if (lone) umma_commit(&sm.q_empty[1]);
+        }
+        if (ok) umma_commit(&sm.k_empty[0]);
+      }
+      int kt = pc.kt0;
+      while (ok && pc.n_tok > 0) {
+        // the key tile after this one: of the same piece, or the next one's first
+        Piece nx = pc;
+        int kt_n = kt + 1;
+        const bool last = kt_n == pc.kt1;
+        if (last) {
+          ok = take(++rd, nx);
+          if (!ok) break;
+          kt_n = nx.kt0;
+        }
+        const bool more = nx.n_tok > 0, two_n = nx.n_tok > kTok;
+        const bool n_last = kt_n + 1 == nx.kt1;
+        const int kv_n = kv + 1;
+        if (!wait_or_abort(&sm.p_full[0], nt[0] & 1, err) ||
+            !wait_or_abort(&sm.v_full[kv & 1], (kv >> 1) & 1, err)) { ok = false; break; }
+        ++nt[0];
+        tc_fence_after();
+        issue_pv(0, kv, kt > pc.kt0);
+        if (!two) umma_commit(&sm.v_empty[kv & 1]);
+        if (last) umma_commit(&sm.o_final[0]);
+        if (more) {
+          ok = first_s(0, last) &&
+               wait_or_abort(&sm.k_full[kv_n & 1], (kv_n >> 1) & 1, err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(0, kv_n);
+          if (n_last) umma_commit(&sm.q_empty[0]);
+        }
+        if (two) {
+          if (!wait_or_abort(&sm.p_full[1], nt[1] & 1, err)) { ok = false; break; }
+          ++nt[1];
+          tc_fence_after();
+          issue_pv(1, kv, kt > pc.kt0);
+          umma_commit(&sm.v_empty[kv & 1]);
+          if (last) umma_commit(&sm.o_final[1]);
+        }
+        if (more) {
+          if (two_n) {
+            ok = first_s(1, last);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(1, kv_n);
+            if (n_last) umma_commit(&sm.q_empty[1]);
+          }
+          umma_commit(&sm.k_empty[kv_n & 1]);
+        }
+        pc = nx;
+        two = two_n;
+        kt = kt_n;
+        kv = kv_n;
+      }
+      umma_commit(&sm.drain);  // no MMA may be running when tensor memory is freed
+      mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax of tile g: thread = row r (token r / G, head r % G) ----
+    const int g = warp >> 2, r = tid & 127;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + 128 * g;
+    const uint32_t t_o = tmem + lane_off + 256 + 128 * g;
+    const float sc = p.scale_log2;
+    uint8_t* stage = sm.stage[warp];
+    int tc = 0;  // S tiles of this half so far
+    int kv = 0;  // key tiles so far
+    int done = 0;
+    bool ok = true;
+    for (int rd = 0; ok; ++rd) {
+      ok = wait_or_abort(&sm.item_full[rd & 3], (rd >> 2) & 1, err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const Piece pc = sm.ring[rd & 3];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[rd & 3]);
+      if (pc.n_tok == 0) break;
+      if (g == 1 && pc.n_tok <= kTok) {  // nothing in tile B
+        kv += pc.kt1 - pc.kt0;
+        continue;
+      }
+      const int my_tok = min(g * kTok + r / G, pc.n_tok - 1);
+      const int limit = pc.pos + my_tok;                // last key of this row
+      const int first_limit = pc.pos + g * kTok;        // of the tile's first row
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++tc, ++kv) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&sm.s_full[g], tc & 1, err));
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = kt * kKeys;
+        const unsigned bad = sm.bad_rows[kv & 3];
+        float alpha = 1.f, sum0 = 0.f, sum1 = 0.f;
+        uint32_t pk[kKeys / 2];
+        // The reference m is the row's maximum of the piece's first tile; it moves when
+        // the weights of a tile add up to more than 2^8 (or m is still -inf), in a
+        // second pass over the tile.
+        bool fresh = __any_sync(0xffffffffu, m == -CUDART_INF_F);
+        const bool start = kt == pc.kt0;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          float s[kKeys];
+          tmem_ld128(t_s, s);
+          if (key0 + kKeys - 1 > first_limit) {
+            const int lim = limit - key0;
+#pragma unroll
+            for (int c = 0; c < kKeys; ++c)
+              if (c > lim) s[c] = -CUDART_INF_F;
+          }
+          if (bad) {
+#pragma unroll
+            for (int c = 0; c < kKeys; ++c)
+              if (bad >> (c / 16) & 1) s[c] = -CUDART_INF_F;
+          }
+          if (fresh) {
+            float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+#pragma unroll
+            for (int c = 4; c < kKeys - 4; c += 8) {
+              mx0 = fmax3(mx0, s[c], s[c + 1]);
+              mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+              mx2 = fmax3(mx2, s[c + 4], s[c + 5]);
+              mx3 = fmax3(mx3, s[c + 6], s[c + 7]);
+            }
+            mx0 = fmax3(mx0, s[kKeys - 4], s[kKeys - 3]);
+            mx1 = fmax3(mx1, s[kKeys - 2], s[kKeys - 1]);
+            const float mn = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc);
+            alpha = start || mn == m ? 1.f : fast_exp2(m - mn);
+            m = mn;
+          }
+          const float nm = m == -CUDART_INF_F ? 0.f : -m;
+          sum0 = 0.f;
+          sum1 = 0.f;
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 2) {
+            float x0, x1;
+            ffma2(x0, x1, s[c], s[c + 1], sc, sc, nm, nm);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            fadd2(sum0, sum1, sum0, sum1, p0, p1);
+            pk[c / 2] = pack2<T>(p0, p1);
+          }
+          if (fresh || !__any_sync(0xffffffffu, !(sum0 + sum1 <= 256.f))) break;
+          fresh = true;
+        }
+        __syncwarp();
+        tmem_st64(t_s, pk);
+        l = l * alpha + (sum0 + sum1);
+        if (!start && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float v[32];
+            tmem_ld32(t_o + c * 32, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] *= alpha;
+            tmem_st32(t_o + c * 32, v);
+          }
+        }
+        // A weight of zero does not cancel an infinity or a NaN.  Rows of V past the
+        // unit's last token are cleared; in those of its own tokens, which only some of its
+        // rows see, what is not finite is cleared here and added to the rows that do see it
+        // at the end.
+        if (g == 0 && key0 + kKeys > pc.pos + 1) {
+          ok = __all_sync(0xffffffffu, wait_or_abort(&sm.v_full[kv & 1], (kv >> 1) & 1, err));
+          if (!ok) break;
+          const int own0 = max(pc.pos + 1 - key0, 0);
+          const int end = pc.pos + pc.n_tok - key0;
+          uint4* v = reinterpret_cast<uint4*>(sm.v[kv & 1]);
+          for (int i = r; i < kBlocks * 8 * kKeys; i += 128) {
+            const int row = i / 8 % kKeys;
+            if (row >= end) {
+              v[i] = make_uint4(0, 0, 0, 0);
+            } else if (row >= own0) {
+              uint4 x = v[i];
+              if (non_finite2<T>(x.x) || non_finite2<T>(x.y) || non_finite2<T>(x.z) ||
+                  non_finite2<T>(x.w)) {
+                x.x = drop_non_finite2<T>(x.x);
+                x.y = drop_non_finite2<T>(x.y);
+                x.z = drop_non_finite2<T>(x.z);
+                x.w = drop_non_finite2<T>(x.w);
+                v[i] = x;
+                *reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) = rd;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[g]);
+      }
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&sm.o_final[g], done & 1, err));
+      ++done;
+      if (!ok) break;
+      tc_fence_after();
+      float o[D];
+      if constexpr (D == 128) {
+        tmem_ld128(t_o, o);
+      } else {
+        float lo[32];
+        tmem_ld32(t_o, lo);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = lo[e];
+        tmem_ld32(t_o + 32, lo);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[32 + e] = lo[e];
+      }
+      if (*reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) == rd) {
+        const int k0 = max(pc.pos + 1, pc.kt0 * kKeys);
+        for (int key = k0; key <= limit && key < pc.kt1 * kKeys; ++key) {
+          const int page = page_of(p.kv, pc.seq, key);
+          if (page < 0) continue;
+          const uint4* row = reinterpret_cast<const uint4*>(
+              static_cast<const T*>(p.kv.v) + row_offset(p.kv, page, pc.head, key));
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 x = row[c];
+            const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float f = Elem<T>::get(e[j]);
+              if (!(fabsf(f) < CUDART_INF_F)) o[c * 8 + j] += f;
+            }
+          }
+        }
+      }
+      // Rows leave through the warp's 4 KB: written a row per thread, read back so that
+      // eight lanes cover 128 bytes of a row (16-byte chunk c of row i at c ^ (i % 8)).
+      const int row_base = (warp & 3) * 32;
+      if (pc.slot < 0) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 x;
+            const float* f = o + b * 64 + c * 8;
+            x.x = pack2<T>(f[0] * inv, f[1] * inv);
+            x.y = pack2<T>(f[2] * inv, f[3] * inv);
+            x.z = pack2<T>(f[4] * inv, f[5] * inv);
+            x.w = pack2<T>(f[6] * inv, f[7] * inv);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = x;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = i * 4 + (lane >> 3), c = lane & 7;
+            const int row = row_base + rr, t = g * kTok + row / G;
+            if (row < kTok * G && t < pc.n_tok) {
+              const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 128 +
+                                                              ((c ^ (rr & 7)) << 4));
+              T* dst = static_cast<T*>(p.out) + (long long)(pc.tok + t) * p.out_stride +
+                       (long long)(pc.head * G + row % G) * D + b * 64 + c * 8;
+              *reinterpret_cast<uint4*>(dst) = x;
+            }
+          }
+          __syncwarp();
+        }
+      } else {
+        const long long base = ((long long)pc.slot * 2 + g) * kRowsTile + row_base;
+        part.chunk_ml[base + lane] = make_float2(m, l);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                make_float4(o[b * 32 + 4 * c], o[b * 32 + 4 * c + 1], o[b * 32 + 4 * c + 2],
+                            o[b * 32 + 4 * c + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = i * 4 + (lane >> 3), c = lane & 7;
+            *reinterpret_cast<float4*>(part.chunk_o + (base + rr) * D + b * 32 + c * 4) =
+                *reinterpret_cast<const float4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (!ok) atomicOr(&sm.err, 1);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && sm.err) atomicOr(p.status, kStatusWaitTimeout);
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// Merges the parts of units that crossed shares: a warp per row, blocks of 8 rows.
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(256) paged_chunk_merge_kernel(const PagedAttnParams p,
+                                                                const PagedPartials part) {
+  pdl_wait();
+  const PagedChunkJob job = part.chunk_jobs[blockIdx.x];
+  if (job.n_parts == 0) return;
+  constexpr int kTok = tile_tokens<G>(), E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int idx = blockIdx.y * 8 + (threadIdx.x >> 5);  // row of the unit's tokens
+  const int t = idx / G, g = idx % G;
+  if (t >= job.n_tok) return;
+  const int row = t < kTok ? idx : kRowsTile + (t - kTok) * G + g;
+  float m = -CUDART_INF_F, l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int i = 0; i < job.n_parts; ++i) {
+    const int slot = i == 0 ? job.slot : 2 * ((int)blockIdx.x + i);
+    const long long at = (long long)slot * 2 * kRowsTile + row;
+    const float2 ml = part.chunk_ml[at];
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = part.chunk_o[at * D + lane * E + e];
+    if (ml.y == 0.f) continue;
+    const float mm = fmaxf(m, ml.x);
+    const float a = exp2f(m - mm), b = exp2f(ml.x - mm);
+    m = mm;
+    l = l * a + ml.y * b;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * a + x[e] * b;
+  }
+  T* out = static_cast<T*>(p.out) + (long long)(job.tok + t) * p.out_stride +
+           (long long)(job.head * G + g) * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = Elem<T>::put(l != 0.f ? o[e] / l : 0.f);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+template <typename T, int D, int G>
+cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int n_sm,
+                       cudaStream_t st, bool pdl) {
+  using V = Vec16<T>;
+  PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
+  if (!encode) return cudaErrorNotSupported;
+  ChunkMaps maps;
+  const CUtensorMapDataType type = __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const int page_rows = 1 << p.kv.page_shift;
+  const int box_rows = std::min(page_rows, kKeys);
+  // the dimension with the smaller stride first
+  const int hnd = p.kv.row_stride <= p.kv.head_stride;
+  const cuuint64_t dims[4] = {D, (cuuint64_t)(hnd ? page_rows : p.n_kv),
+                              (cuuint64_t)(hnd ? p.n_kv : page_rows), (cuuint64_t)p.kv.n_pages};
+  const cuuint64_t strides[3] = {
+      (cuuint64_t)(hnd ? p.kv.row_stride : p.kv.head_stride) * sizeof(T),
+      (cuuint64_t)(hnd ? p.kv.head_stride : p.kv.row_stride) * sizeof(T),
+      (cuuint64_t)p.kv.page_stride * sizeof(T)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(hnd ? box_rows : 1), (cuuint32_t)(hnd ? 1 : box_rows),
+                             1};
+  for (int i = 0; i < 2; ++i)
+    if (encode(i ? &maps.v : &maps.k, type, 4, i ? p.kv.v : p.kv.k, dims, strides, box, ones,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  const cuuint64_t qdims[3] = {D, (cuuint64_t)p.n_q, (cuuint64_t)p.plan.n_tokens};
+  const cuuint64_t qstrides[2] = {D * sizeof(T), (cuuint64_t)p.out_stride * sizeof(T)};
+  const cuuint32_t qbox[3] = {64, G, (cuuint32_t)tile_tokens<G>()};
+  if (encode(&maps.q, type, 3, p.out, qdims, qstrides, qbox, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+
+  const long long items = (long long)p.plan.n_tokens * p.n_kv * (D / 2 / V::n);
+  cudaError_t e = launch_with_pdl(rotate_q_kernel<T, D, G>, dim3((unsigned)((items + 255) / 256)),
+                                  256, 0, st, pdl, p);
+  if (e != cudaSuccess) return e;
+  const long long units =
+      ((long long)p.plan.n_tokens / unit_tokens<G>() + p.plan.n_seq) * p.n_kv;
+  const long long tiles = units * ((p.max_len + kKeys - 1) / kKeys);
+  const int grid = (int)std::min<long long>(n_sm, tiles);
+  e = launch_with_pdl(paged_chunk_kernel<T, D, G>, dim3(grid), kThreads, sizeof(Smem<D>) + 1024,
+                      st, true, p, part, maps, hnd, box_rows);
+  if (e != cudaSuccess) return e;
+  return launch_with_pdl(paged_chunk_merge_kernel<T, D, G>,
+                         dim3(grid, (unit_tokens<G>() * G + 7) / 8), 256, 0, st, true, p, part);
+}
+
+template <typename T, int D, int G>
+cudaError_t prepare_one() {
+  return cudaFuncSetAttribute((const void*)paged_chunk_kernel<T, D, G>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)sizeof(Smem<D>) + 1024);
+}
+
+}  // namespace
+
+cudaError_t prepare_paged_chunk16() {
+  cudaError_t e = prepare_one<__nv_bfloat16, 128, 6>();
+  if (e == cudaSuccess) e = prepare_one<__nv_bfloat16, 64, 7>();
+  if (e == cudaSuccess) e = prepare_one<__half, 128, 6>();
+  if (e == cudaSuccess) e = prepare_one<__half, 64, 7>();
+  return e;
+}
+
+cudaError_t launch_paged_chunk16(const PagedAttnParams& p, const PagedPartials& part, int dtype,
+                                 int head_dim, int n_sm, cudaStream_t st, bool pdl) {
+  const bool wide = head_dim == 128;
+  if (dtype == kDtypeBf16)
+    return wide ? launch_one<__nv_bfloat16, 128, 6>(p, part, n_sm, st, pdl)
+                : launch_one<__nv_bfloat16, 64, 7>(p, part, n_sm, st, pdl);
+  return wide ? launch_one<__half, 128, 6>(p, part, n_sm, st, pdl)
+              : launch_one<__half, 64, 7>(p, part, n_sm, st, pdl);
+}
+
+}  // namespace gqa

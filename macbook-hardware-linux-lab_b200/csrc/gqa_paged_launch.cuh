@@ -16,11 +16,21 @@ struct PagedJob {
   int tok, head, slot;
   int n_parts;  // CTAs from this one on (0: nothing to merge)
 };
+// The same for chunks: units of some tokens, 256 rows a slot.
+struct PagedChunkJob {
+  int tok, n_tok, head, slot;
+  int n_parts;
+};
+constexpr int kChunkSlotRows = 256;
 struct PagedPartials {
   float* o;
   float2* ml;
   PagedJob* jobs;
   int n_ctas;  // that there are slots for
+  float* chunk_o;
+  float2* chunk_ml;
+  PagedChunkJob* chunk_jobs;
+  int n_chunk_ctas;
 };
 
 template <typename... P, typename... A>
@@ -44,6 +54,9 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int head_
                                 cudaStream_t st, bool pdl);
 cudaError_t launch_paged_decode(const PagedAttnParams& p, const PagedPartials& part, int dtype,
                                 int head_dim, int n_sm, cudaStream_t st, bool pdl);
+cudaError_t prepare_paged_chunk16();
+cudaError_t launch_paged_chunk16(const PagedAttnParams& p, const PagedPartials& part, int dtype,
+                                 int head_dim, int n_sm, cudaStream_t st, bool pdl);
 cudaError_t launch_paged_chunks(const PagedAttnParams& p, int dtype, int head_dim,
                                 cudaStream_t st, bool pdl);
 
