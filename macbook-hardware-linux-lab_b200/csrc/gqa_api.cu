@@ -763,6 +763,7 @@ int gqa_create(const gqa_config* cfg, int device, gqa_ctx** out) {
   // graphs never see them move.
   if (e == cudaSuccess) e = prepare_paged_decode();
   if (e == cudaSuccess) e = prepare_paged_chunk16();
+  if (e == cudaSuccess) e = prepare_sample();
   if (e == cudaSuccess) e = alloc_paged(c, group);
   if (e == cudaSuccess) {
     // rotations per position, in 64 bits (the paged operators reach far positions)
@@ -1775,14 +1776,15 @@ int gqa_sample(gqa_ctx* c, gqa_stream_t stream, int n_rows, int vocab, int dtype
   p.vocab = vocab;
   int bits = 0;
   while ((1 << bits) < vocab) ++bits;
-  p.wshift = 62 - bits;  // a row's weights add up to at most 2^62
+  // a row's weights add up to at most 2^62, one weight to at most 2^50
+  p.wshift = std::min(62 - bits, 50);
   p.temperature = temperature;
   p.top_k = top_k;
   p.top_p = top_p;
   p.min_p = min_p;
   p.uniform = uniform;
   p.tokens = tokens;
-  GQA_CUDA(launch_sample(p, dtype, (cudaStream_t)stream, c->pdl != 0));
+  GQA_CUDA(launch_sample(p, dtype, c->n_sm, (cudaStream_t)stream, c->pdl != 0));
   return GQA_OK;
 }
 

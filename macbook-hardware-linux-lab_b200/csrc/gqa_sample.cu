@@ -8,13 +8,26 @@
 // w = exp((x - max) / temperature), every filter keeps a prefix of that order:
 // top-k the first k, top-p the shortest prefix whose weight reaches p times what
 // top-k kept, min-p the weights of at least min_p.  So no sort is needed, only
-// the last key that is kept and how many of its ties are, found by radix
-// selection over counts and over weights.  The token is then the first, in index
-// order, whose cumulative kept weight exceeds u times the total.
+// the last element that is kept, as the pair (logit, index): `ord` below.  The
+// token is then the first, in index order, whose cumulative kept weight exceeds
+// u times the total.
 //
-// Weights are summed as integers (fixed point, 2^-wshift of the largest weight):
-// a sum is exact in any order, so neither the order of atomics nor the split of
-// a row over threads can change a token.
+// Weights are formed in 64 bits and summed as integers (units of 2^-wshift of the
+// largest weight): a sum is exact in any order, so neither the order of atomics nor
+// the split of a row over threads can change a token.  Logits whose weight rounds to
+// zero in these units take part in nothing.
+//
+// A row belongs to a cluster of CTAs, each with a contiguous slice of it in shared
+// memory (logits past what fits are read again from memory), so a row is read from
+// memory once.  The last kept element is found in two steps: a histogram over 2048
+// equal steps of the exponent (they hold few elements each, wherever the logits lie,
+// and equal logits fall together), merged over the cluster by reads of the other CTAs'
+// shared memory, gives the step; its few elements are listed and ranked by comparing all
+// pairs.  Should a step hold more than the list takes (a high temperature, many ties),
+// the step is cut again by the pair's 64 bits.  For top-p the histogram holds weights
+// rounded to 14 bits; they only propose the step, which the exact sums confirm or move.
+#include <algorithm>
+
 #include <math_constants.h>
 
 #include "gqa_paged.cuh"
@@ -22,231 +35,655 @@
 
 namespace gqa {
 
-constexpr int kSampleThreads = 1024;
+namespace {
 
-// Keys in the order of the logits: larger logit, larger key; -0 as 0, NaN as -inf.
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;       // four per thread
+constexpr int kList = 512;
+constexpr int kMaxCluster = 8;
+constexpr int kBlock = kThreads * 4;  // elements of one turn of the CTA's threads
+
+using u64 = unsigned long long;
+
+struct alignas(16) Shared {  // (the slice of the row follows it)
+  union {
+    uint32_t hist[kBins];
+    u64 sums[kBins / 2];  // for the pick: weights of 128 elements each
+  };
+  u64 list_ord[kList], list_w[kList];  // this CTA's elements of the step
+  u64 all_ord[kList], all_w[kList];    // the cluster's
+  u64 x[2][4];                         // values exchanged over the cluster
+  u64 got[kMaxCluster][4];
+  u64 red[kWarps][4];
+  double pow2[64];                     // 2^(j / 64)
+  u64 found_before, cut;
+  int found;
+  uint32_t n_list;
+};
+
+// Keys in the order of the logits: larger logit, larger key.
 __device__ __forceinline__ uint32_t logit_key(float x) {
-  if (x != x) x = -CUDART_INF_F;
-  const uint32_t u = __float_as_uint(x + 0.0f);
+  const uint32_t u = __float_as_uint(x);
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
+// -0 as 0, NaN as -inf.
+__device__ __forceinline__ float clean(float x) { return x != x ? -CUDART_INF_F : x + 0.0f; }
 
-struct RowRule {
-  double inv_t, scale;  // 1 / temperature, 2^wshift
-  float top;            // largest logit
-};
-
-// The weight of a logit relative to the largest one.
-__device__ __forceinline__ double weight_of(float x, const RowRule& r) {
-  if (x == r.top) return 1.0;  // (also where the largest is infinite)
-  if (!(x > -CUDART_INF_F) || r.top == CUDART_INF_F) return 0.0;
-  return exp(((double)x - (double)r.top) * r.inv_t);
+__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
-__device__ __forceinline__ unsigned long long fixed_weight(float x, const RowRule& r) {
-  return (unsigned long long)(weight_of(x, r) * r.scale + 0.5);
+__device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-// Exclusive scan over the block's threads; *total gets the sum.
-__device__ unsigned long long block_scan(unsigned long long v, unsigned long long* total) {
-  __shared__ unsigned long long part[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long x = v;
+__device__ __forceinline__ u64 warp_sum(u64 x) {
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long y = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) part[warp] = x;
-  __syncthreads();
-  unsigned long long before = 0, sum = 0;
-  for (int w = 0; w < kSampleThreads / 32; ++w) {
-    if (w < warp) before += part[w];
-    sum += part[w];
-  }
-  *total = sum;
-  return before + x - v;
+  for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleParams p) {
-  __shared__ unsigned long long hist[256];
-  __shared__ unsigned long long s_best, s_sum;
-  __shared__ uint32_t s_bin;
-  __shared__ unsigned long long s_before;
-  const int row = blockIdx.x, tid = threadIdx.x, n = p.vocab;
-  const T* x = static_cast<const T*>(p.logits) + (long long)row * p.logits_stride;
+struct Row {
+  const SampleParams& p;
+  Shared& sm;
+  const T* logits;  // of the slice
+  const float* held;
+  int lo, n, n_held;  // the slice's first index, its elements, those in shared memory
+  int rank, ranks, tid, lane, warp, turn = 0;
+  float top;          // largest logit
+  u64 top_ord;
+  float c2;           // twice log2(e) / temperature, for the steps
+  double ct;          // log2(e) / temperature
+  float range;        // steps cover weights down to 2^-range
+  double scale;       // 2^wshift
+  float min_p;
+
+  __device__ __forceinline__ u64 ord(float x, int i) const {
+    return (u64)logit_key(x) << 32 | (0xffffffffu - (uint32_t)(lo + i));
+  }
+
+  // f(x, i) for the elements of the slice, four at a time per thread; whole warps take part.
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    for (int b = 0; b < n; b += kBlock) {
+      const int i = b + 4 * tid;
+      float v[4];
+      get4(i, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(v[e], i + e);
+    }
+  }
+  __device__ __forceinline__ void get4(int i, float (&v)[4]) const {
+    if (i < n_held) {  // (n_held is a multiple of 4, padded with -inf)
+      const float4 x = *reinterpret_cast<const float4*>(held + i);
+      v[0] = x.x;
+      v[1] = x.y;
+      v[2] = x.z;
+      v[3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = i + e < n ? clean(Elem<T>::get(logits[i + e])) : -CUDART_INF_F;
+    }
+  }
+
+  // log2 of top's weight over x's, and the step it falls in (kBins: beyond every weight).
+  // Non-decreasing in falling x, so steps cut the sorted order; halves keep the difference
+  // of two far logits finite.
+  __device__ __forceinline__ int step_of(float x, float& d) const {
+    d = x == top ? 0.f : (0.5f * top - 0.5f * x) * c2;
+    return d < range ? min((int)(d * (kBins / range)), kBins - 1) : kBins;
+  }
+
+  // The weight in 64 bits: 2^t as 2^(k/64) times the series of the rest (|rest| <= 2^-7 ln 2;
+  // Tang's table method), and in units of 2^-wshift.
+  __device__ __forceinline__ u64 weight(float x, double& w) const {
+    w = 1.0;
+    if (x == top) return (u64)scale;
+    const double t = ((double)x - (double)top) * ct;
+    w = 0.0;
+    if (!(t > -1000.0) || top == CUDART_INF_F) return 0;
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
+    const double km = fma(t, 64.0, magic);
+    const int k = __double2loint(km);
+    const double y = fma(km - magic, -1.0 / 64.0, t) * 0.693147180559945309;
+    double q = fma(y, 1.0 / 120.0, 1.0 / 24.0);
+    q = fma(q, y, 1.0 / 6.0);
+    q = fma(q, y, 0.5);
+    q = fma(q, y, 1.0);
+    q *= y;
+    const double b = sm.pow2[k & 63];
+    const double m = fma(b, q, b);
+    w = __hiloint2double(__double2hiint(m) + ((k >> 6) << 20), __double2loint(m));
+    // (a product below 2^52 plus 2^52 holds the rounded integer in its low bits)
+    return __double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+
+  // Sums (or, for `largest`, maxima) of four values over the block.
+  template <bool kMax>
+  __device__ void block_reduce(u64 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        const u64 y = __shfl_xor_sync(0xffffffffu, v[j], d);
+        v[j] = kMax ? (y > v[j] ? y : v[j]) : v[j] + y;
+      }
+    __syncthreads();
+    if (lane < 4) sm.red[warp][lane] = lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u64 x = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        const u64 y = sm.red[w][j];
+        x = kMax ? (y > x ? y : x) : x + y;
+      }
+      v[j] = x;
+    }
+  }
+
+  // Every CTA's four values into sm.got[rank] (a cluster barrier; what a CTA wrote to its
+  // shared memory before it, the others may read after it).  The two places alternate: a CTA
+  // is past the next barrier only when all have read this one's.
+  __device__ void exchange(const u64 (&v)[4]) {
+    u64* mine = sm.x[turn & 1];
+    if (tid < 4) mine[tid] = tid == 0 ? v[0] : tid == 1 ? v[1] : tid == 2 ? v[2] : v[3];
+    __syncwarp();
+    cluster_sync();
+    if (tid < ranks * 4) sm.got[tid >> 2][tid & 3] = ld_cluster_u64(cluster_map(mine + (tid & 3), tid >> 2));
+    __syncthreads();
+    ++turn;
+  }
+  __device__ __forceinline__ u64 total(int j) const {
+    u64 x = 0;
+    for (int r = 0; r < ranks; ++r) x += sm.got[r][j];
+    return x;
+  }
+
+  __device__ void clear_hist() {
+    *reinterpret_cast<uint4*>(&sm.hist[4 * tid]) = make_uint4(0, 0, 0, 0);
+    if (tid == 0) sm.n_list = 0;
+    __syncthreads();
+  }
+
+  // This thread's four steps of the cluster's histogram (after a barrier).
+  __device__ void merged(u64 (&h)[4]) {
+    h[0] = h[1] = h[2] = h[3] = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const uint4 v = ld_cluster_v4(cluster_map(&sm.hist[4 * tid], r));
+      h[0] += v.x;
+      h[1] += v.y;
+      h[2] += v.z;
+      h[3] += v.w;
+    }
+  }
+
+  // The step at which the running sum of h reaches `want` (below zero: that share of the
+  // total), the sum before it and the total.
+  __device__ int find_step(const double (&h)[4], double want, double& before, double& all) {
+    __syncthreads();
+    double mine = h[0] + h[1] + h[2] + h[3], incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    double* red = reinterpret_cast<double*>(sm.red);
+    if (lane == 31) red[warp] = incl;
+    if (tid == 0) sm.found = -1;
+    __syncthreads();
+    double base = 0.0;
+    all = 0.0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) base += red[w];
+      all += red[w];
+    }
+    if (want < 0.0) want = -want * all;
+    double run = base + incl - mine;
+    // The last non-empty step before which the sum is below `want`: unlike a test of both
+    // ends, this always names one, however the sums are rounded.
+    int at = -1;
+    double at_before = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (h[j] > 0.0 && run < want) {
+        at = 4 * tid + j;
+        at_before = run;
+      }
+      run += h[j];
+    }
+    if (at >= 0) atomicMax(&sm.found, at);
+    __syncthreads();
+    if (at >= 0 && sm.found == at) *reinterpret_cast<double*>(&sm.found_before) = at_before;
+    __syncthreads();
+    before = *reinterpret_cast<double*>(&sm.found_before);
+    return sm.found;
+  }
+
+  // The cluster's lists into sm.all_*; its elements.
+  __device__ void collect(bool weights) {
+    int at = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const int c = (int)sm.got[r][3];
+      for (int i = tid; i < c; i += kThreads) {
+        sm.all_ord[at + i] = ld_cluster_u64(cluster_map(&sm.list_ord[i], r));
+        if (weights) sm.all_w[at + i] = ld_cluster_u64(cluster_map(&sm.list_w[i], r));
+      }
+      at += c;
+    }
+    __syncthreads();
+  }
+
+  // Element k (from 1) of the sorted row, as an ord; 0 if fewer have a weight.
+  __device__ u64 find_kth(int k) {
+    clear_hist();
+    each([&](float x, int) {
+      float d;
+      const int s = step_of(x, d);
+      if (s < kBins) atomicAdd(&sm.hist[s], 1u);
+    });
+    u64 v[4] = {0, 0, 0, 0};
+    __syncthreads();
+    exchange(v);
+    u64 h[4];
+    merged(h);
+    double hd[4] = {(double)h[0], (double)h[1], (double)h[2], (double)h[3]};
+    double before, all;
+    int step = find_step(hd, k, before, all);
+    if (all <= k) {
+      __syncthreads();
+      cluster_sync();  // (the next step reuses the histograms that the other CTAs may be reading)
+      return 0;
+    }
+    double want = k - before;     // rank within the interval
+    u64 first = 0, last = ~0ull;  // ords of the interval
+    bool by_step = true;
+    // (each turn narrows the interval to one of 2048 parts: 64 bits take six)
+    for (int guard = 0; guard < 16; ++guard) {
+      u64 mm[4] = {0, 0, 0, 0};  // largest ord, largest ~ord
+      each([&](float x, int i) {
+        const u64 o = ord(x, i);
+        float d;
+        if (by_step ? step_of(x, d) == step : o >= first && o <= last) {
+          const uint32_t at = atomicAdd(&sm.n_list, 1u);
+          if (at < kList) sm.list_ord[at] = o;
+          if (o > mm[0]) mm[0] = o;
+          if (~o > mm[1]) mm[1] = ~o;
+        }
+      });
+      block_reduce<true>(mm);
+      mm[3] = sm.n_list;
+      exchange(mm);
+      const u64 n = total(3);
+      if (n <= kList) {
+        collect(false);
+        for (int i = tid; i < (int)n; i += kThreads) {
+          const u64 o = sm.all_ord[i];
+          int at = 0;
+          for (int j = 0; j < (int)n; ++j) at += sm.all_ord[j] > o;
+          if (at == (int)want - 1) sm.cut = o;
+        }
+        __syncthreads();
+        return sm.cut;
+      }
+      narrow(first, last);
+      by_step = false;
+      const int shift = max(0, 53 - __clzll(last - first));  // (last - first) >> shift < kBins
+      clear_hist();
+      each([&](float x, int i) {
+        const u64 o = ord(x, i);
+        if (o >= first && o <= last) atomicAdd(&sm.hist[(last - o) >> shift], 1u);
+      });
+      __syncthreads();
+      exchange(v);
+      merged(h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) hd[j] = (double)h[j];
+      const int b = find_step(hd, want, before, all);
+      want -= before;
+      last -= (u64)b << shift;
+      if (last - first >> shift) first = last - ((1ull << shift) - 1);
+    }
+    return 0;
+  }
+
+  // [first, last] from the largest ord and the largest complement that were exchanged.
+  __device__ void narrow(u64& first, u64& last) {
+    u64 hi = 0, lo_c = 0;
+    for (int r = 0; r < ranks; ++r) {
+      if (sm.got[r][0] > hi) hi = sm.got[r][0];
+      if (sm.got[r][1] > lo_c) lo_c = sm.got[r][1];
+    }
+    last = hi;
+    first = ~lo_c;
+    __syncthreads();
+  }
+
+  // The last element of the shortest prefix, among the ords from `cut` up, whose weight
+  // reaches share times theirs.
+  __device__ u64 find_share(u64 cut, double share) {
+    if (!(share > 0.0)) return top_ord;
+    clear_hist();
+    const float width = range / kBins;
+    each([&](float x, int i) {
+      float d;
+      const int s = step_of(x, d);
+      if (s < kBins && ord(x, i) >= cut)
+        atomicAdd(&sm.hist[s], (uint32_t)(exp2f(s * width - d) * 16384.f + 0.5f));
+    });
+    u64 v[4] = {0, 0, 0, 0};
+    __syncthreads();
+    exchange(v);
+    u64 h[4];
+    merged(h);
+    double hd[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) hd[j] = (double)h[j] * exp2f(-(4 * tid + j) * width);
+    double unused, all;
+    int step = find_step(hd, -share, unused, all);
+    u64 first = cut, last = ~0ull;  // the interval, cut into steps
+    int shift = -1;                 // -1: by exponent
+    u64 above = 0;                  // exact weight of the kept elements before the interval
+    double target = -1.0;
+    for (int guard = 0; guard < 4 * kBins; ++guard) {
+      if (tid == 0) sm.n_list = 0;
+      __syncthreads();
+      u64 s[4] = {0, 0, 0, 0};  // weight of the interval, before the step, of the step
+      each([&](float x, int i) {
+        const u64 o = ord(x, i);
+        if (o < first || o > last) return;
+        int b;
+        if (shift < 0) {
+          float d;
+          b = step_of(x, d);
+          if (b == kBins) return;
+        } else {
+          b = (int)((last - o) >> shift);
+        }
+        if (target >= 0.0 && b > step) return;
+        double w64;
+        const u64 w = weight(x, w64);
+        s[0] += w;
+        if (b < step) s[1] += w;
+        if (b == step) {
+          s[2] += w;
+          const uint32_t at = atomicAdd(&sm.n_list, 1u);
+          if (at < kList) {
+            sm.list_ord[at] = o;
+            sm.list_w[at] = w;
+          }
+        }
+      });
+      block_reduce<false>(s);
+      s[3] = sm.n_list;
+      exchange(s);
+      if (target < 0.0) target = share * (double)total(0);
+      const u64 before = above + total(1), in = total(2), n = total(3);
+      const bool early = (double)before >= target, late = (double)(before + in) < target;
+      if (early || late) {
+        // the 14-bit weights were too coarse: the next non-empty step that way
+        int other = -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int b = 4 * tid + j;
+          if (h[j] == 0) continue;
+          if (early && b < step) other = b;                 // the last before
+          if (late && b > step && other < 0) other = kBins - b;  // the first after
+        }
+        if (tid == 0) sm.found = -1;
+        __syncthreads();
+        atomicMax(&sm.found, other);
+        __syncthreads();
+        if (sm.found < 0) return late ? 0 : top_ord;
+        step = late ? kBins - sm.found : sm.found;
+        __syncthreads();
+        continue;
+      }
+      if (n <= kList) {
+        collect(true);
+        for (int i = tid; i < (int)n; i += kThreads) {
+          const u64 o = sm.all_ord[i];
+          u64 incl = before;
+          for (int j = 0; j < (int)n; ++j) incl += sm.all_ord[j] >= o ? sm.all_w[j] : 0;
+          if ((double)incl >= target && (double)(incl - sm.all_w[i]) < target) sm.cut = o;
+        }
+        __syncthreads();
+        return sm.cut;
+      }
+      // Too many for the list: cut the step by the ords it spans.
+      u64 mm[4] = {0, 0, 0, 0};
+      each([&](float x, int i) {
+        const u64 o = ord(x, i);
+        if (o < first || o > last) return;
+        float d;
+        if ((shift < 0 ? step_of(x, d) : (int)((last - o) >> shift)) != step) return;
+        if (o > mm[0]) mm[0] = o;
+        if (~o > mm[1]) mm[1] = ~o;
+      });
+      block_reduce<true>(mm);
+      exchange(mm);
+      narrow(first, last);
+      above = before;
+      shift = max(0, 53 - __clzll(last - first));
+      clear_hist();
+      double most;
+      weight(key_logit((uint32_t)(last >> 32)), most);
+      const float unit = (float)(16384.0 / most);
+      each([&](float x, int i) {
+        const u64 o = ord(x, i);
+        if (o < first || o > last) return;
+        double w;
+        weight(x, w);
+        atomicAdd(&sm.hist[(last - o) >> shift], (uint32_t)((float)w * unit + 0.5f));
+      });
+      __syncthreads();
+      exchange(v);
+      merged(h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) hd[j] = (double)h[j];
+      step = find_step(hd, fmax((target - (double)above) / scale * unit, 0.5), unused, all);
+    }
+    return cut;
+  }
+
+  // The first index whose cumulative kept weight exceeds u times the total; the CTA that
+  // holds it writes it.
+  __device__ void pick(u64 cut, float u, int* token) {
+    const auto kept = [&](float x, int i) {
+      const u64 o = ord(x, i);
+      if (o < cut) return 0ull;
+      double w64;
+      const u64 w = weight(x, w64);
+      return w64 >= (double)min_p || o == top_ord ? w : 0ull;
+    };
+    u64 v[4] = {0, 0, 0, 0};
+    for (int b = 0; b < n; b += kBlock) {
+      float x[4];
+      get4(b + 4 * tid, x);
+      u64 w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w += kept(x[e], b + 4 * tid + e);
+      w = warp_sum(w);
+      if (lane == 0) {
+        sm.sums[b / kBlock * kWarps + warp] = w;
+        v[0] += w;
+      }
+    }
+    block_reduce<false>(v);
+    exchange(v);
+    u64 before = 0, all = 0;
+    for (int r = 0; r < ranks; ++r) {
+      if (r < rank) before += sm.got[r][0];
+      all += sm.got[r][0];
+    }
+    u = u > 0.f ? u : 0.f;
+    const double ut = (double)u * (double)all;
+    const u64 target = ut < (double)all ? (u64)ut : all - 1;
+    if (warp != 0 || target < before || target >= before + sm.got[rank][0]) return;
+    // Lane by lane: the entry of sums, then the element of its 128.
+    const int entries = (n + kBlock - 1) / kBlock * kWarps;
+    int entry = 0;
+    for (int e0 = 0; e0 < entries; e0 += 32) {
+      const u64 w = e0 + lane < entries ? sm.sums[e0 + lane] : 0;
+      u64 incl = w;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, before + incl > target);
+      if (over) {
+        const int l = __ffs(over) - 1;
+        entry = e0 + l;
+        before += __shfl_sync(0xffffffffu, incl - w, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    const int i = entry / kWarps * kBlock + entry % kWarps * 128 + 4 * lane;
+    float x[4];
+    get4(i, x);
+    u64 w[4], mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mine += w[e] = kept(x[e], i + e);
+    u64 incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    u64 run = before + incl - mine;
+    if (run <= target && run + mine > target) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (run <= target && run + w[e] > target) *token = lo + i + e;
+        run += w[e];
+      }
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+    sample_kernel(const SampleParams p, const int ranks, const int per, const int room) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  Shared& sm = *reinterpret_cast<Shared*>(smem_raw);
+  float* held = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x % ranks, row = blockIdx.x / ranks;
+  const int lo = min(rank * per, p.vocab), n = min(per, p.vocab - lo);
+  const T* x = static_cast<const T*>(p.logits) + (long long)row * p.logits_stride + lo;
+  if (tid < 64) sm.pow2[tid] = exp2(tid / 64.0);
   pdl_wait();
+
+  // The slice into shared memory, and its largest logit (the first of them).
+  static_assert(sizeof(Shared) % 16 == 0, "the slice is read 16 bytes at a time");
+  const int n_held = min((n + 3) & ~3, room);
+  float best = -CUDART_INF_F;
+  int at = 0;
+#pragma unroll 8
+  for (int i = tid; i < n; i += kThreads) {
+    const float v = clean(Elem<T>::get(x[i]));
+    if (i < n_held) held[i] = v;
+    if (v > best) {
+      best = v;
+      at = i;
+    }
+  }
+  for (int i = n + tid; i < n_held; i += kThreads) held[i] = -CUDART_INF_F;
   const float temp = p.temperature ? p.temperature[row] : 1.f;
   const int k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
-  const float min_p = p.min_p ? p.min_p[row] : 0.f;
-
-  // the largest logit, the first of its ties
-  if (tid == 0) s_best = 0;
-  __syncthreads();
-  unsigned long long best = 0;
-  for (int i = tid; i < n; i += kSampleThreads) {
-    const unsigned long long b =
-        (unsigned long long)logit_key(Elem<T>::get(x[i])) << 32 | (0xffffffffu - (uint32_t)i);
-    if (b > best) best = b;
-  }
-  atomicMax(&s_best, best);
-  __syncthreads();
-  best = s_best;
-  const uint32_t top_key = (uint32_t)(best >> 32);
-  const int first = (int)(0xffffffffu - (uint32_t)best);
-  RowRule r;
-  r.top = key_logit(top_key);
-  if (!(temp > 0.f) || r.top == -CUDART_INF_F) {
-    if (tid == 0) p.tokens[row] = r.top == -CUDART_INF_F ? 0 : first;
+  Row<T> r{p, sm, x, held, lo, n, n_held, rank, ranks, tid, lane, warp};
+  u64 v[4] = {r.ord(best, at), 0, 0, 0};
+  if (best == -CUDART_INF_F) v[0] = 0;
+  r.template block_reduce<true>(v);
+  r.exchange(v);
+  u64 top_ord = 0;
+  for (int i = 0; i < ranks; ++i) top_ord = max(top_ord, sm.got[i][0]);
+  const int first = (int)(0xffffffffu - (uint32_t)top_ord);
+  if (top_ord == 0 || !(temp > 0.f)) {  // nothing above -inf, or greedy
+    if (rank == 0 && tid == 0) p.tokens[row] = top_ord == 0 ? 0 : first;
+    __syncthreads();
+    cluster_sync();
     return;
   }
-  r.inv_t = 1.0 / (double)temp;
+  r.top = key_logit((uint32_t)(top_ord >> 32));
+  r.top_ord = top_ord;
+  r.ct = 1.4426950408889634074 / (double)temp;
+  r.c2 = (float)(2.0 * r.ct);
+  r.range = (float)(p.wshift + 2);
   r.scale = (double)(1ull << p.wshift);
-
-  // The last kept key and how many of its ties are kept (all keys to begin with).
-  uint32_t cut = 0;
-  unsigned long long ties = ~0ull;
-  if (k > 0 && k < n) {
-    uint32_t prefix = 0;
-    unsigned long long before = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int b = tid; b < 256; b += kSampleThreads) hist[b] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kSampleThreads) {
-        const uint32_t key = logit_key(Elem<T>::get(x[i]));
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-          atomicAdd(&hist[(key >> shift) & 255], 1ull);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int b = 255;
-        while (b > 0 && before + hist[b] < (unsigned long long)k) before += hist[b--];
-        s_bin = b;
-        s_before = before;
-      }
-      __syncthreads();
-      prefix |= s_bin << shift;
-      before = s_before;
-    }
-    cut = prefix;
-    ties = (unsigned long long)k - before;
-  }
-  if (top_p < 1.f) {
-    const unsigned long long cut_mass = ties == ~0ull ? 0 : ties * fixed_weight(key_logit(cut), r);
-    if (tid == 0) s_sum = 0;
-    __syncthreads();
-    unsigned long long sum = 0;
-    for (int i = tid; i < n; i += kSampleThreads) {
-      const float v = Elem<T>::get(x[i]);
-      const uint32_t key = logit_key(v);
-      if (key > cut || ties == ~0ull) sum += fixed_weight(key_logit(key), r);
-    }
-    atomicAdd(&s_sum, sum);
-    __syncthreads();
-    const double target = (double)top_p * (double)(s_sum + cut_mass);
-    uint32_t prefix = 0;
-    unsigned long long before = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int b = tid; b < 256; b += kSampleThreads) hist[b] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kSampleThreads) {
-        const uint32_t key = logit_key(Elem<T>::get(x[i]));
-        if ((key > cut || ties == ~0ull) &&
-            (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
-          atomicAdd(&hist[(key >> shift) & 255], fixed_weight(key_logit(key), r));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        if (cut_mass && (shift == 24 || (cut >> (shift + 8)) == (prefix >> (shift + 8))))
-          hist[(cut >> shift) & 255] += cut_mass;
-        // down to the first bin whose weight reaches the target (or, should
-        // rounding leave it unreached, the last bin with any weight)
-        int b = 255, last = -1;
-        unsigned long long at_last = before;
-        for (; b >= 0; --b) {
-          if (!hist[b]) continue;
-          last = b;
-          at_last = before;
-          if ((double)(before + hist[b]) >= target) break;
-          before += hist[b];
-        }
-        s_bin = last;
-        s_before = at_last;
-      }
-      __syncthreads();
-      prefix |= s_bin << shift;
-      before = s_before;
-    }
-    // ties of the last key: the fewest, at least one, that reach the target
-    const unsigned long long w = fixed_weight(key_logit(prefix), r);
-    unsigned long long need = 1;
-    if (w && (double)(before + w) < target) {
-      need = (unsigned long long)ceil((target - (double)before) / (double)w);
-      if (need > 1 && (double)(before + (need - 1) * w) >= target) --need;
-      if ((double)(before + need * w) < target) ++need;
-    }
-    ties = prefix == cut && need > ties ? ties : need;
-    cut = prefix;
-  }
-
-  // Cumulative weights in index order: a contiguous range of the row per thread.
-  const int per = (n + kSampleThreads - 1) / kSampleThreads;
-  const int lo = min(tid * per, n), hi = min(lo + per, n);
-  unsigned long long mine = 0;
-  for (int i = lo; i < hi; ++i) mine += logit_key(Elem<T>::get(x[i])) == cut;
-  unsigned long long unused;
-  const unsigned long long tie0 = block_scan(mine, &unused);
-  const auto walk = [&](auto&& f) {
-    unsigned long long tie = tie0;
-    for (int i = lo; i < hi; ++i) {
-      const uint32_t key = logit_key(Elem<T>::get(x[i]));
-      bool keep = key > cut || (key == cut && tie < ties);
-      tie += key == cut;
-      if (!keep) continue;
-      const float v = key_logit(key);
-      if (i != first && weight_of(v, r) < (double)min_p) continue;
-      const unsigned long long w = fixed_weight(v, r);
-      if (w && !f(i, w)) break;
-    }
-  };
-  unsigned long long weight = 0, total;
-  walk([&](int, unsigned long long w) { weight += w; return true; });
-  const unsigned long long before = block_scan(weight, &total);
-  float u = p.uniform[row];
-  u = u > 0.f ? u : 0.f;
-  // the token is the first whose cumulative weight exceeds u * total (the last, should u be
-  // 1 or more)
-  const double ut = (double)u * (double)total;
-  const unsigned long long target = ut < (double)total ? (unsigned long long)ut : total - 1;
-  if (before <= target && before + weight > target) {
-    unsigned long long c = before;
-    walk([&](int i, unsigned long long w) {
-      c += w;
-      if (c <= target) return true;
-      p.tokens[row] = i;
-      return false;
-    });
-  }
+  r.min_p = p.min_p ? p.min_p[row] : 0.f;
+  u64 cut = 0;
+  if (k > 0 && k < p.vocab) cut = r.find_kth(k);
+  if (top_p < 1.f) cut = max(cut, r.find_share(cut, (double)top_p));
+  r.pick(cut, p.uniform[row], p.tokens + row);
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while another may read its shared memory
 }
 
-cudaError_t launch_sample(const SampleParams& p, int dtype, cudaStream_t st, bool pdl) {
+template <typename T>
+cudaError_t launch_one(const SampleParams& p, int ranks, int per, int room, size_t smem,
+                       cudaStream_t st, bool pdl) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.n_rows);
-  cfg.blockDim = dim3(kSampleThreads);
+  cfg.gridDim = dim3((unsigned)(p.n_rows * ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  if (dtype == kDtypeF32) return cudaLaunchKernelEx(&cfg, sample_kernel<float>, p);
-  if (dtype == kDtypeBf16) return cudaLaunchKernelEx(&cfg, sample_kernel<__nv_bfloat16>, p);
-  return cudaLaunchKernelEx(&cfg, sample_kernel<__half>, p);
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p, ranks, per, room);
+}
+
+constexpr int kMaxSmem = 227 * 1024;
+
+}  // namespace
+
+cudaError_t prepare_sample() {
+  cudaError_t e = cudaFuncSetAttribute((const void*)sample_kernel<float>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute((const void*)sample_kernel<__nv_bfloat16>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute((const void*)sample_kernel<__half>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  return e;
+}
+
+cudaError_t launch_sample(const SampleParams& p, int dtype, int n_sm, cudaStream_t st, bool pdl) {
+  // CTAs per row: as many as let two CTAs share an SM with the whole row in shared memory, and
+  // more while the rows alone do not fill the SMs and a slice keeps the threads busy.
+  const int two = (kMaxSmem / 2 - 1024 - (int)sizeof(Shared)) / 4;  // logits that fit beside another CTA
+  int ranks = 1;
+  while (ranks < kMaxCluster &&
+         (p.vocab > two * ranks ||
+          ((long long)p.n_rows * ranks < 2 * n_sm && p.vocab > 2 * kBlock * ranks)))
+    ranks *= 2;
+  const int per = ((p.vocab + ranks - 1) / ranks + 3) & ~3;
+  const int room = std::min(per, (kMaxSmem - (int)sizeof(Shared)) / 4 & ~3);
+  const size_t smem = sizeof(Shared) + (size_t)room * 4;
+  if (dtype == kDtypeF32) return launch_one<float>(p, ranks, per, room, smem, st, pdl);
+  if (dtype == kDtypeBf16) return launch_one<__nv_bfloat16>(p, ranks, per, room, smem, st, pdl);
+  return launch_one<__half>(p, ranks, per, room, smem, st, pdl);
 }
 
 }  // namespace gqa

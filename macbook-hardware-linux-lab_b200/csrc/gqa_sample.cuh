@@ -18,6 +18,7 @@ struct SampleParams {
   int* tokens;              // [n_rows]
 };
 
-cudaError_t launch_sample(const SampleParams& p, int dtype, cudaStream_t st, bool pdl);
+cudaError_t prepare_sample();
+cudaError_t launch_sample(const SampleParams& p, int dtype, int n_sm, cudaStream_t st, bool pdl);
 
 }  // namespace gqa
