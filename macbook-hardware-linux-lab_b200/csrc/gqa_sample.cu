@@ -41,6 +41,8 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;       // four per thread
 constexpr int kList = 512;
+// A top_k up to which the row's first k are looked for by way of the threads' largest logits.
+constexpr int kSmallK = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kBlock = kThreads * 4;  // elements of one turn of the CTA's threads
 
@@ -49,9 +51,10 @@ using u64 = unsigned long long;
 struct alignas(16) Shared {  // (the slice of the row follows it)
   union {
     uint32_t hist[kBins];
-    u64 sums[kBins / 2];  // for the pick: weights of 128 elements each
+    u64 sums[kBins / 2 + kWarps];  // for the pick: weights of 128 elements each
   };
   u64 list_ord[kList], list_w[kList];  // this CTA's elements of the step
+  u64 over_ord[kList], over_w[kList];  // and those before it, while they fit
   u64 all_ord[kList], all_w[kList];    // the cluster's
   u64 x[2][4];                         // values exchanged over the cluster
   u64 got[kMaxCluster][4];
@@ -59,7 +62,7 @@ struct alignas(16) Shared {  // (the slice of the row follows it)
   double pow2[64];                     // 2^(j / 64)
   u64 found_before, cut;
   int found;
-  uint32_t n_list;
+  uint32_t n_list, n_over;
 };
 
 // Keys in the order of the logits: larger logit, larger key.
@@ -100,10 +103,12 @@ struct Row {
   int lo, n, n_held;  // the slice's first index, its elements, those in shared memory
   int rank, ranks, tid, lane, warp, turn = 0;
   float top;          // largest logit
+  bool infinite;      // it is infinite: only its equals have a weight, and the same one
   u64 top_ord;
   float c2;           // twice log2(e) / temperature, for the steps
   double ct;          // log2(e) / temperature
   float range;        // steps cover weights down to 2^-range
+  float per_step;     // kBins / range
   double scale;       // 2^wshift
   float min_p;
 
@@ -111,15 +116,42 @@ struct Row {
     return (u64)logit_key(x) << 32 | (0xffffffffu - (uint32_t)(lo + i));
   }
 
-  // f(x, i) for the elements of the slice, four at a time per thread; whole warps take part.
+  // f(x, i) for the elements of the slice, four at a time per thread.
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll 2
     for (int b = 0; b < n; b += kBlock) {
       const int i = b + 4 * tid;
       float v[4];
       get4(i, v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f(v[e], i + e);
+    }
+  }
+  // f(x, i, step, d, on) with the weights of the elements that f wants (`want` says which, by
+  // ord and step), computed for four elements side by side where a warp has any.
+  template <typename W, typename F>
+  __device__ __forceinline__ void each_weight(W&& want, F&& f) const {
+    for (int b = 0; b < n; b += kBlock) {
+      const int i = b + 4 * tid;
+      float v[4], d[4];
+      int s[4];
+      bool on[4], any = false;
+      get4(i, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e] = step_of(v[e], d[e]);
+        on[e] = s[e] < kBins && want(ord(v[e], i + e), s[e]);
+        any |= on[e];
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+      u64 w[4];
+      double w64[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = weight(v[e], on[e], w64[e]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (on[e]) f(i + e, ord(v[e], i + e), s[e], d[e], w[e], w64[e]);
     }
   }
   __device__ __forceinline__ void get4(int i, float (&v)[4]) const {
@@ -141,17 +173,16 @@ struct Row {
   // of two far logits finite.
   __device__ __forceinline__ int step_of(float x, float& d) const {
     d = x == top ? 0.f : (0.5f * top - 0.5f * x) * c2;
-    return d < range ? min((int)(d * (kBins / range)), kBins - 1) : kBins;
+    return d < range ? min((int)(d * per_step), kBins - 1) : kBins;
   }
 
   // The weight in 64 bits: 2^t as 2^(k/64) times the series of the rest (|rest| <= 2^-7 ln 2;
-  // Tang's table method), and in units of 2^-wshift.
-  __device__ __forceinline__ u64 weight(float x, double& w) const {
-    w = 1.0;
-    if (x == top) return (u64)scale;
-    const double t = ((double)x - (double)top) * ct;
-    w = 0.0;
-    if (!(t > -1000.0) || top == CUDART_INF_F) return 0;
+  // Tang's table method), and in units of 2^-wshift.  `on`: the logit is within the steps
+  // (others weigh nothing).  No branches, so that the four elements a thread has at a time
+  // go through the 64-bit pipe side by side.
+  __device__ __forceinline__ u64 weight(float x, bool on, double& w) const {
+    double t = ((double)(on ? x : top) - (double)top) * ct;
+    if (infinite) t = 0.0;
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
     const double km = fma(t, 64.0, magic);
     const int k = __double2loint(km);
@@ -164,8 +195,10 @@ struct Row {
     const double b = sm.pow2[k & 63];
     const double m = fma(b, q, b);
     w = __hiloint2double(__double2hiint(m) + ((k >> 6) << 20), __double2loint(m));
-    // (a product below 2^52 plus 2^52 holds the rounded integer in its low bits)
-    return __double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xfffffffffffffull;
+    // (a product of at most 2^50 plus 2^52 holds the rounded integer in its low bits)
+    const u64 bits = __double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xfffffffffffffull;
+    if (!on) w = 0.0;
+    return on ? bits : 0ull;
   }
 
   // Sums (or, for `largest`, maxima) of four values over the block.
@@ -212,19 +245,23 @@ struct Row {
 
   __device__ void clear_hist() {
     *reinterpret_cast<uint4*>(&sm.hist[4 * tid]) = make_uint4(0, 0, 0, 0);
-    if (tid == 0) sm.n_list = 0;
+    if (tid == 0) sm.n_list = sm.n_over = 0;
     __syncthreads();
   }
 
   // This thread's four steps of the cluster's histogram (after a barrier).
   __device__ void merged(u64 (&h)[4]) {
+    uint4 v[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      v[r] = r < ranks ? ld_cluster_v4(cluster_map(&sm.hist[4 * tid], r)) : make_uint4(0, 0, 0, 0);
     h[0] = h[1] = h[2] = h[3] = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const uint4 v = ld_cluster_v4(cluster_map(&sm.hist[4 * tid], r));
-      h[0] += v.x;
-      h[1] += v.y;
-      h[2] += v.z;
-      h[3] += v.w;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      h[0] += v[r].x;
+      h[1] += v[r].y;
+      h[2] += v[r].z;
+      h[3] += v[r].w;
     }
   }
 
@@ -270,18 +307,123 @@ struct Row {
     return sm.found;
   }
 
-  // The cluster's lists into sm.all_*; its elements.
-  __device__ void collect(bool weights) {
+  // Appends this thread's element to a list of the CTA.
+  __device__ __forceinline__ static void put(uint32_t& count, u64* list, u64 o) {
+    const uint32_t at = atomicAdd(&count, 1u);
+    if (at < kList) list[at] = o;
+  }
+
+  // The cluster's lists of the step into sm.all_* (counts in the exchange's last value: the
+  // step's elements low, those before it high).
+  __device__ void collect(bool weights, bool over) {
     int at = 0;
     for (int r = 0; r < ranks; ++r) {
-      const int c = (int)sm.got[r][3];
-      for (int i = tid; i < c; i += kThreads) {
-        sm.all_ord[at + i] = ld_cluster_u64(cluster_map(&sm.list_ord[i], r));
-        if (weights) sm.all_w[at + i] = ld_cluster_u64(cluster_map(&sm.list_w[i], r));
+      const int c = (int)(uint32_t)sm.got[r][3], o = over ? (int)(sm.got[r][3] >> 32) : 0;
+      for (int i = tid; i < c + o; i += kThreads) {
+        const u64* from = i < c ? &sm.list_ord[i] : &sm.over_ord[i - c];
+        sm.all_ord[at + i] = ld_cluster_u64(cluster_map(from, r));
+        if (weights) {
+          from = i < c ? &sm.list_w[i] : &sm.over_w[i - c];
+          sm.all_w[at + i] = ld_cluster_u64(cluster_map(from, r));
+        }
       }
-      at += c;
+      at += c + o;
     }
     __syncthreads();
+  }
+
+  // Whether the first k of the row are all among n collected elements, found by way of the
+  // threads' own largest logits: at least k elements are at or above the k-th largest of
+  // those, and few more where the logits are in no particular order.  One count per thread
+  // in place of one per logit.
+  __device__ bool gather_first(int k, float best, int& n) {
+    clear_hist();
+    float d;
+    const int mine = step_of(best, d);
+    if (mine < kBins) atomicAdd(&sm.hist[mine], 1u);
+    u64 v[4] = {0, 0, 0, 0};
+    __syncthreads();
+    exchange(v);
+    u64 h[4];
+    merged(h);
+    const double hd[4] = {(double)h[0], (double)h[1], (double)h[2], (double)h[3]};
+    double before, all;
+    const int step = find_step(hd, k, before, all);
+    const int upto = all < k ? kBins - 1 : step;  // (fewer: all that have a weight)
+    each([&](float x, int i) {
+      if (step_of(x, d) <= upto) put(sm.n_list, sm.list_ord, ord(x, i));
+    });
+    __syncthreads();
+    v[3] = min(sm.n_list, 1u << 30);
+    exchange(v);
+    const u64 count = total(3);
+    n = (int)count;
+    if (count > kList) {
+      __syncthreads();
+      cluster_sync();  // (the lists are reused)
+      return false;
+    }
+    return true;
+  }
+
+  // The token from n collected elements that hold all of the row's first k (and, with
+  // weights, all that top-p keeps, whose weight the target is).  By one CTA: ranks by
+  // comparing all pairs, prefixes by a scan, and the index order again by pairs.
+  __device__ void finish(int n, int k, bool weighed, double target, double share, float u,
+                         int* token) {
+    const int m = min(n, k);
+    for (int i = tid; i < n; i += kThreads) {  // (n <= kList: one element a thread)
+      const u64 o = sm.all_ord[i];
+      int at = 0;
+      for (int j = 0; j < n; ++j) at += sm.all_ord[j] > o;
+      u64 w;
+      double w64;
+      const float x = key_logit((uint32_t)(o >> 32));
+      float d;
+      w = weight(x, step_of(x, d) < kBins, w64);
+      sm.over_ord[at] = o;
+      // the weight with min_p's answer in the sign bit (weights stay below 2^50)
+      sm.over_w[at] = w | (u64)(!(w64 >= (double)min_p) && at > 0) << 63;
+    }
+    __syncthreads();
+    constexpr u64 kMask = ~0ull >> 1;
+    // cumulative weight in rank order, one rank a thread
+    static_assert(kList <= kThreads, "a thread per element");
+    const u64 w = tid < m ? sm.over_w[tid] & kMask : 0;
+    u64 incl = w;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, incl, s);
+      if (lane >= s) incl += y;
+    }
+    __syncthreads();
+    if (lane == 31) sm.red[warp][0] = incl;
+    __syncthreads();
+    u64 all = 0;
+    for (int j = 0; j < kWarps; ++j) {
+      if (j < warp) incl += sm.red[j][0];
+      all += sm.red[j][0];
+    }
+    if (!weighed) target = share * (double)all;
+    // rank i stays while the weight before it is below the target
+    const bool stays = tid < m && !(sm.over_w[tid] >> 63) &&
+                       (tid == 0 || !(share < 1.0) || (double)(incl - w) < target);
+    u64 mass[4] = {stays ? w : 0, 0, 0, 0};
+    // kept elements, for the index order
+    if (tid < n) {
+      sm.list_ord[tid] = stays ? 0xffffffffu - (uint32_t)sm.over_ord[tid] : 0xffffffffu;
+      sm.list_w[tid] = mass[0];
+    }
+    block_reduce<false>(mass);
+    u = u > 0.f ? u : 0.f;
+    const double ut = (double)u * (double)mass[0];
+    const u64 pick = ut < (double)mass[0] ? (u64)ut : mass[0] - 1;
+    if (stays && w) {
+      const u64 me = sm.list_ord[tid];
+      u64 run = 0;
+      for (int j = 0; j < m; ++j) run += sm.list_ord[j] <= me ? sm.list_w[j] : 0;
+      if (run > pick && run - w <= pick) *token = (int)me;
+    }
   }
 
   // Element k (from 1) of the sorted row, as an ord; 0 if fewer have a weight.
@@ -315,8 +457,7 @@ struct Row {
         const u64 o = ord(x, i);
         float d;
         if (by_step ? step_of(x, d) == step : o >= first && o <= last) {
-          const uint32_t at = atomicAdd(&sm.n_list, 1u);
-          if (at < kList) sm.list_ord[at] = o;
+          put(sm.n_list, sm.list_ord, o);
           if (o > mm[0]) mm[0] = o;
           if (~o > mm[1]) mm[1] = ~o;
         }
@@ -326,7 +467,7 @@ struct Row {
       exchange(mm);
       const u64 n = total(3);
       if (n <= kList) {
-        collect(false);
+        collect(false, false);
         for (int i = tid; i < (int)n; i += kThreads) {
           const u64 o = sm.all_ord[i];
           int at = 0;
@@ -370,20 +511,22 @@ struct Row {
   }
 
   // The last element of the shortest prefix, among the ords from `cut` up, whose weight
-  // reaches share times theirs.
-  __device__ u64 find_share(u64 cut, double share) {
+  // reaches share times theirs.  n > 0: instead, n elements that hold all of that prefix are
+  // collected, and `target` is the weight to reach.
+  __device__ u64 find_share(u64 cut, double share, int& n, double& target) {
+    n = 0;
     if (!(share > 0.0)) return top_ord;
     clear_hist();
     const float width = range / kBins;
-    each([&](float x, int i) {
-      float d;
-      const int s = step_of(x, d);
-      if (s < kBins && ord(x, i) >= cut)
-        atomicAdd(&sm.hist[s], (uint32_t)(exp2f(s * width - d) * 16384.f + 0.5f));
-    });
     u64 v[4] = {0, 0, 0, 0};
-    __syncthreads();
+    each_weight([&](u64 o, int) { return o >= cut; },
+                [&](int, u64, int b, float d, u64 w, double) {
+                  v[0] += w;
+                  atomicAdd(&sm.hist[b], (uint32_t)(exp2f(b * width - d) * 16384.f + 0.5f));
+                });
+    block_reduce<false>(v);
     exchange(v);
+    target = share * (double)total(0);
     u64 h[4];
     merged(h);
     double hd[4];
@@ -394,41 +537,40 @@ struct Row {
     u64 first = cut, last = ~0ull;  // the interval, cut into steps
     int shift = -1;                 // -1: by exponent
     u64 above = 0;                  // exact weight of the kept elements before the interval
-    double target = -1.0;
     for (int guard = 0; guard < 4 * kBins; ++guard) {
-      if (tid == 0) sm.n_list = 0;
+      if (tid == 0) sm.n_list = sm.n_over = 0;
       __syncthreads();
-      u64 s[4] = {0, 0, 0, 0};  // weight of the interval, before the step, of the step
-      each([&](float x, int i) {
-        const u64 o = ord(x, i);
-        if (o < first || o > last) return;
-        int b;
-        if (shift < 0) {
-          float d;
-          b = step_of(x, d);
-          if (b == kBins) return;
-        } else {
-          b = (int)((last - o) >> shift);
-        }
-        if (target >= 0.0 && b > step) return;
-        double w64;
-        const u64 w = weight(x, w64);
-        s[0] += w;
-        if (b < step) s[1] += w;
-        if (b == step) {
-          s[2] += w;
-          const uint32_t at = atomicAdd(&sm.n_list, 1u);
-          if (at < kList) {
-            sm.list_ord[at] = o;
-            sm.list_w[at] = w;
-          }
-        }
-      });
+      u64 s[4] = {0, 0, 0, 0};  // weight before the step, of the step
+      const auto part = [&](u64 o, int b) { return shift < 0 ? b : (int)((last - o) >> shift); };
+      each_weight([&](u64 o, int b) { return o >= first && o <= last && part(o, b) <= step; },
+                  [&](int, u64 o, int b, float, u64 w, double) {
+                    if (part(o, b) < step) {
+                      s[0] += w;
+                      if (shift < 0 && *(volatile uint32_t*)&sm.n_over < kList) {
+                        const uint32_t at = atomicAdd(&sm.n_over, 1u);
+                        if (at < kList) {
+                          sm.over_ord[at] = o;
+                          sm.over_w[at] = w;
+                        }
+                      }
+                    } else {
+                      s[1] += w;
+                      const uint32_t at = atomicAdd(&sm.n_list, 1u);
+                      if (at < kList) {
+                        sm.list_ord[at] = o;
+                        sm.list_w[at] = w;
+                      }
+                    }
+                  });
       block_reduce<false>(s);
-      s[3] = sm.n_list;
+      s[3] = sm.n_list | (u64)sm.n_over << 32;
       exchange(s);
-      if (target < 0.0) target = share * (double)total(0);
-      const u64 before = above + total(1), in = total(2), n = total(3);
+      const u64 before = above + total(0), in = total(1);
+      u64 n_in = 0, n_over = 0;
+      for (int r = 0; r < ranks; ++r) {
+        n_in += (uint32_t)sm.got[r][3];
+        n_over += sm.got[r][3] >> 32;
+      }
       const bool early = (double)before >= target, late = (double)(before + in) < target;
       if (early || late) {
         // the 14-bit weights were too coarse: the next non-empty step that way
@@ -437,24 +579,29 @@ struct Row {
         for (int j = 0; j < 4; ++j) {
           const int b = 4 * tid + j;
           if (h[j] == 0) continue;
-          if (early && b < step) other = b;                 // the last before
+          if (early && b < step) other = b;                      // the last before
           if (late && b > step && other < 0) other = kBins - b;  // the first after
         }
         if (tid == 0) sm.found = -1;
         __syncthreads();
         atomicMax(&sm.found, other);
         __syncthreads();
-        if (sm.found < 0) return late ? 0 : top_ord;
-        step = late ? kBins - sm.found : sm.found;
+        const int next = sm.found;
         __syncthreads();
+        if (next < 0) return late ? 0 : top_ord;
+        step = late ? kBins - next : next;
         continue;
       }
-      if (n <= kList) {
-        collect(true);
-        for (int i = tid; i < (int)n; i += kThreads) {
+      if (shift < 0 && n_in + n_over <= kList) {
+        n = (int)(n_in + n_over);
+        return 0;
+      }
+      if (n_in <= kList) {
+        collect(true, false);
+        for (int i = tid; i < (int)n_in; i += kThreads) {
           const u64 o = sm.all_ord[i];
           u64 incl = before;
-          for (int j = 0; j < (int)n; ++j) incl += sm.all_ord[j] >= o ? sm.all_w[j] : 0;
+          for (int j = 0; j < (int)n_in; ++j) incl += sm.all_ord[j] >= o ? sm.all_w[j] : 0;
           if ((double)incl >= target && (double)(incl - sm.all_w[i]) < target) sm.cut = o;
         }
         __syncthreads();
@@ -464,9 +611,9 @@ struct Row {
       u64 mm[4] = {0, 0, 0, 0};
       each([&](float x, int i) {
         const u64 o = ord(x, i);
-        if (o < first || o > last) return;
         float d;
-        if ((shift < 0 ? step_of(x, d) : (int)((last - o) >> shift)) != step) return;
+        const int b = step_of(x, d);
+        if (b == kBins || o < first || o > last || part(o, b) != step) return;
         if (o > mm[0]) mm[0] = o;
         if (~o > mm[1]) mm[1] = ~o;
       });
@@ -477,15 +624,13 @@ struct Row {
       shift = max(0, 53 - __clzll(last - first));
       clear_hist();
       double most;
-      weight(key_logit((uint32_t)(last >> 32)), most);
+      weight(key_logit((uint32_t)(last >> 32)), true, most);
       const float unit = (float)(16384.0 / most);
-      each([&](float x, int i) {
-        const u64 o = ord(x, i);
-        if (o < first || o > last) return;
-        double w;
-        weight(x, w);
-        atomicAdd(&sm.hist[(last - o) >> shift], (uint32_t)((float)w * unit + 0.5f));
-      });
+      each_weight([&](u64 o, int) { return o >= first && o <= last; },
+                  [&](int, u64 o, int, float, u64, double w) {
+                    atomicAdd(&sm.hist[(last - o) >> shift], (uint32_t)((float)w * unit + 0.5f));
+                  });
+      v[0] = 0;
       __syncthreads();
       exchange(v);
       merged(h);
@@ -499,24 +644,37 @@ struct Row {
   // The first index whose cumulative kept weight exceeds u times the total; the CTA that
   // holds it writes it.
   __device__ void pick(u64 cut, float u, int* token) {
-    const auto kept = [&](float x, int i) {
-      const u64 o = ord(x, i);
-      if (o < cut) return 0ull;
-      double w64;
-      const u64 w = weight(x, w64);
-      return w64 >= (double)min_p || o == top_ord ? w : 0ull;
+    // min_p's logits lie before the step of 2^-reach; the comparison itself is in 64 bits.
+    const float reach = min_p > 0.f ? -log2f(min_p) * 1.0001f + 0.01f : range;
+    const auto weights4 = [&](int i, const float (&x)[4], u64 (&w)[4]) {
+      bool on[4], any = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float d;
+        const u64 o = ord(x[e], i + e);
+        on[e] = step_of(x[e], d) < kBins && o >= cut && (d <= reach || o == top_ord);
+        any |= on[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = 0;
+      if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        double w64;
+        w[e] = weight(x[e], on[e], w64);
+        if (!(w64 >= (double)min_p) && ord(x[e], i + e) != top_ord) w[e] = 0;
+      }
     };
     u64 v[4] = {0, 0, 0, 0};
     for (int b = 0; b < n; b += kBlock) {
       float x[4];
+      u64 w[4];
       get4(b + 4 * tid, x);
-      u64 w = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w += kept(x[e], b + 4 * tid + e);
-      w = warp_sum(w);
+      weights4(b + 4 * tid, x, w);
+      const u64 sum = warp_sum(w[0] + w[1] + w[2] + w[3]);
       if (lane == 0) {
-        sm.sums[b / kBlock * kWarps + warp] = w;
-        v[0] += w;
+        sm.sums[b / kBlock * kWarps + warp] = sum;
+        v[0] += sum;
       }
     }
     block_reduce<false>(v);
@@ -553,9 +711,9 @@ struct Row {
     const int i = entry / kWarps * kBlock + entry % kWarps * 128 + 4 * lane;
     float x[4];
     get4(i, x);
-    u64 w[4], mine = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mine += w[e] = kept(x[e], i + e);
+    u64 w[4];
+    weights4(i, x, w);
+    const u64 mine = w[0] + w[1] + w[2] + w[3];
     u64 incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -573,6 +731,55 @@ struct Row {
   }
 };
 
+// The slice into shared memory in 16-byte loads, several in flight per thread, and the
+// thread's largest logit (the first of them).  Element `skip` of base is the slice's first;
+// base is 16-byte aligned, and what stands before the slice is held as -inf.
+template <typename T>
+__device__ void load_slice(const T* base, int skip, int n, int n_held, float* held, float& best,
+                           int& at) {
+  constexpr int V = 16 / (int)sizeof(T), kAhead = 4;
+  best = -CUDART_INF_F;
+  at = 0;
+  const auto see = [&](float v, int i) {
+    if (v > best || (v == best && i < at)) {
+      best = v;
+      at = i;
+    }
+  };
+  const int tid = threadIdx.x;
+  const int g0 = skip ? 1 : 0, g1 = max(g0, min(n, n_held) / V);  // whole vectors
+  for (int g = g0 + tid; g < g1; g += kAhead * kThreads) {
+    uint4 r[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (g + u * kThreads < g1)
+        r[u] = __ldg(reinterpret_cast<const uint4*>(base) + g + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = (g + u * kThreads) * V;
+      if (g + u * kThreads < g1) {
+        const T* e = reinterpret_cast<const T*>(&r[u]);
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          v[j] = clean(Elem<T>::get(e[j]));
+          see(v[j], i + j);
+        }
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          *reinterpret_cast<float4*>(held + i + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+    }
+  }
+  const auto one = [&](int i) {
+    const float v = i >= skip && i < n ? clean(Elem<T>::get(base[i])) : -CUDART_INF_F;
+    if (i < n_held) held[i] = v;
+    see(v, i);
+  };
+  for (int i = tid; i < g0 * V; i += kThreads) one(i);
+  for (int i = g1 * V + tid; i < max(n, n_held); i += kThreads) one(i);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const SampleParams p, const int ranks, const int per, const int room) {
@@ -581,54 +788,65 @@ __global__ void __launch_bounds__(kThreads, 2)
   float* held = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % ranks, row = blockIdx.x / ranks;
-  const int lo = min(rank * per, p.vocab), n = min(per, p.vocab - lo);
+  const int lo = min(rank * per, p.vocab);
   const T* x = static_cast<const T*>(p.logits) + (long long)row * p.logits_stride + lo;
+  const int skip = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const int n = lo < p.vocab ? min(per, p.vocab - lo) + skip : 0;
+  static_assert(sizeof(Shared) % 16 == 0, "the slice is read 16 bytes at a time");
+  const int n_held = min((n + 7) & ~7, room);
   if (tid < 64) sm.pow2[tid] = exp2(tid / 64.0);
   pdl_wait();
 
-  // The slice into shared memory, and its largest logit (the first of them).
-  static_assert(sizeof(Shared) % 16 == 0, "the slice is read 16 bytes at a time");
-  const int n_held = min((n + 3) & ~3, room);
-  float best = -CUDART_INF_F;
-  int at = 0;
-#pragma unroll 8
-  for (int i = tid; i < n; i += kThreads) {
-    const float v = clean(Elem<T>::get(x[i]));
-    if (i < n_held) held[i] = v;
-    if (v > best) {
-      best = v;
-      at = i;
-    }
-  }
-  for (int i = n + tid; i < n_held; i += kThreads) held[i] = -CUDART_INF_F;
+  float best;
+  int at;
+  load_slice(x - skip, skip, n, n_held, held, best, at);
   const float temp = p.temperature ? p.temperature[row] : 1.f;
   const int k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
-  Row<T> r{p, sm, x, held, lo, n, n_held, rank, ranks, tid, lane, warp};
+  const float u = p.uniform[row];
+  Row<T> r{p, sm, x - skip, held, lo - skip, n, n_held, rank, ranks, tid, lane, warp};
   u64 v[4] = {r.ord(best, at), 0, 0, 0};
   if (best == -CUDART_INF_F) v[0] = 0;
   r.template block_reduce<true>(v);
   r.exchange(v);
   u64 top_ord = 0;
   for (int i = 0; i < ranks; ++i) top_ord = max(top_ord, sm.got[i][0]);
-  const int first = (int)(0xffffffffu - (uint32_t)top_ord);
+  int* token = p.tokens + row;
   if (top_ord == 0 || !(temp > 0.f)) {  // nothing above -inf, or greedy
-    if (rank == 0 && tid == 0) p.tokens[row] = top_ord == 0 ? 0 : first;
-    __syncthreads();
-    cluster_sync();
-    return;
+    if (rank == 0 && tid == 0) *token = top_ord == 0 ? 0 : (int)(0xffffffffu - (uint32_t)top_ord);
+  } else {
+    r.top = key_logit((uint32_t)(top_ord >> 32));
+    r.infinite = r.top == CUDART_INF_F;
+    r.top_ord = top_ord;
+    r.ct = 1.4426950408889634074 / (double)temp;
+    r.c2 = (float)(2.0 * r.ct);
+    r.range = (float)(p.wshift + 2);
+    r.per_step = kBins / r.range;
+    r.scale = (double)(1ull << p.wshift);
+    r.min_p = p.min_p ? p.min_p[row] : 0.f;
+    const bool by_count = k > 0 && k < p.vocab;
+    int listed = 0;       // elements collected that hold all that is kept
+    u64 cut = 0;          // otherwise: the last kept element
+    double target = 0.0;  // the weight that top-p keeps, where it is known
+    if (by_count && k <= kSmallK && r.gather_first(k, best, listed)) {
+      // (all is in the list)
+    } else {
+      listed = 0;
+      if (by_count) cut = r.find_kth(k);
+      if (top_p < 1.f) {
+        const u64 c = r.find_share(cut, (double)top_p, listed, target);
+        cut = max(cut, c);
+        if (listed) target = fmax(target, 0.0);
+      }
+    }
+    if (listed == 0) {
+      r.pick(cut, u, token);
+    } else if (rank == 0) {
+      const bool weighed = !(by_count && k <= kSmallK && target == 0.0);
+      r.collect(false, weighed);
+      r.finish(listed, weighed ? kList : k, weighed, target, (double)top_p, u, token);
+    }
   }
-  r.top = key_logit((uint32_t)(top_ord >> 32));
-  r.top_ord = top_ord;
-  r.ct = 1.4426950408889634074 / (double)temp;
-  r.c2 = (float)(2.0 * r.ct);
-  r.range = (float)(p.wshift + 2);
-  r.scale = (double)(1ull << p.wshift);
-  r.min_p = p.min_p ? p.min_p[row] : 0.f;
-  u64 cut = 0;
-  if (k > 0 && k < p.vocab) cut = r.find_kth(k);
-  if (top_p < 1.f) cut = max(cut, r.find_share(cut, (double)top_p));
-  r.pick(cut, p.uniform[row], p.tokens + row);
   __syncthreads();
   cluster_sync();  // no CTA leaves while another may read its shared memory
 }
@@ -678,8 +896,9 @@ cudaError_t launch_sample(const SampleParams& p, int dtype, int n_sm, cudaStream
          (p.vocab > two * ranks ||
           ((long long)p.n_rows * ranks < 2 * n_sm && p.vocab > 2 * kBlock * ranks)))
     ranks *= 2;
-  const int per = ((p.vocab + ranks - 1) / ranks + 3) & ~3;
-  const int room = std::min(per, (kMaxSmem - (int)sizeof(Shared)) / 4 & ~3);
+  const int per = ((p.vocab + ranks - 1) / ranks + 7) & ~7;
+  // (a slice that starts off a 16-byte boundary is held from that boundary on)
+  const int room = std::min(per + 8, (kMaxSmem - (int)sizeof(Shared)) / 4 & ~7);
   const size_t smem = sizeof(Shared) + (size_t)room * 4;
   if (dtype == kDtypeF32) return launch_one<float>(p, ranks, per, room, smem, st, pdl);
   if (dtype == kDtypeBf16) return launch_one<__nv_bfloat16>(p, ranks, per, room, smem, st, pdl);

@@ -53,6 +53,7 @@ STATUS_BAD_PAGE = 16
 
 F32, BF16, F16 = 0, 1, 2   # GQA_F32, GQA_BF16, GQA_F16
 SAMPLE_MAX_VOCAB = 1 << 20
+_I32 = 16                  # int32 among the types that arguments are checked for
 
 HEAD_Q6_K = 0   # gqa_model.lm_head_type: gqa_lm_head_pack layout (Qwen2.5-1.5B)
 HEAD_Q8_0 = 1   # gqa_lm_head_q8_0_pack layout (Qwen2.5-0.5B)
@@ -267,45 +268,62 @@ def ffn_weights_of(w_gate, w_up, w_down, gamma) -> FfnWeights:
     return FfnWeights(_ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(gamma))
 
 
+_TORCH_TYPES: dict = {}  # torch dtype -> GQA_F32 / GQA_BF16 / GQA_F16 or _I32
+
+
+def _types() -> dict:
+    if not _TORCH_TYPES:
+        import torch
+        _TORCH_TYPES.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
+                             torch.int32: _I32})
+    return _TORCH_TYPES
+
+
 def _dtype_of(x) -> int:
-    """GQA_F32 / GQA_BF16 / GQA_F16 of a torch tensor or a numpy array."""
-    name = str(x.dtype).removeprefix("torch.")
-    codes = {"float32": F32, "bfloat16": BF16, "float16": F16}
-    if name not in codes:
-        raise GqaError(GQA_ERR_INVALID_ARG, f"type {name} is not float32, bfloat16 or float16")
-    return codes[name]
+    """GQA_F32 / GQA_BF16 / GQA_F16 of a torch tensor."""
+    code = _types().get(x.dtype, _I32)
+    if code == _I32:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"type {x.dtype} is not float32, bfloat16 or float16")
+    return code
 
 
-def _expect(x, what: str, device: int, dtype: int | str | None = None) -> None:
-    """Refuses a tensor argument of another type, on another device, or whose last dimension is
-    not dense (plain pointers are taken as they are)."""
-    if x is None or not hasattr(x, "data_ptr"):
-        return
-    if not x.is_cuda or x.device.index != device:
-        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is on {x.device}, not on cuda:{device}")
-    if dtype == "int32":
-        if str(x.dtype) != "torch.int32":
-            raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is {x.dtype}, not int32")
-    elif dtype is not None and _dtype_of(x) != dtype:
-        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is {x.dtype}, not the cache's or float32")
-    if x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
-        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is not dense in its last dimension")
+def _vector(x, what: str, device: int, dtype: int, need: int) -> int | None:
+    """Address of a device vector of at least `need` elements; refuses a tensor of another type,
+    on another device or with gaps (plain pointers are taken as they are)."""
+    if x is None or isinstance(x, int):
+        return x
+    if (_types().get(x.dtype) != dtype or x.get_device() != device or x.numel() < need
+            or not x.is_contiguous()):
+        raise GqaError(GQA_ERR_INVALID_ARG,
+                       f"{what}: {need} dense elements of "
+                       f"{'int32' if dtype == _I32 else 'float32'} on cuda:{device} are needed, "
+                       f"not {tuple(x.shape)} of {x.dtype} on {x.device}")
+    return x.data_ptr()
 
 
-def _count(x, what: str, need: int) -> None:
-    if x is not None and hasattr(x, "numel") and x.numel() < need:
-        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} holds {x.numel()} elements, {need} needed")
-
-
-def _row_stride(x, what: str, rows: int, width: int, stride: int | None) -> int:
-    """Elements between the rows of a [rows, width] argument: as given, or the tensor's own."""
-    if hasattr(x, "data_ptr") and x.dim() == 2:
-        if x.shape[0] < rows or x.shape[1] < width:
+def _matrix(x, what: str, device: int, dtype: int, rows: int, width: int,
+            stride: int | None) -> tuple[int | None, int]:
+    """Address of `rows` rows of `width` elements and the elements between them, as given or as
+    the tensor has them; refuses a tensor of another type or size, on another device, or whose
+    rows are not dense."""
+    if x is None or isinstance(x, int):
+        return x, width if stride is None else stride
+    if _types().get(x.dtype) != dtype or x.get_device() != device:
+        raise GqaError(GQA_ERR_INVALID_ARG,
+                       f"{what} is {x.dtype} on {x.device}: the call's type (GQA dtype {dtype}) on "
+                       f"cuda:{device} is needed")
+    if x.dim() == 2:
+        n, w = x.shape
+        own = x.stride()
+        if n < rows or w < width or (w > 1 and own[1] != 1):
             raise GqaError(GQA_ERR_INVALID_ARG,
-                           f"{what} is {tuple(x.shape)}, needs {rows} rows of {width}")
+                           f"{what} is {tuple(x.shape)}, strides {own}; {rows} dense rows of "
+                           f"{width} are needed")
         if stride is None:
-            return x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    return width if stride is None else stride
+            stride = own[0] if n > 1 else w
+    elif x.dim() and x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is not dense in its last dimension")
+    return x.data_ptr(), width if stride is None else stride
 
 
 def paged_kv_of(k_pages, v_pages, page_table, layout: str = "hnd") -> PagedKV:
@@ -319,10 +337,13 @@ def paged_kv_of(k_pages, v_pages, page_table, layout: str = "hnd") -> PagedKV:
         raise GqaError(GQA_ERR_INVALID_ARG, "the pools must be two 4-d tensors alike")
     if page_table.dim() != 2:
         raise GqaError(GQA_ERR_INVALID_ARG, "the page table must be [n_seq, max_pages]")
-    device = k_pages.device.index
-    _expect(k_pages, "k_pages", device)
-    _expect(v_pages, "v_pages", device)
-    _expect(page_table, "page_table", device, "int32")
+    device = k_pages.get_device()
+    if (device < 0 or page_table.get_device() != device
+            or _types().get(page_table.dtype) != _I32):
+        raise GqaError(GQA_ERR_INVALID_ARG, "the pools and the int32 page table must be on one GPU")
+    if k_pages.stride(3) != 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise GqaError(GQA_ERR_INVALID_ARG, "pools and page table must be dense in their last "
+                       "dimension")
     rows, heads = (2, 1) if layout == "hnd" else (1, 2)
 
     def stride(dim, dense):
@@ -785,58 +806,57 @@ class Context:
         return _stream(stream)
 
     def _paged_args(self, kv: PagedKV, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride):
-        width = (self.n_heads_q + 2 * self.cfg.n_heads_kv) * self.head_dim
-        if hasattr(kv, "sizes"):
-            heads, d, seqs, device = kv.sizes
-            if heads != self.n_heads_kv or d != self.head_dim or device != self.device:
+        """Checked addresses: q_starts, seq_lens, qkv, and qkv's stride."""
+        device = self.device
+        sizes = getattr(kv, "sizes", None)
+        if sizes is not None:
+            heads, d, seqs, on = sizes
+            if heads != self.n_heads_kv or d != self.head_dim or on != device:
                 raise GqaError(GQA_ERR_INVALID_ARG,
-                               f"the pools hold {heads} heads of {d} on cuda:{device}; the context "
-                               f"has {self.n_heads_kv} of {self.head_dim} on cuda:{self.device}")
+                               f"the pools hold {heads} heads of {d} on cuda:{on}; the context "
+                               f"has {self.n_heads_kv} of {self.head_dim} on cuda:{device}")
             if n_seq > seqs:
                 raise GqaError(GQA_ERR_INVALID_ARG, f"the page table has {seqs} rows of {n_seq}")
-        _expect(qkv, "qkv", self.device, kv.dtype)
-        _expect(q_starts, "q_starts", self.device, "int32")
-        _expect(seq_lens, "seq_lens", self.device, "int32")
-        _count(q_starts, "q_starts", n_seq + 1)
-        _count(seq_lens, "seq_lens", n_seq)
-        return _row_stride(qkv, "qkv", n_tokens, width, qkv_stride)
+        q, stride = _matrix(qkv, "qkv", device, kv.dtype, n_tokens,
+                            (self.n_heads_q + 2 * self.n_heads_kv) * self.head_dim, qkv_stride)
+        return (_vector(q_starts, "q_starts", device, _I32, n_seq + 1),
+                _vector(seq_lens, "seq_lens", device, _I32, n_seq), q, stride)
 
     def paged_append(self, kv: PagedKV, n_seq: int, n_tokens: int, q_starts, seq_lens, qkv,
                      qkv_stride: int | None = None, stream=None) -> None:
         """Rotated k and raw v of the new tokens into the pages (gqa_paged_append)."""
-        qkv_stride = self._paged_args(kv, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride)
-        _check(lib().gqa_paged_append(self._h, self._stream_of(stream), ctypes.byref(kv), n_seq,
-                                      n_tokens, _ptr(q_starts), _ptr(seq_lens), _ptr(qkv),
-                                      qkv_stride))
+        starts, lens, q, stride = self._paged_args(kv, n_seq, n_tokens, q_starts, seq_lens, qkv,
+                                                   qkv_stride)
+        _check(lib().gqa_paged_append(self._h, self._stream_of(stream), kv, n_seq, n_tokens,
+                                      starts, lens, q, stride))
 
     def paged_attention(self, kv: PagedKV, n_seq: int, n_tokens: int, q_starts, seq_lens,
                         max_new: int, max_len: int, qkv, out, qkv_stride: int | None = None,
                         out_stride: int | None = None, stream=None) -> None:
         """Attention of the new tokens over their pages (gqa_paged_attention)."""
-        qkv_stride = self._paged_args(kv, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride)
-        _expect(out, "out", self.device, kv.dtype)
-        out_stride = _row_stride(out, "out", n_tokens, self.n_heads_q * self.head_dim, out_stride)
-        _check(lib().gqa_paged_attention(self._h, self._stream_of(stream), ctypes.byref(kv), n_seq,
-                                         n_tokens, _ptr(q_starts), _ptr(seq_lens), max_new,
-                                         max_len, _ptr(qkv), qkv_stride, _ptr(out), out_stride))
+        starts, lens, q, stride = self._paged_args(kv, n_seq, n_tokens, q_starts, seq_lens, qkv,
+                                                   qkv_stride)
+        o, o_stride = _matrix(out, "out", self.device, kv.dtype, n_tokens,
+                              self.n_heads_q * self.head_dim, out_stride)
+        _check(lib().gqa_paged_attention(self._h, self._stream_of(stream), kv, n_seq, n_tokens,
+                                         starts, lens, max_new, max_len, q, stride, o, o_stride))
 
     def sample(self, n_rows: int, vocab: int, logits, temperature, top_k, top_p, min_p, uniform,
                tokens, logits_stride: int | None = None, dtype: int | None = None,
                stream=None) -> None:
         """A token per row of logits (gqa_sample); temperature, top_k, top_p and min_p may be
         None.  dtype is the logits tensor's unless given."""
+        device = self.device
         if dtype is None:
             dtype = _dtype_of(logits)
-        _expect(logits, "logits", self.device, dtype)
-        logits_stride = _row_stride(logits, "logits", n_rows, vocab, logits_stride)
-        for x, what, t in ((temperature, "temperature", F32), (top_k, "top_k", "int32"),
-                           (top_p, "top_p", F32), (min_p, "min_p", F32),
-                           (uniform, "uniform", F32), (tokens, "tokens", "int32")):
-            _expect(x, what, self.device, t)
-            _count(x, what, n_rows)
-        _check(lib().gqa_sample(self._h, self._stream_of(stream), n_rows, vocab, dtype,
-                                _ptr(logits), logits_stride, _ptr(temperature), _ptr(top_k),
-                                _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens)))
+        x, stride = _matrix(logits, "logits", device, dtype, n_rows, vocab, logits_stride)
+        _check(lib().gqa_sample(self._h, self._stream_of(stream), n_rows, vocab, dtype, x, stride,
+                                _vector(temperature, "temperature", device, F32, n_rows),
+                                _vector(top_k, "top_k", device, _I32, n_rows),
+                                _vector(top_p, "top_p", device, F32, n_rows),
+                                _vector(min_p, "min_p", device, F32, n_rows),
+                                _vector(uniform, "uniform", device, F32, n_rows),
+                                _vector(tokens, "tokens", device, _I32, n_rows)))
 
     def fill_normal(self, dst, n: int, seed: int, stream_id: int, offset: int = 0,
                     stream=None) -> None:

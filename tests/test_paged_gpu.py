@@ -4,7 +4,7 @@ import math
 import numpy as np
 import pytest
 
-from paged_ref import DTYPES, THETA, Batch
+from paged_ref import THETA, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -387,8 +387,3 @@ def test_refusals(pkg, cuda):
         ctx.paged_attention(r.kv, 2, 0, None, r.lens, 1, 30, r.qkv, out)
     with make_ctx(pkg, 64) as ctx, bad:
         ctx.paged_append(r.kv, 2, 2, None, r.lens, r.qkv)              # heads of another size
-
-
-def test_dtype_table(pkg):
-    assert [pkg.gqa._dtype_of(np.empty(0, np.float32))] == [pkg.gqa.F32]
-    assert set(DTYPES) == {"f32", "bf16", "f16"}

@@ -123,6 +123,46 @@ def test_infinities_and_nan(pkg, cuda):
     run(pkg, cuda, x, [0.0] * 12, None, None, None, u)
 
 
+@pytest.mark.parametrize("vocab", [3000, 60001, 500000])
+def test_top_k_beyond_the_weighted(pkg, cuda, vocab):
+    """A top_k that takes in every logit with a weight, on one CTA and on clusters of them, and
+    a vocabulary of which a part stays in memory."""
+    g = np.random.default_rng(10)
+    x = cuda.from_numpy(g.standard_normal((12, vocab)).astype(np.float32) * 3)
+    u = g.random(12).tolist()
+    for p, m in ((None, None), ([0.8] * 12, None), (None, [0.01] * 12)):
+        run(pkg, cuda, x, [0.02] * 6 + [0.9] * 6, [2500] * 11 + [vocab - 1], p, m, u)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_largest_vocabulary_off_alignment(pkg, cuda, dtype):
+    """Rows that start off a 16-byte boundary, at the limit of the vocabulary."""
+    g = cuda.Generator().manual_seed(4)
+    vocab = pkg.gqa.SAMPLE_MAX_VOCAB
+    x = (cuda.randn(3, vocab + 3, generator=g) * 2).to(DTYPES[dtype]).cuda()
+    u = cuda.tensor([0.999999, 0.5, 0.25], device="cuda")
+    p = cuda.tensor([1.0, 0.9, 1.0], device="cuda")
+    k = cuda.tensor([0, 0, 5000], dtype=cuda.int32, device="cuda")
+    tok = cuda.empty(3, dtype=cuda.int32, device="cuda")
+    with pkg.Context() as ctx:
+        ctx.sample(3, vocab, x[:, 1:], None, k, p, None, u, tok)
+    want = [sample_row(x[i, 1:vocab + 1].double().cpu().numpy(), 1.0, int(k[i]), float(p[i]), 0.0,
+                       float(u[i])) for i in range(3)]
+    np.testing.assert_array_equal(tok.cpu().numpy(), want)
+
+
+def test_high_temperature(pkg, cuda):
+    """All logits within a few steps of the exponent: the steps are cut again by the logits."""
+    g = np.random.default_rng(11)
+    x = cuda.from_numpy(g.standard_normal((10, 40000)).astype(np.float32))
+    u = g.random(10).tolist()
+    t = [100.0, 1e4, 1e30, 300.0, 50.0] * 2
+    run(pkg, cuda, x, t, [20000, 7] * 5, None, None, u)
+    run(pkg, cuda, x, t, None, [0.5, 0.9] * 5, None, u)
+    run(pkg, cuda, x, t, [30000, 600] * 5, [0.7, 0.1] * 5, None, u)
+    run(pkg, cuda, cuda.zeros(10, 40000), t, [20000, 7] * 5, [0.37, 0.71] * 5, None, u)
+
+
 def test_distribution(pkg, cuda):
     """Evenly spaced uniform numbers give each token its share, to one number each way."""
     rows = 4096
