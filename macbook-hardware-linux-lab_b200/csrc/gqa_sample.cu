@@ -48,19 +48,23 @@ constexpr int kBlock = kThreads * 4;  // elements of one turn of the CTA's threa
 
 using u64 = unsigned long long;
 
+constexpr int kGroups = 64;                 // of the steps, for the first look over the cluster
+constexpr int kInGroup = kBins / kGroups;   // 32: a warp's lanes
+
 struct alignas(16) Shared {  // (the slice of the row follows it)
   union {
     uint32_t hist[kBins];
     u64 sums[kBins / 2 + kWarps];  // for the pick: weights of 128 elements each
   };
+  alignas(16) u64 group[kGroups];      // sums of the histogram's groups
   u64 list_ord[kList], list_w[kList];  // this CTA's elements of the step
   u64 over_ord[kList], over_w[kList];  // and those before it, while they fit
   u64 all_ord[kList], all_w[kList];    // the cluster's
   u64 x[2][4];                         // values exchanged over the cluster
   u64 got[kMaxCluster][4];
   u64 red[kWarps][4];
-  double pow2[64];                     // 2^(j / 64)
-  u64 found_before, cut;
+  double pow2[64];                     // 2^(j / 64 + wshift)
+  u64 found_before, found_all, cut;
   int found;
   uint32_t n_list, n_over;
 };
@@ -76,21 +80,32 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 // -0 as 0, NaN as -inf.
 __device__ __forceinline__ float clean(float x) { return x != x ? -CUDART_INF_F : x + 0.0f; }
 
-__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
   u64 v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ld_cluster_v2(uint32_t addr, u64 (&v)[2]) {
+  asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 
 __device__ __forceinline__ u64 warp_sum(u64 x) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+__device__ __forceinline__ u64 warp_scan(u64 x, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
   return x;
 }
 
@@ -103,57 +118,54 @@ struct Row {
   int lo, n, n_held;  // the slice's first index, its elements, those in shared memory
   int rank, ranks, tid, lane, warp, turn = 0;
   float top;          // largest logit
-  bool infinite;      // it is infinite: only its equals have a weight, and the same one
+  bool infinite = false;      // it was infinite: it counts as 0, and all others as -inf
   u64 top_ord;
-  float c2;           // twice log2(e) / temperature, for the steps
-  double ct;          // log2(e) / temperature
-  float range;        // steps cover weights down to 2^-range
-  float per_step;     // kBins / range
-  double scale;       // 2^wshift
+  int range;          // the steps cover weights down to 2^-range; others round to zero
+  float logits_per_step;
+  float half_top, rate;  // step of a logit: (half_top - x / 2) * rate
+  float floor_x;      // no logit up to this one has a weight
+  double t_scale, t_shift;  // a logit's exponent in 64ths: x * t_scale + t_shift
+  double most;              // weight of the largest (2^wshift, to the rounding of t_shift)
   float min_p;
+
+  __device__ void settle(u64 best, float temp) {
+    top_ord = best;
+    top = key_logit((uint32_t)(top_ord >> 32));
+    range = p.wshift + 2;
+    const double ct = 1.4426950408889634074 / (double)temp;  // of the exponent, per logit
+    t_scale = 64.0 * ct;
+    t_shift = -(double)top * t_scale;
+    half_top = 0.5f * top;
+    rate = (float)(2.0 * ct * kBins / range);
+    logits_per_step = (float)(range / ct / kBins);
+    // Where float logits lie so far apart that the next one below the largest weighs nothing,
+    // only the largest (and its equals) count.
+    floor_x = -CUDART_INF_F;
+    const float next = prev_logit(top);
+    if (((double)top - (double)next) * ct > range) {
+      floor_x = next;
+      t_scale = t_shift = 0.0;
+    } else {
+      floor_x = below(kBins);
+    }
+    weight(top, true, most);
+  }
+
+  static __device__ __forceinline__ float prev_logit(float x) {
+    const uint32_t k = logit_key(x) - 1;
+    return key_logit(k == 0x7fffffffu ? k - 1 : k);  // (-0 is not below 0)
+  }
+
+  // A logit below all those of step `steps` and less that have a weight.
+  __device__ __forceinline__ float below(int steps) const {
+    if (steps >= kBins - 1) steps = kBins;  // (the last step takes in what rounds past it)
+    return fmaxf(floor_x, top - (steps + 1.5f) * logits_per_step - 1e-6f * fabsf(top));
+  }
 
   __device__ __forceinline__ u64 ord(float x, int i) const {
     return (u64)logit_key(x) << 32 | (0xffffffffu - (uint32_t)(lo + i));
   }
 
-  // f(x, i) for the elements of the slice, four at a time per thread.
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-#pragma unroll 2
-    for (int b = 0; b < n; b += kBlock) {
-      const int i = b + 4 * tid;
-      float v[4];
-      get4(i, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f(v[e], i + e);
-    }
-  }
-  // f(x, i, step, d, on) with the weights of the elements that f wants (`want` says which, by
-  // ord and step), computed for four elements side by side where a warp has any.
-  template <typename W, typename F>
-  __device__ __forceinline__ void each_weight(W&& want, F&& f) const {
-    for (int b = 0; b < n; b += kBlock) {
-      const int i = b + 4 * tid;
-      float v[4], d[4];
-      int s[4];
-      bool on[4], any = false;
-      get4(i, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[e] = step_of(v[e], d[e]);
-        on[e] = s[e] < kBins && want(ord(v[e], i + e), s[e]);
-        any |= on[e];
-      }
-      if (!__any_sync(0xffffffffu, any)) continue;
-      u64 w[4];
-      double w64[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = weight(v[e], on[e], w64[e]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (on[e]) f(i + e, ord(v[e], i + e), s[e], d[e], w[e], w64[e]);
-    }
-  }
   __device__ __forceinline__ void get4(int i, float (&v)[4]) const {
     if (i < n_held) {  // (n_held is a multiple of 4, padded with -inf)
       const float4 x = *reinterpret_cast<const float4*>(held + i);
@@ -164,76 +176,106 @@ struct Row {
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        v[e] = i + e < n ? clean(Elem<T>::get(logits[i + e])) : -CUDART_INF_F;
+        v[e] = i + e < n ? finite(clean(Elem<T>::get(logits[i + e]))) : -CUDART_INF_F;
     }
   }
-
-  // log2 of top's weight over x's, and the step it falls in (kBins: beyond every weight).
-  // Non-decreasing in falling x, so steps cut the sorted order; halves keep the difference
-  // of two far logits finite.
-  __device__ __forceinline__ int step_of(float x, float& d) const {
-    d = x == top ? 0.f : (0.5f * top - 0.5f * x) * c2;
-    return d < range ? min((int)(d * per_step), kBins - 1) : kBins;
+  __device__ __forceinline__ float finite(float x) const {
+    return !infinite ? x : x == CUDART_INF_F ? 0.f : -CUDART_INF_F;
   }
 
-  // The weight in 64 bits: 2^t as 2^(k/64) times the series of the rest (|rest| <= 2^-7 ln 2;
-  // Tang's table method), and in units of 2^-wshift.  `on`: the logit is within the steps
-  // (others weigh nothing).  No branches, so that the four elements a thread has at a time
-  // go through the 64-bit pipe side by side.
+  // f(v, i) for the slice's elements i .. i + 3, four at a time per thread, where one of them
+  // is above `least`.
+  template <typename F>
+  __device__ __forceinline__ void each4(float least, F&& f) const {
+#pragma unroll 2
+    for (int b = 0; b < n; b += kBlock) {
+      const int i = b + 4 * tid;
+      float v[4];
+      get4(i, v);
+      if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) > least) f(v, i);
+    }
+  }
+  // f(x, i) for the elements above `least`.
+  template <typename F>
+  __device__ __forceinline__ void each(float least, F&& f) const {
+    each4(least, [&](const float (&v)[4], int i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v[e] > least) f(v[e], i + e);
+    });
+  }
+
+  // The step of a logit above floor_x: how far below the largest it lies, in equal parts of
+  // the exponent.  Non-decreasing in falling x, so steps cut the sorted order; halves keep the
+  // difference of two far logits finite.
+  __device__ __forceinline__ int step_of(float x) const {
+    const int s = (int)(fmaf(-0.5f, x, half_top) * rate);
+    return min(s, kBins - 1);
+  }
+
+  // The weight in units of 2^-wshift, from 64 bits: 2^(t/64) as 2^(k/64) times the series of
+  // the rest (|rest| <= 1/2; Tang's table method, the series to the fourth power is off by
+  // 4e-14).  `on`: the logit is above floor_x (others weigh nothing).  No branches, so that the
+  // four elements a thread has at a time go through the 64-bit pipe side by side.
   __device__ __forceinline__ u64 weight(float x, bool on, double& w) const {
-    double t = ((double)(on ? x : top) - (double)top) * ct;
-    if (infinite) t = 0.0;
+    const double t = fma((double)x, t_scale, t_shift);
+    return weight_at(__hiloint2double(on ? __double2hiint(t) : (int)0xc0ef4000, __double2loint(t)),
+                     w);
+  }
+  __device__ __forceinline__ u64 weight_at(double t, double& w) const {
+    constexpr double c = 0.693147180559945309 / 64.0;
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
-    const double km = fma(t, 64.0, magic);
+    const double km = t + magic;
     const int k = __double2loint(km);
-    const double y = fma(km - magic, -1.0 / 64.0, t) * 0.693147180559945309;
-    double q = fma(y, 1.0 / 120.0, 1.0 / 24.0);
-    q = fma(q, y, 1.0 / 6.0);
-    q = fma(q, y, 0.5);
-    q = fma(q, y, 1.0);
+    const double y = t - (km - magic);
+    double q = fma(y, c * c * c * c / 24.0, c * c * c / 6.0);
+    q = fma(q, y, c * c / 2.0);
+    q = fma(q, y, c);
     q *= y;
     const double b = sm.pow2[k & 63];
     const double m = fma(b, q, b);
-    w = __hiloint2double(__double2hiint(m) + ((k >> 6) << 20), __double2loint(m));
+    w = __hiloint2double(__double2hiint(m) + ((k & ~63) << 14), __double2loint(m));
     // (a product of at most 2^50 plus 2^52 holds the rounded integer in its low bits)
-    const u64 bits = __double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xfffffffffffffull;
-    if (!on) w = 0.0;
-    return on ? bits : 0ull;
+    return __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
   }
 
-  // Sums (or, for `largest`, maxima) of four values over the block.
-  template <bool kMax>
-  __device__ void block_reduce(u64 (&v)[4]) {
+  // Sums or maxima of N values over the block.
+  template <bool kMax, int N>
+  __device__ void block_reduce(u64 (&v)[N]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < N; ++j)
 #pragma unroll
       for (int d = 16; d; d >>= 1) {
         const u64 y = __shfl_xor_sync(0xffffffffu, v[j], d);
         v[j] = kMax ? (y > v[j] ? y : v[j]) : v[j] + y;
       }
     __syncthreads();
-    if (lane < 4) sm.red[warp][lane] = lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
+    if (lane == 0)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sm.red[warp][j] = v[j];
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u64 x = 0;
-      for (int w = 0; w < kWarps; ++w) {
-        const u64 y = sm.red[w][j];
+    for (int j = 0; j < N; ++j) {
+      u64 x = sm.red[lane % kWarps][j];
+#pragma unroll
+      for (int d = kWarps / 2; d; d >>= 1) {
+        const u64 y = __shfl_xor_sync(0xffffffffu, x, d);
         x = kMax ? (y > x ? y : x) : x + y;
       }
       v[j] = x;
     }
   }
 
-  // Every CTA's four values into sm.got[rank] (a cluster barrier; what a CTA wrote to its
+  // Every CTA's values into sm.got[rank] (a cluster barrier; what a CTA wrote to its
   // shared memory before it, the others may read after it).  The two places alternate: a CTA
   // is past the next barrier only when all have read this one's.
-  __device__ void exchange(const u64 (&v)[4]) {
+  __device__ void exchange(u64 a, u64 b = 0, u64 c = 0, u64 d = 0) {
     u64* mine = sm.x[turn & 1];
-    if (tid < 4) mine[tid] = tid == 0 ? v[0] : tid == 1 ? v[1] : tid == 2 ? v[2] : v[3];
+    if (tid < 4) mine[tid] = tid == 0 ? a : tid == 1 ? b : tid == 2 ? c : d;
     __syncwarp();
     cluster_sync();
-    if (tid < ranks * 4) sm.got[tid >> 2][tid & 3] = ld_cluster_u64(cluster_map(mine + (tid & 3), tid >> 2));
+    if (tid < ranks * 4)
+      sm.got[tid >> 2][tid & 3] = ld_cluster_u64(cluster_map(mine + (tid & 3), tid >> 2));
     __syncthreads();
     ++turn;
   }
@@ -249,68 +291,90 @@ struct Row {
     __syncthreads();
   }
 
-  // This thread's four steps of the cluster's histogram (after a barrier).
-  __device__ void merged(u64 (&h)[4]) {
-    uint4 v[kMaxCluster];
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r)
-      v[r] = r < ranks ? ld_cluster_v4(cluster_map(&sm.hist[4 * tid], r)) : make_uint4(0, 0, 0, 0);
-    h[0] = h[1] = h[2] = h[3] = 0;
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) {
-      h[0] += v[r].x;
-      h[1] += v[r].y;
-      h[2] += v[r].z;
-      h[3] += v[r].w;
-    }
+  // A weight in a histogram of steps: its leading 14 bits or so, shifted by the step's exponent
+  // (the same for all of a step, so sums keep their meaning).
+  __device__ __forceinline__ int shift_of(int step) const {
+    return max(p.wshift - 14 - (step * range / kBins), 0);
   }
 
-  // The step at which the running sum of h reaches `want` (below zero: that share of the
-  // total), the sum before it and the total.
-  __device__ int find_step(const double (&h)[4], double want, double& before, double& all) {
+  // Puts the sums of the histogram's groups beside it (before an exchange).
+  __device__ void sum_groups(bool by_weight) {
     __syncthreads();
-    double mine = h[0] + h[1] + h[2] + h[3], incl = mine;
+    const int s = 4 * tid;
+    u64 x = 0;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += y;
-    }
-    double* red = reinterpret_cast<double*>(sm.red);
-    if (lane == 31) red[warp] = incl;
-    if (tid == 0) sm.found = -1;
-    __syncthreads();
-    double base = 0.0;
-    all = 0.0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) base += red[w];
-      all += red[w];
-    }
-    if (want < 0.0) want = -want * all;
-    double run = base + incl - mine;
-    // The last non-empty step before which the sum is below `want`: unlike a test of both
-    // ends, this always names one, however the sums are rounded.
-    int at = -1;
-    double at_before = 0.0;
+    for (int j = 0; j < 4; ++j) x += (u64)sm.hist[s + j] << (by_weight ? shift_of(s + j) : 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (h[j] > 0.0 && run < want) {
-        at = 4 * tid + j;
-        at_before = run;
+    for (int d = kInGroup / 8; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    if (tid % (kInGroup / 4) == 0) sm.group[tid / (kInGroup / 4)] = x;
+  }
+
+  // After the exchange: the step of the cluster's histogram at which the running sum reaches
+  // want (by_weight: that share of the total), into sm.found, the sum before it and the total.
+  // The last non-empty one if none does.  By one warp: the groups first, then the group's steps.
+  __device__ void find_step(double want, bool share, bool by_weight) {
+    if (warp == 0) {
+      u64 part[kMaxCluster][2], g[2] = {0, 0};
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        ld_cluster_v2(cluster_map(&sm.group[2 * lane], min(r, ranks - 1)), part[r]);
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < ranks) {
+          g[0] += part[r][0];
+          g[1] += part[r][1];
+        }
+      const u64 incl = warp_scan(g[0] + g[1], lane);
+      const u64 all = __shfl_sync(0xffffffffu, incl, 31);
+      if (share) want *= (double)all;
+      // the last non-empty group before which the sum is below `want`
+      const u64 b0 = incl - g[0] - g[1], b1 = incl - g[1];
+      int at = -1;
+      if (g[0] && (double)b0 < want) at = 2 * lane;
+      if (g[1] && (double)b1 < want) at = 2 * lane + 1;
+      const int gr = max(__reduce_max_sync(0xffffffffu, at), 0);
+      u64 before = __shfl_sync(0xffffffffu, gr & 1 ? b1 : b0, gr >> 1);
+      const int s = gr * kInGroup + lane;
+      uint32_t ph[kMaxCluster];
+      u64 h = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        ph[r] = ld_cluster_u32(cluster_map(&sm.hist[s], min(r, ranks - 1)));
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) h += r < ranks ? ph[r] : 0;
+      if (by_weight) h <<= shift_of(s);
+      const u64 b = before + warp_scan(h, lane) - h;
+      const int in = max(__reduce_max_sync(0xffffffffu, h && (double)b < want ? lane : -1), 0);
+      before = __shfl_sync(0xffffffffu, b, in);
+      if (lane == 0) {
+        sm.found = gr * kInGroup + in;
+        sm.found_before = before;
+        sm.found_all = all;
       }
-      run += h[j];
     }
-    if (at >= 0) atomicMax(&sm.found, at);
     __syncthreads();
-    if (at >= 0 && sm.found == at) *reinterpret_cast<double*>(&sm.found_before) = at_before;
-    __syncthreads();
-    before = *reinterpret_cast<double*>(&sm.found_before);
-    return sm.found;
   }
 
-  // Appends this thread's element to a list of the CTA.
-  __device__ __forceinline__ static void put(uint32_t& count, u64* list, u64 o) {
+  // The nearest non-empty step after (or before) `step`, or -1 (rarely needed).
+  __device__ int neighbour(int step, bool after) {
+    int best = -1;
+    for (int s = tid; s < kBins; s += kThreads) {
+      if (after ? s <= step : s >= step) continue;
+      uint32_t h = 0;
+      for (int r = 0; r < ranks; ++r) h |= ld_cluster_u32(cluster_map(&sm.hist[s], r));
+      if (h) best = max(best, after ? kBins - s : s);
+    }
+    u64 v[1] = {(u64)(best + 1)};
+    block_reduce<true, 1>(v);
+    best = (int)v[0] - 1;
+    return best < 0 ? -1 : after ? kBins - best : best;
+  }
+
+  // Appends an element to a list of the CTA.
+  __device__ __forceinline__ static int put(uint32_t& count, u64* list, u64 o) {
     const uint32_t at = atomicAdd(&count, 1u);
     if (at < kList) list[at] = o;
+    return (int)min(at, 1u << 30);
   }
 
   // The cluster's lists of the step into sm.all_* (counts in the exchange's last value: the
@@ -336,67 +400,50 @@ struct Row {
   // threads' own largest logits: at least k elements are at or above the k-th largest of
   // those, and few more where the logits are in no particular order.  One count per thread
   // in place of one per logit.
-  __device__ bool gather_first(int k, float best, int& n) {
+  __device__ bool gather_first(int k, float best, int& n_all) {
     clear_hist();
-    float d;
-    const int mine = step_of(best, d);
-    if (mine < kBins) atomicAdd(&sm.hist[mine], 1u);
-    u64 v[4] = {0, 0, 0, 0};
-    __syncthreads();
-    exchange(v);
-    u64 h[4];
-    merged(h);
-    const double hd[4] = {(double)h[0], (double)h[1], (double)h[2], (double)h[3]};
-    double before, all;
-    const int step = find_step(hd, k, before, all);
-    const int upto = all < k ? kBins - 1 : step;  // (fewer: all that have a weight)
-    each([&](float x, int i) {
-      if (step_of(x, d) <= upto) put(sm.n_list, sm.list_ord, ord(x, i));
+    if (best > floor_x) atomicAdd(&sm.hist[step_of(best)], 1u);
+    sum_groups(false);
+    exchange(0);
+    find_step(k, false, false);
+    // (fewer threads than k have a weight: all that have one)
+    const int upto = sm.found_all < (u64)k ? kBins - 1 : sm.found;
+    each(below(upto), [&](float x, int i) {
+      if (step_of(x) <= upto) put(sm.n_list, sm.list_ord, ord(x, i));
     });
     __syncthreads();
-    v[3] = min(sm.n_list, 1u << 30);
-    exchange(v);
+    exchange(0, 0, 0, sm.n_list);
     const u64 count = total(3);
-    n = (int)count;
-    if (count > kList) {
-      __syncthreads();
-      cluster_sync();  // (the lists are reused)
-      return false;
-    }
-    return true;
+    n_all = (int)min(count, (u64)(1 << 30));
+    if (count <= kList) return true;
+    __syncthreads();
+    cluster_sync();  // (the lists are reused)
+    return false;
   }
 
-  // The token from n collected elements that hold all of the row's first k (and, with
-  // weights, all that top-p keeps, whose weight the target is).  By one CTA: ranks by
-  // comparing all pairs, prefixes by a scan, and the index order again by pairs.
-  __device__ void finish(int n, int k, bool weighed, double target, double share, float u,
-                         int* token) {
-    const int m = min(n, k);
-    for (int i = tid; i < n; i += kThreads) {  // (n <= kList: one element a thread)
-      const u64 o = sm.all_ord[i];
+  // The token from n collected elements that hold all of the row's first k (and, where a
+  // target is given, all that it takes to reach it).  By one CTA: ranks by comparing all
+  // pairs, prefixes by a scan, and the index order again by pairs.
+  __device__ void finish(int n_all, int k, double target, double share, float u, int* token) {
+    const int m = min(n_all, k);
+    if (tid < n_all) {
+      const u64 o = sm.all_ord[tid];
       int at = 0;
-      for (int j = 0; j < n; ++j) at += sm.all_ord[j] > o;
-      u64 w;
-      double w64;
+#pragma unroll 8
+      for (int j = 0; j < n_all; ++j) at += sm.all_ord[j] > o;
       const float x = key_logit((uint32_t)(o >> 32));
-      float d;
-      w = weight(x, step_of(x, d) < kBins, w64);
+      double w64;
+      const u64 w = weight(x, x > floor_x, w64);
       sm.over_ord[at] = o;
-      // the weight with min_p's answer in the sign bit (weights stay below 2^50)
-      sm.over_w[at] = w | (u64)(!(w64 >= (double)min_p) && at > 0) << 63;
+      // the weight, and whether min_p leaves it out in the top bit (weights stay below 2^51)
+      sm.over_w[at] = w | (u64)(w64 < (double)min_p * most && at > 0) << 63;
     }
     __syncthreads();
-    constexpr u64 kMask = ~0ull >> 1;
     // cumulative weight in rank order, one rank a thread
     static_assert(kList <= kThreads, "a thread per element");
-    const u64 w = tid < m ? sm.over_w[tid] & kMask : 0;
-    u64 incl = w;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, incl, s);
-      if (lane >= s) incl += y;
-    }
-    __syncthreads();
+    const u64 marked = tid < m ? sm.over_w[tid] : 0;
+    const u64 w = marked & (~0ull >> 1);
+    u64 incl = warp_scan(w, lane);
     if (lane == 31) sm.red[warp][0] = incl;
     __syncthreads();
     u64 all = 0;
@@ -404,74 +451,77 @@ struct Row {
       if (j < warp) incl += sm.red[j][0];
       all += sm.red[j][0];
     }
-    if (!weighed) target = share * (double)all;
+    if (target < 0.0) target = share * (double)all;
     // rank i stays while the weight before it is below the target
-    const bool stays = tid < m && !(sm.over_w[tid] >> 63) &&
+    const bool stays = tid < m && !(marked >> 63) &&
                        (tid == 0 || !(share < 1.0) || (double)(incl - w) < target);
-    u64 mass[4] = {stays ? w : 0, 0, 0, 0};
-    // kept elements, for the index order
-    if (tid < n) {
+    u64 mass[1] = {stays ? w : 0};
+    if (tid < m) {
       sm.list_ord[tid] = stays ? 0xffffffffu - (uint32_t)sm.over_ord[tid] : 0xffffffffu;
       sm.list_w[tid] = mass[0];
     }
-    block_reduce<false>(mass);
+    block_reduce<false, 1>(mass);
     u = u > 0.f ? u : 0.f;
     const double ut = (double)u * (double)mass[0];
     const u64 pick = ut < (double)mass[0] ? (u64)ut : mass[0] - 1;
     if (stays && w) {
       const u64 me = sm.list_ord[tid];
       u64 run = 0;
+#pragma unroll 8
       for (int j = 0; j < m; ++j) run += sm.list_ord[j] <= me ? sm.list_w[j] : 0;
       if (run > pick && run - w <= pick) *token = (int)me;
     }
   }
 
+  // [first, last] from the largest ord and the largest complement that were exchanged.
+  __device__ void narrow(u64& first, u64& last) {
+    u64 hi = 0, lo_c = 0;
+    for (int r = 0; r < ranks; ++r) {
+      hi = max(hi, sm.got[r][0]);
+      lo_c = max(lo_c, sm.got[r][1]);
+    }
+    last = hi;
+    first = ~lo_c;
+    __syncthreads();
+  }
+
   // Element k (from 1) of the sorted row, as an ord; 0 if fewer have a weight.
   __device__ u64 find_kth(int k) {
     clear_hist();
-    each([&](float x, int) {
-      float d;
-      const int s = step_of(x, d);
-      if (s < kBins) atomicAdd(&sm.hist[s], 1u);
-    });
-    u64 v[4] = {0, 0, 0, 0};
-    __syncthreads();
-    exchange(v);
-    u64 h[4];
-    merged(h);
-    double hd[4] = {(double)h[0], (double)h[1], (double)h[2], (double)h[3]};
-    double before, all;
-    int step = find_step(hd, k, before, all);
-    if (all <= k) {
+    each(floor_x, [&](float x, int) { atomicAdd(&sm.hist[step_of(x)], 1u); });
+    sum_groups(false);
+    exchange(0);
+    find_step(k, false, false);
+    if (sm.found_all <= (u64)k) {
       __syncthreads();
       cluster_sync();  // (the next step reuses the histograms that the other CTAs may be reading)
       return 0;
     }
-    double want = k - before;     // rank within the interval
-    u64 first = 0, last = ~0ull;  // ords of the interval
+    const int step = sm.found;
+    u64 want = k - sm.found_before;  // rank within the interval
+    u64 first = 0, last = ~0ull;     // ords of the interval
     bool by_step = true;
     // (each turn narrows the interval to one of 2048 parts: 64 bits take six)
     for (int guard = 0; guard < 16; ++guard) {
-      u64 mm[4] = {0, 0, 0, 0};  // largest ord, largest ~ord
-      each([&](float x, int i) {
+      u64 mm[2] = {0, 0};  // largest ord, largest ~ord
+      each(by_step ? below(step) : below(kBins), [&](float x, int i) {
         const u64 o = ord(x, i);
-        float d;
-        if (by_step ? step_of(x, d) == step : o >= first && o <= last) {
+        if (by_step ? step_of(x) == step : o >= first && o <= last) {
           put(sm.n_list, sm.list_ord, o);
-          if (o > mm[0]) mm[0] = o;
-          if (~o > mm[1]) mm[1] = ~o;
+          mm[0] = max(mm[0], o);
+          mm[1] = max(mm[1], ~o);
         }
       });
-      block_reduce<true>(mm);
-      mm[3] = sm.n_list;
-      exchange(mm);
-      const u64 n = total(3);
-      if (n <= kList) {
+      block_reduce<true, 2>(mm);
+      exchange(mm[0], mm[1], 0, sm.n_list);
+      const u64 count = total(3);
+      if (count <= kList) {
         collect(false, false);
-        for (int i = tid; i < (int)n; i += kThreads) {
+        for (int i = tid; i < (int)count; i += kThreads) {
           const u64 o = sm.all_ord[i];
           int at = 0;
-          for (int j = 0; j < (int)n; ++j) at += sm.all_ord[j] > o;
+#pragma unroll 8
+          for (int j = 0; j < (int)count; ++j) at += sm.all_ord[j] > o;
           if (at == (int)want - 1) sm.cut = o;
         }
         __syncthreads();
@@ -481,90 +531,81 @@ struct Row {
       by_step = false;
       const int shift = max(0, 53 - __clzll(last - first));  // (last - first) >> shift < kBins
       clear_hist();
-      each([&](float x, int i) {
+      each(below(kBins), [&](float x, int i) {
         const u64 o = ord(x, i);
         if (o >= first && o <= last) atomicAdd(&sm.hist[(last - o) >> shift], 1u);
       });
-      __syncthreads();
-      exchange(v);
-      merged(h);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) hd[j] = (double)h[j];
-      const int b = find_step(hd, want, before, all);
-      want -= before;
-      last -= (u64)b << shift;
+      sum_groups(false);
+      exchange(0);
+      find_step((double)want, false, false);
+      want -= sm.found_before;
+      last -= (u64)sm.found << shift;
       if (last - first >> shift) first = last - ((1ull << shift) - 1);
+      __syncthreads();
     }
     return 0;
   }
 
-  // [first, last] from the largest ord and the largest complement that were exchanged.
-  __device__ void narrow(u64& first, u64& last) {
-    u64 hi = 0, lo_c = 0;
-    for (int r = 0; r < ranks; ++r) {
-      if (sm.got[r][0] > hi) hi = sm.got[r][0];
-      if (sm.got[r][1] > lo_c) lo_c = sm.got[r][1];
-    }
-    last = hi;
-    first = ~lo_c;
-    __syncthreads();
-  }
-
   // The last element of the shortest prefix, among the ords from `cut` up, whose weight
-  // reaches share times theirs.  n > 0: instead, n elements that hold all of that prefix are
-  // collected, and `target` is the weight to reach.
-  __device__ u64 find_share(u64 cut, double share, int& n, double& target) {
-    n = 0;
+  // reaches share times theirs.  n_all > 0: instead, so many elements that hold all of that
+  // prefix are listed, and `target` is the weight to reach.
+  __device__ u64 find_share(u64 cut, double share, int& n_all, double& target) {
+    n_all = 0;
     if (!(share > 0.0)) return top_ord;
     clear_hist();
-    const float width = range / kBins;
-    u64 v[4] = {0, 0, 0, 0};
-    each_weight([&](u64 o, int) { return o >= cut; },
-                [&](int, u64, int b, float d, u64 w, double) {
-                  v[0] += w;
-                  atomicAdd(&sm.hist[b], (uint32_t)(exp2f(b * width - d) * 16384.f + 0.5f));
-                });
-    block_reduce<false>(v);
-    exchange(v);
-    target = share * (double)total(0);
-    u64 h[4];
-    merged(h);
-    double hd[4];
+    const float least = cut ? fmaxf(floor_x, before_cut(cut)) : floor_x;
+    u64 v[1] = {0};
+    each4(least, [&](const float (&x)[4], int i) {
+      bool on[4];
+      u64 w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) hd[j] = (double)h[j] * exp2f(-(4 * tid + j) * width);
-    double unused, all;
-    int step = find_step(hd, -share, unused, all);
+      for (int e = 0; e < 4; ++e) {
+        double w64;
+        on[e] = x[e] > floor_x && ord(x[e], i + e) >= cut;
+        w[e] = weight(x[e], on[e], w64);
+        v[0] += w[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (on[e]) {
+          const int s = step_of(x[e]);
+          atomicAdd(&sm.hist[s], (uint32_t)(w[e] >> shift_of(s)));
+        }
+    });
+    block_reduce<false, 1>(v);
+    sum_groups(true);
+    exchange(v[0]);
+    target = share * (double)total(0);
+    find_step(share, true, true);
+    int step = sm.found;
     u64 first = cut, last = ~0ull;  // the interval, cut into steps
     int shift = -1;                 // -1: by exponent
     u64 above = 0;                  // exact weight of the kept elements before the interval
     for (int guard = 0; guard < 4 * kBins; ++guard) {
       if (tid == 0) sm.n_list = sm.n_over = 0;
       __syncthreads();
-      u64 s[4] = {0, 0, 0, 0};  // weight before the step, of the step
-      const auto part = [&](u64 o, int b) { return shift < 0 ? b : (int)((last - o) >> shift); };
-      each_weight([&](u64 o, int b) { return o >= first && o <= last && part(o, b) <= step; },
-                  [&](int, u64 o, int b, float, u64 w, double) {
-                    if (part(o, b) < step) {
-                      s[0] += w;
-                      if (shift < 0 && *(volatile uint32_t*)&sm.n_over < kList) {
-                        const uint32_t at = atomicAdd(&sm.n_over, 1u);
-                        if (at < kList) {
-                          sm.over_ord[at] = o;
-                          sm.over_w[at] = w;
-                        }
-                      }
-                    } else {
-                      s[1] += w;
-                      const uint32_t at = atomicAdd(&sm.n_list, 1u);
-                      if (at < kList) {
-                        sm.list_ord[at] = o;
-                        sm.list_w[at] = w;
-                      }
-                    }
-                  });
-      block_reduce<false>(s);
-      s[3] = sm.n_list | (u64)sm.n_over << 32;
-      exchange(s);
+      u64 s[2] = {0, 0};  // weight before the step, of the step
+      each(shift < 0 ? fmaxf(floor_x, below(step)) : least, [&](float x, int i) {
+        const u64 o = ord(x, i);
+        if (o < first || o > last) return;
+        const int b = shift < 0 ? step_of(x) : (int)((last - o) >> shift);
+        if (b > step) return;
+        double w64;
+        const u64 w = weight(x, x > floor_x, w64);
+        if (b < step) {
+          s[0] += w;
+          if (shift < 0 && *(volatile uint32_t*)&sm.n_over < kList) {
+            const int at = put(sm.n_over, sm.over_ord, o);
+            if (at < kList) sm.over_w[at] = w;
+          }
+        } else {
+          s[1] += w;
+          const int at = put(sm.n_list, sm.list_ord, o);
+          if (at < kList) sm.list_w[at] = w;
+        }
+      });
+      block_reduce<false, 2>(s);
+      exchange(s[0], s[1], 0, sm.n_list | (u64)sm.n_over << 32);
       const u64 before = above + total(0), in = total(1);
       u64 n_in = 0, n_over = 0;
       for (int r = 0; r < ranks; ++r) {
@@ -572,28 +613,18 @@ struct Row {
         n_over += sm.got[r][3] >> 32;
       }
       const bool early = (double)before >= target, late = (double)(before + in) < target;
-      if (early || late) {
-        // the 14-bit weights were too coarse: the next non-empty step that way
-        int other = -1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int b = 4 * tid + j;
-          if (h[j] == 0) continue;
-          if (early && b < step) other = b;                      // the last before
-          if (late && b > step && other < 0) other = kBins - b;  // the first after
+      if (early || late) {  // the short weights were too coarse: on to the next step that way
+        const int next = neighbour(step, late);
+        if (next < 0) {
+          __syncthreads();
+          cluster_sync();
+          return late ? 0 : top_ord;
         }
-        if (tid == 0) sm.found = -1;
-        __syncthreads();
-        atomicMax(&sm.found, other);
-        __syncthreads();
-        const int next = sm.found;
-        __syncthreads();
-        if (next < 0) return late ? 0 : top_ord;
-        step = late ? kBins - next : next;
+        step = next;
         continue;
       }
       if (shift < 0 && n_in + n_over <= kList) {
-        n = (int)(n_in + n_over);
+        n_all = (int)(n_in + n_over);
         return 0;
       }
       if (n_in <= kList) {
@@ -601,6 +632,7 @@ struct Row {
         for (int i = tid; i < (int)n_in; i += kThreads) {
           const u64 o = sm.all_ord[i];
           u64 incl = before;
+#pragma unroll 8
           for (int j = 0; j < (int)n_in; ++j) incl += sm.all_ord[j] >= o ? sm.all_w[j] : 0;
           if ((double)incl >= target && (double)(incl - sm.all_w[i]) < target) sm.cut = o;
         }
@@ -608,77 +640,82 @@ struct Row {
         return sm.cut;
       }
       // Too many for the list: cut the step by the ords it spans.
-      u64 mm[4] = {0, 0, 0, 0};
-      each([&](float x, int i) {
+      u64 mm[2] = {0, 0};
+      each(least, [&](float x, int i) {
         const u64 o = ord(x, i);
-        float d;
-        const int b = step_of(x, d);
-        if (b == kBins || o < first || o > last || part(o, b) != step) return;
-        if (o > mm[0]) mm[0] = o;
-        if (~o > mm[1]) mm[1] = ~o;
+        if (x <= floor_x || o < first || o > last) return;
+        if ((shift < 0 ? step_of(x) : (int)((last - o) >> shift)) != step) return;
+        mm[0] = max(mm[0], o);
+        mm[1] = max(mm[1], ~o);
       });
-      block_reduce<true>(mm);
-      exchange(mm);
+      block_reduce<true, 2>(mm);
+      exchange(mm[0], mm[1]);
       narrow(first, last);
       above = before;
       shift = max(0, 53 - __clzll(last - first));
       clear_hist();
-      double most;
-      weight(key_logit((uint32_t)(last >> 32)), true, most);
-      const float unit = (float)(16384.0 / most);
-      each_weight([&](u64 o, int) { return o >= first && o <= last; },
-                  [&](int, u64 o, int, float, u64, double w) {
-                    atomicAdd(&sm.hist[(last - o) >> shift], (uint32_t)((float)w * unit + 0.5f));
-                  });
-      v[0] = 0;
-      __syncthreads();
-      exchange(v);
-      merged(h);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) hd[j] = (double)h[j];
-      step = find_step(hd, fmax((target - (double)above) / scale * unit, 0.5), unused, all);
+      double largest;
+      weight(key_logit((uint32_t)(last >> 32)), true, largest);
+      const float unit = (float)(16384.0 / largest);
+      each(least, [&](float x, int i) {
+        const u64 o = ord(x, i);
+        if (o < first || o > last) return;
+        double w;
+        weight(x, x > floor_x, w);
+        atomicAdd(&sm.hist[(last - o) >> shift], (uint32_t)((float)w * unit + 0.5f));
+      });
+      sum_groups(false);
+      exchange(0);
+      find_step(fmax((target - (double)above) * unit, 0.5), false, false);
+      step = sm.found;
     }
     return cut;
+  }
+
+  // The largest logit below the cut's.
+  __device__ __forceinline__ float before_cut(u64 cut) const {
+    return prev_logit(key_logit((uint32_t)(cut >> 32)));
   }
 
   // The first index whose cumulative kept weight exceeds u times the total; the CTA that
   // holds it writes it.
   __device__ void pick(u64 cut, float u, int* token) {
-    // min_p's logits lie before the step of 2^-reach; the comparison itself is in 64 bits.
-    const float reach = min_p > 0.f ? -log2f(min_p) * 1.0001f + 0.01f : range;
-    const auto weights4 = [&](int i, const float (&x)[4], u64 (&w)[4]) {
-      bool on[4], any = false;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float d;
-        const u64 o = ord(x[e], i + e);
-        on[e] = step_of(x[e], d) < kBins && o >= cut && (d <= reach || o == top_ord);
-        any |= on[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = 0;
-      if (!__any_sync(0xffffffffu, any)) return;
+    // min_p's logits lie above a bound; the comparison itself is in 64 bits.
+    float least = floor_x;
+    if (cut) least = fmaxf(least, before_cut(cut));
+    if (min_p > 0.f)
+      least = fmaxf(least, below((int)fminf(-log2f(min_p) * (1.f * kBins / range) + 2.f, kBins)));
+    const float cut_x = cut ? key_logit((uint32_t)(cut >> 32)) : -CUDART_INF_F;
+    const int cut_i = (int)(0xffffffffu - (uint32_t)cut) - lo;  // the last of its ties
+    const double min_w = (double)min_p * most;
+    const auto weights4 = [&](const float (&x)[4], int i, u64 (&w)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         double w64;
-        w[e] = weight(x[e], on[e], w64);
-        if (!(w64 >= (double)min_p) && ord(x[e], i + e) != top_ord) w[e] = 0;
+        const bool on = x[e] > least && (x[e] != cut_x || i + e <= cut_i);
+        w[e] = weight(x[e], on, w64);
+        if (w64 < min_w) w[e] = 0;
       }
     };
-    u64 v[4] = {0, 0, 0, 0};
+    u64 v[1] = {0};
     for (int b = 0; b < n; b += kBlock) {
+      const int i = b + 4 * tid;
       float x[4];
-      u64 w[4];
-      get4(b + 4 * tid, x);
-      weights4(b + 4 * tid, x, w);
-      const u64 sum = warp_sum(w[0] + w[1] + w[2] + w[3]);
+      get4(i, x);
+      const bool any = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > least;
+      u64 sum = 0;
+      if (__any_sync(0xffffffffu, any)) {
+        u64 w[4];
+        weights4(x, i, w);
+        sum = warp_sum(w[0] + w[1] + w[2] + w[3]);
+      }
       if (lane == 0) {
         sm.sums[b / kBlock * kWarps + warp] = sum;
         v[0] += sum;
       }
     }
-    block_reduce<false>(v);
-    exchange(v);
+    block_reduce<false, 1>(v);
+    exchange(v[0]);
     u64 before = 0, all = 0;
     for (int r = 0; r < ranks; ++r) {
       if (r < rank) before += sm.got[r][0];
@@ -688,17 +725,12 @@ struct Row {
     const double ut = (double)u * (double)all;
     const u64 target = ut < (double)all ? (u64)ut : all - 1;
     if (warp != 0 || target < before || target >= before + sm.got[rank][0]) return;
-    // Lane by lane: the entry of sums, then the element of its 128.
+    // The entry of sums, then the element of its 128.
     const int entries = (n + kBlock - 1) / kBlock * kWarps;
     int entry = 0;
     for (int e0 = 0; e0 < entries; e0 += 32) {
       const u64 w = e0 + lane < entries ? sm.sums[e0 + lane] : 0;
-      u64 incl = w;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += y;
-      }
+      const u64 incl = warp_scan(w, lane);
       const unsigned over = __ballot_sync(0xffffffffu, before + incl > target);
       if (over) {
         const int l = __ffs(over) - 1;
@@ -710,17 +742,11 @@ struct Row {
     }
     const int i = entry / kWarps * kBlock + entry % kWarps * 128 + 4 * lane;
     float x[4];
-    get4(i, x);
     u64 w[4];
-    weights4(i, x, w);
+    get4(i, x);
+    weights4(x, i, w);
     const u64 mine = w[0] + w[1] + w[2] + w[3];
-    u64 incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += y;
-    }
-    u64 run = before + incl - mine;
+    u64 run = before + warp_scan(mine, lane) - mine;
     if (run <= target && run + mine > target) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -794,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int n = lo < p.vocab ? min(per, p.vocab - lo) + skip : 0;
   static_assert(sizeof(Shared) % 16 == 0, "the slice is read 16 bytes at a time");
   const int n_held = min((n + 7) & ~7, room);
-  if (tid < 64) sm.pow2[tid] = exp2(tid / 64.0);
+  if (tid < 64) sm.pow2[tid] = exp2(tid / 64.0 + p.wshift);
   pdl_wait();
 
   float best;
@@ -805,46 +831,48 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
   const float u = p.uniform[row];
   Row<T> r{p, sm, x - skip, held, lo - skip, n, n_held, rank, ranks, tid, lane, warp};
-  u64 v[4] = {r.ord(best, at), 0, 0, 0};
-  if (best == -CUDART_INF_F) v[0] = 0;
-  r.template block_reduce<true>(v);
-  r.exchange(v);
+  u64 v[1] = {best == -CUDART_INF_F ? 0 : r.ord(best, at)};
+  r.template block_reduce<true, 1>(v);
+  r.exchange(v[0]);
   u64 top_ord = 0;
   for (int i = 0; i < ranks; ++i) top_ord = max(top_ord, sm.got[i][0]);
   int* token = p.tokens + row;
   if (top_ord == 0 || !(temp > 0.f)) {  // nothing above -inf, or greedy
     if (rank == 0 && tid == 0) *token = top_ord == 0 ? 0 : (int)(0xffffffffu - (uint32_t)top_ord);
   } else {
-    r.top = key_logit((uint32_t)(top_ord >> 32));
-    r.infinite = r.top == CUDART_INF_F;
-    r.top_ord = top_ord;
-    r.ct = 1.4426950408889634074 / (double)temp;
-    r.c2 = (float)(2.0 * r.ct);
-    r.range = (float)(p.wshift + 2);
-    r.per_step = kBins / r.range;
-    r.scale = (double)(1ull << p.wshift);
+    if (top_ord >> 32 == logit_key(CUDART_INF_F)) {
+      // an infinite logit: only its equals count, all alike
+      r.infinite = true;
+      for (int i = tid; i < n_held; i += kThreads) held[i] = r.finite(held[i]);
+      best = r.finite(best);
+      top_ord = (top_ord & 0xffffffffull) | (u64)logit_key(0.f) << 32;
+      __syncthreads();
+    }
+    r.settle(top_ord, temp);
     r.min_p = p.min_p ? p.min_p[row] : 0.f;
+    if (!(r.min_p <= 1.f)) r.min_p = 2.f;  // (a NaN too) only the first token
     const bool by_count = k > 0 && k < p.vocab;
-    int listed = 0;       // elements collected that hold all that is kept
-    u64 cut = 0;          // otherwise: the last kept element
-    double target = 0.0;  // the weight that top-p keeps, where it is known
-    if (by_count && k <= kSmallK && r.gather_first(k, best, listed)) {
-      // (all is in the list)
-    } else {
+    const bool small = by_count && k <= kSmallK;
+    int listed = 0;        // elements listed that hold all that is kept
+    u64 cut = 0;           // otherwise: the last kept element
+    double target = -1.0;  // the weight that top-p keeps, where it is known
+    if (!small || !r.gather_first(k, best, listed)) {
       listed = 0;
       if (by_count) cut = r.find_kth(k);
       if (top_p < 1.f) {
         const u64 c = r.find_share(cut, (double)top_p, listed, target);
         cut = max(cut, c);
-        if (listed) target = fmax(target, 0.0);
+      }
+      if (r.min_p > 1.f && listed == 0) {
+        cut = top_ord;
+        r.min_p = 0.f;
       }
     }
     if (listed == 0) {
       r.pick(cut, u, token);
     } else if (rank == 0) {
-      const bool weighed = !(by_count && k <= kSmallK && target == 0.0);
-      r.collect(false, weighed);
-      r.finish(listed, weighed ? kList : k, weighed, target, (double)top_p, u, token);
+      r.collect(false, target >= 0.0);
+      r.finish(listed, target >= 0.0 ? kList : k, target, (double)top_p, u, token);
     }
   }
   __syncthreads();
