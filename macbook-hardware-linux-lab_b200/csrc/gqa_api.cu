@@ -763,6 +763,7 @@ int gqa_create(const gqa_config* cfg, int device, gqa_ctx** out) {
   // graphs never see them move.
   if (e == cudaSuccess) e = prepare_paged_decode();
   if (e == cudaSuccess) e = prepare_paged_chunk16();
+  if (e == cudaSuccess) e = prepare_paged_chunk32();
   if (e == cudaSuccess) e = prepare_sample();
   if (e == cudaSuccess) e = alloc_paged(c, group);
   if (e == cudaSuccess) {
@@ -1743,7 +1744,7 @@ int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv,
   p.status = c->status;
   cudaStream_t st = (cudaStream_t)stream;
   if (max_new > 1 && kv->dtype == GQA_F32)
-    GQA_CUDA(launch_paged_chunks(p, kv->dtype, hd, st, c->pdl != 0));
+    GQA_CUDA(launch_paged_chunk32(p, c->paged, hd, c->n_sm, st, c->pdl != 0));
   else if (max_new > 1)
     GQA_CUDA(launch_paged_chunk16(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));
   GQA_CUDA(launch_paged_decode(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));

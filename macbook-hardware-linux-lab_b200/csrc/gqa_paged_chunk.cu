@@ -31,9 +31,7 @@
 #include <cudaTypedefs.h>
 #include <math_constants.h>
 
-#include "gqa_paged.cuh"
-#include "gqa_paged_launch.cuh"
-#include "gqa_tc.cuh"
+#include "gqa_paged_chunk.cuh"
 
 namespace gqa {
 
@@ -41,22 +39,7 @@ namespace {
 
 constexpr int kKeys = 128;
 constexpr int kThreads = 320;
-constexpr int kRowsTile = 128;
-
-template <int G>
-__host__ __device__ constexpr int tile_tokens() { return kRowsTile / G; }
-template <int G>
-__host__ __device__ constexpr int unit_tokens() { return 2 * tile_tokens<G>(); }
-
-// One piece of a CTA's share: key tiles [kt0, kt1) of a unit.
-struct Piece {
-  int seq, head;
-  int tok, n_tok;  // the unit's first token row and its tokens
-  int pos;         // position of the first
-  int len;         // rows of the sequence
-  int kt0, kt1;
-  int slot;        // -1: the unit is whole here
-};
+constexpr int kRowsTile = kChunkRows;
 
 template <int D>
 struct alignas(1024) Smem {
@@ -73,8 +56,6 @@ struct alignas(1024) Smem {
   uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_final[2], drain;
   long long scan[kThreads / 32];
-  long long found_before;
-  int found_seq;
   uint32_t tmem_base;
   int err;
 };
@@ -101,21 +82,6 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
   const uint32_t t = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
   return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)b_mn_major << 16) |
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc));
-}
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc));
 }
 
 __device__ __forceinline__ void tma_load4(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
@@ -158,123 +124,6 @@ __device__ __forceinline__ uint32_t drop_non_finite2(uint32_t x) {
   if (((x >> 16) & e) == e) x &= 0xffffu;
   return x;
 }
-
-// The new tokens of sequence s and its rows, when this kernel takes them (two or more).
-__device__ __forceinline__ bool chunk_of(const PagedAttnParams& p, int s, int& tok, int& n_new,
-                                         int& len) {
-  tok = p.plan.q_starts[s];
-  const long long n = p.plan.q_starts[s + 1] - (long long)tok;
-  if (n < 2 || n > p.max_new || tok < 0 || tok + n > p.plan.n_tokens) return false;
-  int pos;
-  return place_token(p.plan, p.kv, s, tok, pos, n_new, len) == kPlaced && len <= p.max_len;
-}
-
-// Key tiles of a unit of the chunk.
-template <int G>
-__device__ __forceinline__ int unit_tiles(int n_new, int len, int unit) {
-  return (len - n_new + min(n_new, (unit + 1) * unit_tokens<G>()) + kKeys - 1) / kKeys;
-}
-template <int G>
-__device__ __forceinline__ long long chunk_tiles(int n_new, int len) {
-  long long sum = 0;
-  for (int u = 0; u * unit_tokens<G>() < n_new; ++u) sum += unit_tiles<G>(n_new, len, u);
-  return sum;
-}
-
-// q rotated into the rows of out: one thread per (token, KV head, 16-byte chunk of the
-// first half of a row), all heads of the group.
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(256) rotate_q_kernel(const PagedAttnParams p) {
-  using V = Vec16<T>;
-  constexpr int kChunks = D / 2 / V::n;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int per_token = p.n_kv * kChunks;
-  const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long last = (long long)p.plan.n_tokens * per_token - 1;
-  const int tok = (int)(min(item, last) / per_token);
-  const int tok0 = __shfl_sync(0xffffffffu, tok, 0);
-  int s = find_sequence(p.plan.q_starts, p.plan.n_seq, tok0);
-  while (s + 1 < p.plan.n_seq && p.plan.q_starts[s + 1] <= tok) ++s;
-  if (item > last) return;
-  int first, n_new, len;
-  if (!chunk_of(p, s, first, n_new, len) || tok < first || tok >= first + n_new) {
-    return;  // (another kernel's sequence, or one that is reported there)
-  }
-  const int pos = len - n_new + tok - first;
-  const int rem = (int)(item - (long long)tok * per_token);
-  const int h = rem / kChunks, c = rem % kChunks;
-  float co[V::n], si[V::n];
-#pragma unroll
-  for (int e = 0; e < V::n; ++e) rope_cos_sin(pos, p.turns[c * V::n + e], co[e], si[e]);
-  const T* src = static_cast<const T*>(p.qkv) + (long long)tok * p.qkv_stride +
-                 (long long)h * G * D + c * V::n;
-  T* dst = static_cast<T*>(p.out) + (long long)tok * p.out_stride + (long long)h * G * D +
-           c * V::n;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const V a = *reinterpret_cast<const V*>(src + g * D);
-    const V b = *reinterpret_cast<const V*>(src + g * D + D / 2);
-    V y0, y1;
-#pragma unroll
-    for (int e = 0; e < V::n; ++e) {
-      const float x = Elem<T>::get(a.e[e]), y = Elem<T>::get(b.e[e]);
-      y0.e[e] = Elem<T>::put(x * co[e] - y * si[e]);
-      y1.e[e] = Elem<T>::put(x * si[e] + y * co[e]);
-    }
-    *reinterpret_cast<V*>(dst + g * D) = y0;
-    *reinterpret_cast<V*>(dst + g * D + D / 2) = y1;
-  }
-}
-
-// The pieces of a CTA's share, in order.
-template <int G>
-struct Walk {
-  long long tile, first, last, total, n;
-  long long seq_first;  // first tile of sequence seq
-  int seq;
-
-  __device__ bool next(const PagedAttnParams& p, const PagedPartials& part, Piece& out) {
-    while (tile < last && seq < p.plan.n_seq) {
-      int tok, n_new, len;
-      if (!chunk_of(p, seq, tok, n_new, len)) {
-        ++seq;
-        continue;
-      }
-      const long long per_head = chunk_tiles<G>(n_new, len);
-      if (tile >= seq_first + per_head * p.n_kv) {
-        seq_first += per_head * p.n_kv;
-        ++seq;
-        continue;
-      }
-      const int h = (int)((tile - seq_first) / per_head);
-      long long at = seq_first + h * per_head;  // first tile of the unit
-      int u = 0, tiles = unit_tiles<G>(n_new, len, 0);
-      while (tile >= at + tiles) {
-        at += tiles;
-        tiles = unit_tiles<G>(n_new, len, ++u);
-      }
-      out.seq = seq;
-      out.head = h;
-      out.tok = tok + u * unit_tokens<G>();
-      out.n_tok = min(unit_tokens<G>(), n_new - u * unit_tokens<G>());
-      out.pos = len - n_new + u * unit_tokens<G>();
-      out.len = len;
-      out.kt0 = (int)(tile - at);
-      out.kt1 = (int)min((long long)tiles, last - at);
-      const bool whole = out.kt0 == 0 && out.kt1 == tiles;
-      out.slot = whole ? -1 : 2 * (int)blockIdx.x + (tile == first ? 0 : 1);
-      if (!whole && out.kt0 == 0) {
-        const int last_cta = (int)(((at + tiles) * n + total - 1) / total) - 1;
-        part.chunk_jobs[blockIdx.x] = PagedChunkJob{out.tok, out.n_tok, h, out.slot,
-                                                    last_cta - (int)blockIdx.x + 1};
-      }
-      tile = at + out.kt1;
-      return true;
-    }
-    return false;
-  }
-};
 
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -328,34 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_launch_dependents();
 
-  // Tiles of all units, and this CTA's share of them.
-  Walk<G> walk{};
-  {
-    long long mine = 0;
-    for (int s = tid; s < p.plan.n_seq; s += kThreads) {
-      int tok, n_new, len;
-      if (chunk_of(p, s, tok, n_new, len))
-        mine += chunk_tiles<G>(n_new, len);
-      else if (blockIdx.x == 0 && p.plan.q_starts[s + 1] - (long long)p.plan.q_starts[s] > 1)
-        atomicOr(p.status, kStatusBadLength);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    if (lane == 0) sm.scan[warp] = mine;
-    if (tid == 0) part.chunk_jobs[blockIdx.x].n_parts = 0;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    long long total = 0;
-    for (int w = 0; w < kThreads / 32; ++w) total += sm.scan[w];
-    walk.total = total * p.n_kv;
-    walk.n = min((long long)gridDim.x, walk.total);
-    if (blockIdx.x < walk.n) {
-      walk.first = blockIdx.x * walk.total / walk.n;
-      walk.last = (blockIdx.x + 1) * walk.total / walk.n;
-    }
-    walk.tile = walk.first;
-  }
+  tc_fence_before();
+  Walk<2 * kTok, kKeys> walk;
+  walk.begin(p, part, sm.scan);
+  tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
 
   if (warp == 8) {
@@ -804,43 +629,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Merges the parts of units that crossed shares: a warp per row, blocks of 8 rows.
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(256) paged_chunk_merge_kernel(const PagedAttnParams p,
-                                                                const PagedPartials part) {
-  pdl_wait();
-  const PagedChunkJob job = part.chunk_jobs[blockIdx.x];
-  if (job.n_parts == 0) return;
-  constexpr int kTok = tile_tokens<G>(), E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int idx = blockIdx.y * 8 + (threadIdx.x >> 5);  // row of the unit's tokens
-  const int t = idx / G, g = idx % G;
-  if (t >= job.n_tok) return;
-  const int row = t < kTok ? idx : kRowsTile + (t - kTok) * G + g;
-  float m = -CUDART_INF_F, l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i = 0; i < job.n_parts; ++i) {
-    const int slot = i == 0 ? job.slot : 2 * ((int)blockIdx.x + i);
-    const long long at = (long long)slot * 2 * kRowsTile + row;
-    const float2 ml = part.chunk_ml[at];
-    float x[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = part.chunk_o[at * D + lane * E + e];
-    if (ml.y == 0.f) continue;
-    const float mm = fmaxf(m, ml.x);
-    const float a = exp2f(m - mm), b = exp2f(ml.x - mm);
-    m = mm;
-    l = l * a + ml.y * b;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + x[e] * b;
-  }
-  T* out = static_cast<T*>(p.out) + (long long)(job.tok + t) * p.out_stride +
-           (long long)(job.head * G + g) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = Elem<T>::put(l != 0.f ? o[e] / l : 0.f);
-}
-
 PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* f = nullptr;
@@ -895,14 +683,14 @@ cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int 
                                   256, 0, st, pdl, p);
   if (e != cudaSuccess) return e;
   const long long units =
-      ((long long)p.plan.n_tokens / unit_tokens<G>() + p.plan.n_seq) * p.n_kv;
+      ((long long)p.plan.n_tokens / (2 * tile_tokens<G>()) + p.plan.n_seq) * p.n_kv;
   const long long tiles = units * ((p.max_len + kKeys - 1) / kKeys);
   const int grid = (int)std::min<long long>(n_sm, tiles);
   e = launch_with_pdl(paged_chunk_kernel<T, D, G>, dim3(grid), kThreads, sizeof(Smem<D>) + 1024,
                       st, true, p, part, maps, hnd, box_rows);
   if (e != cudaSuccess) return e;
   return launch_with_pdl(paged_chunk_merge_kernel<T, D, G>,
-                         dim3(grid, (unit_tokens<G>() * G + 7) / 8), 256, 0, st, true, p, part);
+                         dim3(grid, ((2 * tile_tokens<G>()) * G + 7) / 8), 256, 0, st, true, p, part);
 }
 
 template <typename T, int D, int G>

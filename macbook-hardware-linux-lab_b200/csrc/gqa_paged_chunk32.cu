@@ -1,0 +1,579 @@
+// Attention of chunks of new tokens over a paged KV cache in fp32, on the
+// 5th-generation tensor cores.
+//
+// Each fp32 number enters as three bf16 terms (x = h + m + l, 8 significant bits each, to
+// 2^-25 of x), and a product of two as the six products of terms that matter (hh, hm, mh, mm,
+// hl, lh; the rest is below 2^-24): six bf16 matrix products in place of one, 279 TFLOP/s at
+// the measured bf16 rate against some 70 of the fp32 units, with fp32's accuracy.  bf16 terms
+// rather than fp16 ones (which would do with three products) because they have fp32's range:
+// no scales, and columns of V of very different size keep their digits.  The products of
+// small terms are added first.  Sums of many tiles are kept in registers: the tensor cores
+// add within a tile only (24 steps of 16 keys), so that how they round an addition cannot
+// build up over a long cache.
+//
+// Rows, units and shares are as in gqa_paged_chunk.cu, with one tile of 126 rows per unit and
+// 64 keys per tile (three terms of Q, K and V fill the shared memory).
+//
+// Warps 0-3: softmax (a row per thread, its output in registers); 4-7: read Q, K and V from
+// the pages, split them and write the operands; 8: MMA (9-11 only give their registers).  K and V have one place each: the
+// next tile is read into registers while this one is worked on.  Tensor memory: two S, two P
+// of three terms, one O of a single tile.
+#include "gqa_paged_chunk.cuh"
+
+namespace gqa {
+
+namespace {
+
+constexpr int kKeys = 64;
+constexpr int kThreads = 384;
+// Registers of a thread in each group of four warps; three groups of 168 at the launch.
+constexpr int kRegsSoftmax = 240, kRegsOperands = 184, kRegsMma = 80;
+static_assert(kRegsSoftmax + kRegsOperands + kRegsMma == 3 * 168, "the launch's registers");
+constexpr int kTerms = 3;
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 320;  // S: 2 x 64, P: 2 x 96, O: D
+
+template <int D, int G>
+struct alignas(1024) Smem {
+  uint16_t q[kTerms][kChunkRows * D];
+  uint16_t k[kTerms][kKeys * D];
+  uint16_t v[kTerms][kKeys * D];
+  uint8_t stage[4][4096];
+  Piece ring[4];
+  int poison[4];      // number of the last piece of this ring place with a non-finite V
+  uint8_t bad[4][4];  // per key tile: its 16-row parts without a page
+  uint64_t item_full[4], item_empty[4];
+  uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty;
+  uint64_t s_full[2], p_full, o_full, o_empty, drain;
+  long long scan[kThreads / 32];
+  Walk<tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
+  uint32_t tmem_base;
+  int err;
+};
+
+// Rows of 128 bytes in 64-column blocks, 128-byte swizzle; `rows` rows a block.  lead: bytes
+// between blocks (for operands read across their rows).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(lead >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn_major << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// x and y as three bf16 pairs.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&t)[kTerms]) {
+  t[0] = pack_bf16(x, y);
+  x -= __uint_as_float(t[0] << 16);
+  y -= __uint_as_float(t[0] & 0xffff0000u);
+  t[1] = pack_bf16(x, y);
+  x -= __uint_as_float(t[1] << 16);
+  y -= __uint_as_float(t[1] & 0xffff0000u);
+  t[2] = pack_bf16(x, y);
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+        "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Four floats of column c (a multiple of 4) of row r as three terms, at their place in an
+// operand of `rows` rows.
+template <int N>
+__device__ __forceinline__ void put4(uint16_t (*term)[N], int rows, int r, int c, float4 x) {
+  uint32_t a[kTerms], b[kTerms];
+  split3(x.x, x.y, a);
+  split3(x.z, x.w, b);
+  const int at = (c >> 6) * rows * 64 + r * 64 + ((((c & 63) >> 3) ^ (r & 7)) << 3) + (c & 7);
+#pragma unroll
+  for (int i = 0; i < kTerms; ++i)
+    *reinterpret_cast<uint2*>(term[i] + at) = make_uint2(a[i], b[i]);
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < CUDART_INF_F; }
+
+template <int D, int G>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_chunk32_kernel(const __grid_constant__ PagedAttnParams p,
+                         const __grid_constant__ PagedPartials part) {
+  extern __shared__ unsigned char smem_raw[];
+  using S = Smem<D, G>;
+  S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                ~static_cast<uintptr_t>(1023));
+  constexpr int kTok = tile_tokens<G>();
+  constexpr uint32_t kIdS = idesc(kKeys, false), kIdO = idesc(D, true);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* err = &sm.err;
+
+  if (tid == 0) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&sm.item_full[s], 1);
+      mbar_init(&sm.item_empty[s], 9);  // the MMA thread, the softmax and the operand warps
+      sm.poison[s] = -1;
+    }
+    mbar_init(&sm.q_full, 4);
+    mbar_init(&sm.k_full, 4);
+    mbar_init(&sm.v_full, 4);
+    mbar_init(&sm.p_full, 4);
+    mbar_init(&sm.o_empty, 4);
+    mbar_init(&sm.q_empty, 1);
+    mbar_init(&sm.k_empty, 1);
+    mbar_init(&sm.v_empty, 1);
+    mbar_init(&sm.s_full[0], 1);
+    mbar_init(&sm.s_full[1], 1);
+    mbar_init(&sm.o_full, 1);
+    mbar_init(&sm.drain, 1);
+    sm.err = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_addr(&sm.tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  tc_fence_before();
+  {
+    Walk<kTok, kKeys> walk;
+    walk.begin(p, part, sm.scan);
+    if (tid == 128) sm.walk = walk;  // (the thread that walks)
+  }
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  // A piece of the ring; false when another role gave up.
+  const auto take = [&](int n, Piece& pc) {
+    if (!wait_or_abort(&sm.item_full[n & 3], (n >> 2) & 1, err)) return false;
+    pc = sm.ring[n & 3];
+    return true;
+  };
+
+  if (warp >= 4 && warp < 8) {
+    // ---- operands ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOperands));
+    const int w = warp - 4;
+    constexpr int kLanes = D / 4;          // lanes that cover a row
+    constexpr int kSide = 32 / kLanes;     // rows side by side in a load
+    constexpr int kLoads = 16 / kSide;     // loads of a warp's 16 rows
+    const int sub = lane / kLanes, col = lane % kLanes * 4;
+    int t = 0;
+    bool ok = true;
+    for (int rd = 0; ok; ++rd) {
+      const int place = rd & 3;
+      if (w == 0) {  // this warp hands the pieces out
+        if (rd >= 4) ok = wait_or_abort(&sm.item_empty[place], ((rd >> 2) - 1) & 1, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          if (!sm.walk.next(p, part, sm.ring[place])) sm.ring[place].n_tok = 0;
+          mbar_arrive(&sm.item_full[place]);
+        }
+        __syncwarp();
+      }
+      Piece pc;
+      ok = __all_sync(0xffffffffu, take(rd, pc));
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[place]);
+      if (pc.n_tok == 0) break;
+
+      // K or V rows of the warp's part of key tile kt into registers.
+      int page = 0;
+      const auto look_up = [&](int kt) {
+        const int row = kt * kKeys + w * 16;
+        page = p.kv.n_pages;  // (nothing there)
+        if (row < pc.pos + pc.n_tok) {
+          page = page_of(p.kv, pc.seq, row);
+          if (page < 0 && lane == 0) atomicOr(p.status, kStatusBadPage);
+        }
+      };
+      const auto load = [&](const void* pool, int kt, float4 (&x)[kLoads]) {
+        const int row0 = kt * kKeys + w * 16;
+        const bool there = page >= 0 && page < p.kv.n_pages;
+        const float* src = static_cast<const float*>(pool) +
+                           (there ? row_offset(p.kv, page, pc.head, row0) : 0);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int r = i * kSide + sub;
+          x[i] = there && row0 + r < pc.pos + pc.n_tok
+                     ? __ldg(reinterpret_cast<const float4*>(src + r * p.kv.row_stride + col))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      };
+      float4 xk[kLoads], xv[kLoads];
+      look_up(pc.kt0);
+      load(p.kv.k, pc.kt0, xk);
+
+      // Q (rotated, in the rows of out)
+      if (rd > 0) ok = wait_or_abort(&sm.q_empty, (rd - 1) & 1, err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      for (int r0 = w * 32; r0 < w * 32 + 32; r0 += kSide * 4) {
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = r0 + i * kSide + sub, tk = r / G;
+          x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < kTok * G && tk < pc.n_tok)
+            x[i] = *reinterpret_cast<const float4*>(
+                static_cast<const float*>(p.out) + (long long)(pc.tok + tk) * p.out_stride +
+                (long long)(pc.head * G + r % G) * D + col);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put4(sm.q, kChunkRows, r0 + i * kSide + sub, col, x[i]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full);
+
+      for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++t) {
+        load(p.kv.v, kt, xv);
+        if (t > 0) ok = wait_or_abort(&sm.k_empty, (t - 1) & 1, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) put4(sm.k, kKeys, w * 16 + i * kSide + sub, col, xk[i]);
+        if (lane == 0) sm.bad[t & 3][w] = page < 0;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.k_full);
+        if (kt + 1 < pc.kt1) {
+          look_up(kt + 1);
+          load(p.kv.k, kt + 1, xk);
+        }
+        // A weight of zero does not cancel an infinity or a NaN (and the terms of a weight
+        // have signs): what is not finite stays out of the product, and is added at the end to
+        // the rows that see it.
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          float4& x = xv[i];
+          if (!(finite(x.x) && finite(x.y) && finite(x.z) && finite(x.w))) {
+            odd = true;
+            x.x = finite(x.x) ? x.x : 0.f;
+            x.y = finite(x.y) ? x.y : 0.f;
+            x.z = finite(x.z) ? x.z : 0.f;
+            x.w = finite(x.w) ? x.w : 0.f;
+          }
+        }
+        if (odd) *reinterpret_cast<volatile int*>(&sm.poison[place]) = rd;
+        if (t > 0) ok = wait_or_abort(&sm.v_empty, (t - 1) & 1, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) put4(sm.v, kKeys, w * 16 + i * kSide + sub, col, xv[i]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.v_full);
+      }
+    }
+    if (!ok) atomicOr(&sm.err, 1);
+  } else if (warp >= 8) {
+    // ---- MMA issuer ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
+    if (warp == 8 && lane == 0) {
+      // Pairs of terms, small products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), a digit each.
+      // (Not unrolled: the descriptors of all products would not fit the registers.)
+      constexpr uint32_t kA = 0x001102, kB = 0x010120;
+      const auto issue_s = [&](int t) {
+        bool acc = false;
+#pragma unroll 1
+        for (int i = 0; i < 6; ++i) {
+          const uint32_t q = smem_addr(sm.q[kA >> 4 * i & 15]);
+          const uint32_t k = smem_addr(sm.k[kB >> 4 * i & 15]);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t in = (ks & 3) * 32;
+            umma_ss(tmem + kColS + 64 * (t & 1),
+                    smem_desc(q + (ks >> 2) * (kChunkRows * 128) + in, 16),
+                    smem_desc(k + (ks >> 2) * (kKeys * 128) + in, 16), kIdS, acc);
+            acc = true;
+          }
+        }
+        umma_commit(&sm.s_full[t & 1]);
+        umma_commit(&sm.k_empty);
+      };
+      const auto issue_pv = [&](int t) {
+        bool acc = false;
+#pragma unroll 1
+        for (int i = 0; i < 6; ++i) {
+          const uint32_t v = smem_addr(sm.v[kB >> 4 * i & 15]);
+          const uint32_t p_at = tmem + kColP + 96 * (t & 1) + 32 * (kA >> 4 * i & 15);
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks) {
+            umma_ts(tmem + kColO, p_at + ks * 8, smem_desc(v + ks * 2048, kKeys * 128), kIdO, acc);
+            acc = true;
+          }
+        }
+        umma_commit(&sm.o_full);
+        umma_commit(&sm.v_empty);
+      };
+      Piece pc{};
+      int rd = 0, t = 0;
+      bool ok = take(0, pc);
+      if (ok) mbar_arrive(&sm.item_empty[0]);
+      if (ok && pc.n_tok > 0) {
+        ok = wait_or_abort(&sm.q_full, 0, err) && wait_or_abort(&sm.k_full, 0, err);
+        if (ok) {
+          tc_fence_after();
+          issue_s(0);
+          if (pc.kt1 - pc.kt0 == 1) umma_commit(&sm.q_empty);
+        }
+      }
+      int kt = pc.kt0;
+      while (ok && pc.n_tok > 0) {
+        Piece nx = pc;
+        int kt_n = kt + 1;
+        const bool last = kt_n == pc.kt1;
+        if (last) {
+          ok = take(++rd, nx);
+          if (!ok) break;
+          mbar_arrive(&sm.item_empty[rd & 3]);
+          kt_n = nx.kt0;
+        }
+        if (nx.n_tok > 0) {
+          if ((last && !wait_or_abort(&sm.q_full, rd & 1, err)) ||
+              !wait_or_abort(&sm.k_full, (t + 1) & 1, err)) { ok = false; break; }
+          tc_fence_after();
+          issue_s(t + 1);
+          if (kt_n + 1 == nx.kt1) umma_commit(&sm.q_empty);
+        }
+        if (!wait_or_abort(&sm.p_full, t & 1, err) || !wait_or_abort(&sm.v_full, t & 1, err) ||
+            (t > 0 && !wait_or_abort(&sm.o_empty, (t - 1) & 1, err))) { ok = false; break; }
+        tc_fence_after();
+        issue_pv(t);
+        pc = nx;
+        kt = kt_n;
+        ++t;
+      }
+      umma_commit(&sm.drain);  // no MMA may be running when tensor memory is freed
+      mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread = row r (token r / G, head r % G) ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int r = tid;
+    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    const float sc = p.scale_log2;
+    uint8_t* stage = sm.stage[warp];
+    int t = 0;
+    bool ok = true;
+    for (int rd = 0; ok; ++rd) {
+      Piece pc;
+      ok = __all_sync(0xffffffffu, take(rd, pc));
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[rd & 3]);
+      if (pc.n_tok == 0) break;
+      const int limit = pc.pos + min(r / G, pc.n_tok - 1);  // last key of this row
+      float m = -CUDART_INF_F, l = 0.f, o[D];
+#pragma unroll
+      for (int e = 0; e < D; ++e) o[e] = 0.f;
+      // Adds the product of tile n to the row.
+      const auto add_o = [&](int n) {
+        const bool good = __all_sync(0xffffffffu, wait_or_abort(&sm.o_full, n & 1, err));
+        if (!good) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          tmem_ld32(t_lane + kColO + c * 32, v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[c * 32 + e] += v[e];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.o_empty);
+        return true;
+      };
+      for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++t) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&sm.s_full[t & 1], (t >> 1) & 1, err));
+        if (!ok) break;
+        tc_fence_after();
+        const int lim = limit - kt * kKeys;
+        const uint32_t bad = *reinterpret_cast<const uint32_t*>(sm.bad[t & 3]);
+        // Half a row of scores at a time (read twice: a whole one beside the output's
+        // registers would not fit).
+        const auto scores = [&](int half, float (&s)[32]) {
+          tmem_ld32(t_lane + kColS + 64 * (t & 1) + 32 * half, s);
+          if (lim < 32 * half + 31) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (32 * half + c > lim) s[c] = -CUDART_INF_F;
+          }
+          if (bad) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (bad >> ((2 * half + c / 16) * 8) & 1) s[c] = -CUDART_INF_F;
+          }
+        };
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float s[32];
+          scores(half, s);
+          float mx0 = s[0], mx1 = s[1];
+#pragma unroll
+          for (int c = 2; c < 30; c += 4) {
+            mx0 = fmax3(mx0, s[c], s[c + 1]);
+            mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+          }
+          top = fmax3(top, fmax3(mx0, s[30], s[31]), mx1);
+        }
+        const float mn = fmaxf(m, top * sc);
+        const float alpha = mn == m ? 1.f : exp2f(m - mn);
+        m = mn;
+        const float ref = m == -CUDART_INF_F ? 0.f : m;
+        float sum0 = 0.f, sum1 = 0.f;
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float s[32];
+          scores(half, s);
+#pragma unroll
+          for (int c = 0; c < 32; c += 16) {
+            uint32_t pk[kTerms][8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float p0 = exp2f(fmaf(s[c + e], sc, -ref));
+              const float p1 = exp2f(fmaf(s[c + e + 1], sc, -ref));
+              sum0 += p0;
+              sum1 += p1;
+              uint32_t x[kTerms];
+              split3(p0, p1, x);
+#pragma unroll
+              for (int i = 0; i < kTerms; ++i) pk[i][e / 2] = x[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kTerms; ++i)
+              tmem_st8(t_lane + kColP + 96 * (t & 1) + 32 * i + 16 * half + c / 2, pk[i]);
+          }
+        }
+        tmem_wait_st();
+        l = l * alpha + (sum0 + sum1);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full);
+        if (kt > pc.kt0) {
+          ok = add_o(t - 1);
+          if (!ok) break;
+        }
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int e = 0; e < D; ++e) o[e] *= alpha;
+        }
+      }
+      if (!ok) break;
+      ok = add_o(t - 1);
+      if (!ok) break;
+      if (*reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) == rd) {
+        for (int key = pc.kt0 * kKeys; key <= limit && key < pc.kt1 * kKeys; ++key) {
+          const int page = page_of(p.kv, pc.seq, key);
+          if (page < 0) continue;
+          const float4* row = reinterpret_cast<const float4*>(
+              static_cast<const float*>(p.kv.v) + row_offset(p.kv, page, pc.head, key));
+#pragma unroll
+          for (int c = 0; c < D / 4; ++c) {
+            const float4 x = row[c];
+            if (!finite(x.x)) o[4 * c] += x.x;
+            if (!finite(x.y)) o[4 * c + 1] += x.y;
+            if (!finite(x.z)) o[4 * c + 2] += x.z;
+            if (!finite(x.w)) o[4 * c + 3] += x.w;
+          }
+        }
+      }
+      // Rows leave through the warp's 4 KB: written a row per thread, read back so that eight
+      // lanes cover 128 bytes of a row (16-byte chunk c of row i at c ^ (i % 8)).
+      const bool whole = pc.slot < 0;
+      const float by = !whole ? 1.f : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const long long base = (long long)pc.slot * kChunkSlotRows + warp * 32;
+      if (!whole) part.chunk_ml[base + lane] = make_float2(m, l);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+              make_float4(o[b * 32 + 4 * c] * by, o[b * 32 + 4 * c + 1] * by,
+                          o[b * 32 + 4 * c + 2] * by, o[b * 32 + 4 * c + 3] * by);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = i * 4 + (lane >> 3), c = lane & 7;
+          const float4 x = *reinterpret_cast<const float4*>(stage + rr * 128 +
+                                                            ((c ^ (rr & 7)) << 4));
+          const int row = warp * 32 + rr, tk = row / G;
+          if (!whole)
+            *reinterpret_cast<float4*>(part.chunk_o + (base + rr) * D + b * 32 + c * 4) = x;
+          else if (row < kTok * G && tk < pc.n_tok)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) +
+                                       (long long)(pc.tok + tk) * p.out_stride +
+                                       (long long)(pc.head * G + row % G) * D + b * 32 + c * 4) = x;
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) atomicOr(&sm.err, 1);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && sm.err) atomicOr(p.status, kStatusWaitTimeout);
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+template <int D, int G>
+cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int n_sm,
+                       cudaStream_t st, bool pdl) {
+  constexpr int kTok = tile_tokens<G>();
+  const long long items = (long long)p.plan.n_tokens * p.n_kv * (D / 2 / Vec16<float>::n);
+  cudaError_t e = launch_with_pdl(rotate_q_kernel<float, D, G>,
+                                  dim3((unsigned)((items + 255) / 256)), 256, 0, st, pdl, p);
+  if (e != cudaSuccess) return e;
+  const long long units = ((long long)p.plan.n_tokens / kTok + p.plan.n_seq) * p.n_kv;
+  const long long tiles = units * ((p.max_len + kKeys - 1) / kKeys);
+  const int grid = (int)std::min<long long>(n_sm, tiles);
+  e = launch_with_pdl(paged_chunk32_kernel<D, G>, dim3(grid), kThreads, sizeof(Smem<D, G>) + 1024, st,
+                      true, p, part);
+  if (e != cudaSuccess) return e;
+  return launch_with_pdl(paged_chunk_merge_kernel<float, D, G>, dim3(grid, (kTok * G + 7) / 8), 256,
+                         0, st, true, p, part);
+}
+
+template <int D, int G>
+constexpr int kSmemBytes = (int)sizeof(Smem<D, G>) + 1024;
+
+}  // namespace
+
+cudaError_t prepare_paged_chunk32() {
+  cudaError_t e = cudaFuncSetAttribute((const void*)paged_chunk32_kernel<128, 6>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kSmemBytes<128, 6>);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute((const void*)paged_chunk32_kernel<64, 7>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<64, 7>);
+  return e;
+}
+
+cudaError_t launch_paged_chunk32(const PagedAttnParams& p, const PagedPartials& part, int head_dim,
+                                 int n_sm, cudaStream_t st, bool pdl) {
+  return head_dim == 128 ? launch_one<128, 6>(p, part, n_sm, st, pdl)
+                         : launch_one<64, 7>(p, part, n_sm, st, pdl);
+}
+
+}  // namespace gqa

@@ -57,7 +57,8 @@ cudaError_t launch_paged_decode(const PagedAttnParams& p, const PagedPartials& p
 cudaError_t prepare_paged_chunk16();
 cudaError_t launch_paged_chunk16(const PagedAttnParams& p, const PagedPartials& part, int dtype,
                                  int head_dim, int n_sm, cudaStream_t st, bool pdl);
-cudaError_t launch_paged_chunks(const PagedAttnParams& p, int dtype, int head_dim,
-                                cudaStream_t st, bool pdl);
+cudaError_t prepare_paged_chunk32();
+cudaError_t launch_paged_chunk32(const PagedAttnParams& p, const PagedPartials& part, int head_dim,
+                                 int n_sm, cudaStream_t st, bool pdl);
 
 }  // namespace gqa
