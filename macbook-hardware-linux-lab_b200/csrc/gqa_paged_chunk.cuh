@@ -200,24 +200,42 @@ __global__ void __launch_bounds__(256) paged_chunk_merge_kernel(const PagedAttnP
   const int t = idx / G, g = idx % G;
   if (t >= job.n_tok) return;
   const int row = t < kTok ? idx : kChunkRows + (t - kTok) * G + g;
+  const auto at = [&](int i) {
+    return (long long)(i == 0 ? job.slot : 2 * ((int)blockIdx.x + i)) * kChunkSlotRows + row;
+  };
+  // the parts' weights, a part per lane; then loads that depend on nothing
   float m = -CUDART_INF_F, l = 0.f, o[E];
+  for (int i = lane; i < job.n_parts; i += 32) {
+    const float2 ml = part.chunk_ml[at(i)];
+    if (ml.y != 0.f) m = fmaxf(m, ml.x);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i = 0; i < job.n_parts; ++i) {
-    const int slot = i == 0 ? job.slot : 2 * ((int)blockIdx.x + i);
-    const long long at = (long long)slot * kChunkSlotRows + row;
-    const float2 ml = part.chunk_ml[at];
-    float x[E];
+  for (int i0 = 0; i0 < job.n_parts; i0 += 32) {
+    float2 ml = make_float2(0.f, 0.f);
+    if (i0 + lane < job.n_parts) ml = part.chunk_ml[at(i0 + lane)];
+    const float weight = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
+    l += weight * ml.y;
+    for (int i = i0; i < min(i0 + 32, job.n_parts); i += 8) {
+      float x[8][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = part.chunk_o[at * D + lane * E + e];
-    if (ml.y == 0.f) continue;
-    const float mm = fmaxf(m, ml.x);
-    const float a = exp2f(m - mm), b = exp2f(ml.x - mm);
-    m = mm;
-    l = l * a + ml.y * b;
+      for (int u = 0; u < 8; ++u)
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + x[e] * b;
+        for (int e = 0; e < E; ++e)
+          x[u][e] = i + u < job.n_parts ? part.chunk_o[at(i + u) * D + lane * E + e] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float a = __shfl_sync(0xffffffffu, weight, i - i0 + u);
+        if (a != 0.f)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += a * x[u][e];
+      }
+    }
   }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
   T* out = static_cast<T*>(p.out) + (long long)(job.tok + t) * p.out_stride +
            (long long)(job.head * G + g) * D + lane * E;
 #pragma unroll

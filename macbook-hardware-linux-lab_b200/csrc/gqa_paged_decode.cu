@@ -581,59 +581,81 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedAt
   }
 }
 
-// Merges the parts of a pair: one block per (CTA that holds a first part, query head).
+// Merges the parts of a pair: one block per (CTA that holds a first part, query head).  The
+// parts' weights first (a part per thread), so that the loads of the outputs depend on nothing
+// and go out together.
 constexpr int kMergeWarps = 8;
+constexpr int kMaxParts = 512;  // two CTAs on each SM of the largest parts, and some
 
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(kMergeWarps * 32)
     paged_merge_kernel(const PagedAttnParams p, const PagedPartials part) {
-  __shared__ float sm[kMergeWarps], sl[kMergeWarps], so[kMergeWarps][D];
+  __shared__ float weight[kMaxParts], red[2][kMergeWarps], so[kMergeWarps][D];
   pdl_wait();
   const PagedJob job = part.jobs[blockIdx.x];
   if (job.n_parts == 0) return;
-  const int g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // the first part's slot, then slot 0 of each CTA after it
   const auto slot_of = [&](int i) { return i == 0 ? job.slot : 2 * ((int)blockIdx.x + i); };
+  constexpr int kOwn = kMaxParts / (kMergeWarps * 32);
+  float2 ml[kOwn];
+  float m = -CUDART_INF_F;
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    const int i = tid + j * kMergeWarps * 32;
+    ml[j] = i < job.n_parts ? part.ml[slot_of(i) * G + g] : make_float2(-CUDART_INF_F, 0.f);
+    if (ml[j].y != 0.f) m = fmaxf(m, ml[j].x);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, red[0][w]);
+  float l = 0.f;
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    const float a = ml[j].y != 0.f ? exp2f(ml[j].x - m) : 0.f;
+    l += a * ml[j].y;
+    weight[tid + j * kMergeWarps * 32] = a;
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) l += red[1][w];
   constexpr int E = D / 32;
-  float m = -CUDART_INF_F, l = 0.f, o[E];
+  float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i = warp; i < job.n_parts; i += kMergeWarps) {
-    const float2 ml = part.ml[slot_of(i) * G + g];
-    const float* src = part.o + ((long long)slot_of(i) * G + g) * D + lane * E;
-    float x[E];
+  for (int i0 = warp; i0 < job.n_parts; i0 += 8 * kMergeWarps) {
+    float x[8][E], a[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = src[e];
-    if (ml.y == 0.f) continue;
-    const float mm = fmaxf(m, ml.x);
-    const float a = exp2f(m - mm), b = exp2f(ml.x - mm);
-    m = mm;
-    l = l * a + ml.y * b;
+    for (int u = 0; u < 8; ++u) {
+      const int i = min(i0 + u * kMergeWarps, job.n_parts - 1);
+      a[u] = i0 + u * kMergeWarps < job.n_parts ? weight[i] : 0.f;
+      const float* src = part.o + ((long long)slot_of(i) * G + g) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + x[e] * b;
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+      for (int e = 0; e < E; ++e) x[u][e] = src[e];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (a[u] != 0.f)  // (a part without a row holds nothing to be added)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += a[u] * x[u][e];
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
   __syncthreads();
   T* out = static_cast<T*>(p.out) + (long long)job.tok * p.out_stride +
            (long long)(job.head * G + g) * D;
-  for (int e = threadIdx.x; e < D; e += kMergeWarps * 32) {
-    float mm = -CUDART_INF_F;
+  for (int e = tid; e < D; e += kMergeWarps * 32) {
+    float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) mm = fmaxf(mm, sm[w]);
-    float ll = 0.f, oo = 0.f;
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) {
-      if (sl[w] == 0.f) continue;
-      const float a = exp2f(sm[w] - mm);
-      ll += a * sl[w];
-      oo += a * so[w][e];
-    }
-    out[e] = Elem<T>::put(ll != 0.f ? oo / ll : 0.f);
+    for (int w = 0; w < kMergeWarps; ++w) sum += so[w][e];
+    out[e] = Elem<T>::put(l != 0.f ? sum / l : 0.f);
   }
 }
 
@@ -649,7 +671,7 @@ cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int 
                        cudaStream_t st, bool pdl) {
   const long long tiles =
       (long long)p.plan.n_seq * p.n_kv * ((p.max_len + tile_rows<T>() - 1) / tile_rows<T>());
-  const long long most = std::min<long long>(2LL * n_sm, part.n_ctas);
+  const long long most = std::min<long long>({2LL * n_sm, part.n_ctas, kMaxParts});
   const int grid = (int)std::min(most, tiles);
   cudaError_t e = launch_with_pdl(paged_decode_kernel<T, D, G>, dim3(grid), kThreads,
                                   sizeof(Smem<T, D>), st, pdl, p, part);
