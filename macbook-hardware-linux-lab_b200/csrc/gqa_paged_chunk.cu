@@ -23,8 +23,10 @@
 // there is what the projection before it would do with a rotated q; scores and sums are
 // fp32, weights are rounded to the type for the second product.
 //
-// Warps 0-3 / 4-7: softmax of tile A / B, a row per thread; 8: loader (TMA of the pages);
-// 9: MMA.  Tensor memory: S_A | S_B | O_A | O_B, P over the first half of its S.
+// Warps 0-7 / 8-15: softmax of tile A / B, two threads per row (64 keys each: with one thread a
+// row, two warps a scheduler waited for their own instructions, 1800 clocks a tile against 1024
+// of the exponential unit); 16: loader (TMA of the pages); 17: MMA.  Tensor memory: S_A | S_B |
+// O_A | O_B, the P of each half of the keys over the first half of its scores.
 // Every wait is bounded; a wait that runs out sets the status bit, and the CTA drains
 // what it issued and returns its tensor memory.
 #include <cuda.h>
@@ -38,15 +40,16 @@ namespace gqa {
 namespace {
 
 constexpr int kKeys = 128;
-constexpr int kThreads = 320;
+constexpr int kSoftmaxWarps = 16, kLoader = 16, kMma = 17;
+constexpr int kThreads = 18 * 32;
 constexpr int kRowsTile = kChunkRows;
 
-template <int D>
+template <int D, int G>
 struct alignas(1024) Smem {
   uint16_t q[2][kRowsTile * D];
   uint16_t k[2][kKeys * D];
   uint16_t v[2][kKeys * D];
-  uint8_t stage[8][4096];
+  float xch[2][2][2][kRowsTile];  // [turn][tile A, B][half of the keys][row]: maxima, sums
   Piece ring[4];
   int poison[4];         // number of the last piece of this ring place with a non-finite V
   // per key tile: its 16-row parts without a page (four tiles: the softmax of a tile may
@@ -55,7 +58,8 @@ struct alignas(1024) Smem {
   uint64_t item_full[4], item_empty[4];
   uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_final[2], drain;
-  long long scan[kThreads / 32];
+  long long scan[kThreads / 32], found[2];
+  Walk<2 * tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
   uint32_t tmem_base;
   int err;
 };
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ PagedPartials part,
                        const __grid_constant__ ChunkMaps maps, const int hnd, const int box_rows) {
   extern __shared__ unsigned char smem_raw[];
-  using S = Smem<D>;
+  using S = Smem<D, G>;
   S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                 ~static_cast<uintptr_t>(1023));
   constexpr int kTok = tile_tokens<G>();
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < 4; ++s) {
       mbar_init(&sm.item_full[s], 1);
-      mbar_init(&sm.item_empty[s], 9);  // the MMA thread and the softmax warps
+      mbar_init(&sm.item_empty[s], 1 + kSoftmaxWarps);  // the MMA thread and the softmax warps
       sm.poison[s] = -1;
     }
     for (int s = 0; s < 2; ++s) {
@@ -156,14 +160,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.v_full[s], 1);
       mbar_init(&sm.v_empty[s], 1);
       mbar_init(&sm.s_full[s], 1);
-      mbar_init(&sm.p_full[s], 4);
+      mbar_init(&sm.p_full[s], kSoftmaxWarps / 2);
       mbar_init(&sm.o_final[s], 1);
     }
     mbar_init(&sm.drain, 1);
     sm.err = 0;
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_addr(&sm.tmem_base)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -174,18 +178,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm.q[b / kBlocks][(b % kBlocks) * kRowsTile * 64 + (kTok * G + r) * 64 + x] = 0;
   }
   fence_proxy_async_smem();
-  pdl_wait();
+  // The kernel before this one waited for all that came before it and wrote only q: the plan,
+  // the pages and the slots can be used before it is done.
   pdl_launch_dependents();
-
   tc_fence_before();
-  Walk<2 * kTok, kKeys> walk;
-  walk.begin(p, part, sm.scan);
+  {
+    Walk<2 * kTok, kKeys> walk;
+    walk.begin(p, part, sm.scan, sm.found);
+    if (tid == kLoader * 32) sm.walk = walk;
+  }
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
 
-  if (warp == 8) {
+  if (warp == kLoader) {
     // ---- loader ----
-    const bool some = walk.first < walk.last;
+    bool waited = false;  // for q
     Piece pc{};
     int kv = 0, rd = 0, nq[2] = {0, 0};
     bool ok = true;
@@ -196,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!__all_sync(0xffffffffu, ok)) break;
       int more = 0;
       if (lane == 0) {
-        more = some && walk.next(p, part, pc);
+        more = sm.walk.next(p, part, pc);
         if (!more) pc.n_tok = 0;
         sm.ring[place] = pc;
         mbar_arrive(&sm.item_full[place]);
@@ -211,6 +218,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = __shfl_sync(0xffffffffu, pc.len, 0);
       const int kt0 = __shfl_sync(0xffffffffu, pc.kt0, 0);
       const int kt1 = __shfl_sync(0xffffffffu, pc.kt1, 0);
+      if (!waited) pdl_wait();
+      waited = true;
       for (int g = 0; g < (n_tok > kTok ? 2 : 1) && ok; ++g, __syncwarp()) {
         if (nq[g] > 0) ok = wait_or_abort(&sm.q_empty[g], (nq[g] - 1) & 1, err);
         ok = __all_sync(0xffffffffu, ok);
@@ -274,6 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
     }
+    if (!waited) pdl_wait();  // (the grid must not end before the one whose q it stands for)
     if (*err && lane == 0) {
       // Let the copies already issued land before the CTA's shared memory is handed on
       // (a phase that was never armed runs into the wait's bound).
@@ -287,11 +297,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ---- MMA issuer ----
-    if (lane == 0) {
+  } else if (warp == kMma) {
+    // ---- MMA issuer (the whole warp, one lane issues) ----
+    const auto all_wait = [&](uint64_t* bar, uint32_t parity, volatile int* e) {
+      return (bool)__all_sync(0xffffffffu, wait_or_abort(bar, parity, e));
+    };
+    {
       const auto issue_s = [&](int g, int kv) {
         const uint32_t q = smem_addr(sm.q[g]), k = smem_addr(sm.k[kv & 1]);
+        if (!elect_one()) return;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
@@ -301,16 +315,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       const auto issue_pv = [&](int g, int kv, bool acc) {
         const uint32_t v = smem_addr(sm.v[kv & 1]);
+        if (!elect_one()) return;
 #pragma unroll
         for (int ks = 0; ks < kKeys / 16; ++ks)
-          umma_ts(tmem + 256 + 128 * g, tmem + 128 * g + ks * 8, desc_mn_major(v + ks * 2048), kIdO,
-                  acc || ks > 0);
+          umma_ts(tmem + 256 + 128 * g, tmem + 128 * g + (ks & 3) * 8 + (ks >> 2) * 64,
+                  desc_mn_major(v + ks * 2048), kIdO, acc || ks > 0);
       };
       const auto take = [&](int n, Piece& pc) {
-        if (!wait_or_abort(&sm.item_full[n & 3], (n >> 2) & 1, err)) return false;
+        if (!all_wait(&sm.item_full[n & 3], (n >> 2) & 1, err)) return false;
         pc = sm.ring[n & 3];
-        mbar_arrive(&sm.item_empty[n & 3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[n & 3]);
         return true;
+      };
+      // (after the matrix instructions before it, whichever lane issued them: the elected lane
+      // is the same one throughout)
+      const auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+        __syncwarp();
       };
       Piece pc{};
       int rd = 0, kv = 0, nq[2] = {0, 0}, nt[2] = {0, 0};  // Q tiles, S tiles of A and B
@@ -319,26 +341,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       // S of the first key tile of a piece or of the next one
       const auto first_s = [&](int g, bool start) {
         if (start) {
-          if (!wait_or_abort(&sm.q_full[g], nq[g] & 1, err)) return false;
+          if (!all_wait(&sm.q_full[g], nq[g] & 1, err)) return false;
           ++nq[g];
         }
         return true;
       };
       if (ok && pc.n_tok > 0) {
         const bool lone = pc.kt1 - pc.kt0 == 1;
-        ok = wait_or_abort(&sm.k_full[0], 0, err) && first_s(0, true);
+        ok = all_wait(&sm.k_full[0], 0, err) && first_s(0, true);
         if (ok) {
           tc_fence_after();
           issue_s(0, 0);
-          if (lone) umma_commit(&sm.q_empty[0]);
+          if (lone) commit(&sm.q_empty[0]);
           if (two) ok = first_s(1, true);
         }
         if (ok && two) {
           tc_fence_after();
           issue_s(1, 0);
-          if (lone) umma_commit(&sm.q_empty[1]);
+          if (lone) commit(&sm.q_empty[1]);
         }
-        if (ok) umma_commit(&sm.k_empty[0]);
+        if (ok) commit(&sm.k_empty[0]);
       }
       int kt = pc.kt0;
       while (ok && pc.n_tok > 0) {
@@ -354,57 +376,66 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool more = nx.n_tok > 0, two_n = nx.n_tok > kTok;
         const bool n_last = kt_n + 1 == nx.kt1;
         const int kv_n = kv + 1;
-        if (!wait_or_abort(&sm.p_full[0], nt[0] & 1, err) ||
-            !wait_or_abort(&sm.v_full[kv & 1], (kv >> 1) & 1, err)) { ok = false; break; }
+        // What the loader brings is waited for first, while the softmax is still at work: the
+        // products then follow the weights at once, P V of this tile and S of the next.
+        ok = all_wait(&sm.v_full[kv & 1], (kv >> 1) & 1, err);
+        if (ok && more)
+          ok = first_s(0, last) && all_wait(&sm.k_full[kv_n & 1], (kv_n >> 1) & 1, err);
+        if (!ok || !all_wait(&sm.p_full[0], nt[0] & 1, err)) { ok = false; break; }
         ++nt[0];
         tc_fence_after();
         issue_pv(0, kv, kt > pc.kt0);
-        if (!two) umma_commit(&sm.v_empty[kv & 1]);
-        if (last) umma_commit(&sm.o_final[0]);
-        if (more) {
-          ok = first_s(0, last) &&
-               wait_or_abort(&sm.k_full[kv_n & 1], (kv_n >> 1) & 1, err);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(0, kv_n);
-          if (n_last) umma_commit(&sm.q_empty[0]);
-        }
+        if (more) issue_s(0, kv_n);
+        if (!two) commit(&sm.v_empty[kv & 1]);
+        if (last) commit(&sm.o_final[0]);
+        if (more && n_last) commit(&sm.q_empty[0]);
+        if (more && two_n && !first_s(1, last)) { ok = false; break; }
         if (two) {
-          if (!wait_or_abort(&sm.p_full[1], nt[1] & 1, err)) { ok = false; break; }
+          if (!all_wait(&sm.p_full[1], nt[1] & 1, err)) { ok = false; break; }
           ++nt[1];
           tc_fence_after();
           issue_pv(1, kv, kt > pc.kt0);
-          umma_commit(&sm.v_empty[kv & 1]);
-          if (last) umma_commit(&sm.o_final[1]);
+        }
+        if (more && two_n) issue_s(1, kv_n);
+        if (two) {
+          commit(&sm.v_empty[kv & 1]);
+          if (last) commit(&sm.o_final[1]);
         }
         if (more) {
-          if (two_n) {
-            ok = first_s(1, last);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(1, kv_n);
-            if (n_last) umma_commit(&sm.q_empty[1]);
-          }
-          umma_commit(&sm.k_empty[kv_n & 1]);
+          if (two_n && n_last) commit(&sm.q_empty[1]);
+          commit(&sm.k_empty[kv_n & 1]);
         }
         pc = nx;
         two = two_n;
         kt = kt_n;
         kv = kv_n;
       }
-      umma_commit(&sm.drain);  // no MMA may be running when tensor memory is freed
+      commit(&sm.drain);  // no MMA may be running when tensor memory is freed
       mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
     }
     __syncwarp();
   } else {
-    // ---- softmax of tile g: thread = row r (token r / G, head r % G) ----
-    const int g = warp >> 2, r = tid & 127;
+    // ---- softmax of tile g: row r (token r / G, head r % G), keys 64 half .. 64 half + 63 ----
+    const int g = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_off + 128 * g;
-    const uint32_t t_o = tmem + lane_off + 256 + 128 * g;
+    const uint32_t t_s = tmem + lane_off + 128 * g + 64 * half;
+    const uint32_t t_o = tmem + lane_off + 256 + 128 * g + D / 2 * half;  // its half of O
     const float sc = p.scale_log2;
-    uint8_t* stage = sm.stage[warp];
-    int tc = 0;  // S tiles of this half so far
+    // The two warps of 32 rows exchange a value per row; the places alternate, so that one
+    // meeting a turn is enough.  A warp that gives up arrives once more on its way out: its
+    // partner meets it there at most once before its own next wait gives up too.
+    const int meeting = 1 + g * 4 + (warp & 3);
+    int turn = 0;
+    const auto other = [&](float x) {
+      float(&box)[2][kRowsTile] = sm.xch[turn++ & 1][g];
+      box[half][r] = x;
+      named_barrier_sync(meeting, 64);
+      return box[half ^ 1][r];
+    };
+    // (whole 32-byte sectors: with 16-byte stores a row per thread writes each twice)
+    const bool wide_out =
+        (reinterpret_cast<uintptr_t>(p.out) | (uint64_t)p.out_stride * sizeof(T)) % 32 == 0;
+    int tc = 0;  // S tiles of this tile's so far
     int kv = 0;  // key tiles so far
     int done = 0;
     bool ok = true;
@@ -420,9 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         kv += pc.kt1 - pc.kt0;
         continue;
       }
-      const int my_tok = min(g * kTok + r / G, pc.n_tok - 1);
-      const int limit = pc.pos + my_tok;                // last key of this row
-      const int first_limit = pc.pos + g * kTok;        // of the tile's first row
+      const int limit = pc.pos + min(g * kTok + r / G, pc.n_tok - 1);  // last key of this row
+      const int first_limit = pc.pos + g * kTok;                       // of the tile's first row
       float m = -CUDART_INF_F, l = 0.f;
       for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++tc, ++kv) {
         ok = __all_sync(0xffffffffu, wait_or_abort(&sm.s_full[g], tc & 1, err));
@@ -430,63 +460,70 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const int key0 = kt * kKeys;
         const unsigned bad = sm.bad_rows[kv & 3];
-        float alpha = 1.f, sum0 = 0.f, sum1 = 0.f;
-        uint32_t pk[kKeys / 2];
-        // The reference m is the row's maximum of the piece's first tile; it moves when
-        // the weights of a tile add up to more than 2^8 (or m is still -inf), in a
-        // second pass over the tile.
-        bool fresh = __any_sync(0xffffffffu, m == -CUDART_INF_F);
-        const bool start = kt == pc.kt0;
-#pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
-          float s[kKeys];
-          tmem_ld128(t_s, s);
+        // 32 scores at a time, masked
+        const auto scores = [&](int c0, float (&s)[32]) {
+          tmem_ld32(t_s + c0, s);
           if (key0 + kKeys - 1 > first_limit) {
-            const int lim = limit - key0;
+            const int lim = limit - key0 - 64 * half - c0;
 #pragma unroll
-            for (int c = 0; c < kKeys; ++c)
+            for (int c = 0; c < 32; ++c)
               if (c > lim) s[c] = -CUDART_INF_F;
           }
           if (bad) {
+            const unsigned here = bad >> (4 * half + c0 / 16);
 #pragma unroll
-            for (int c = 0; c < kKeys; ++c)
-              if (bad >> (c / 16) & 1) s[c] = -CUDART_INF_F;
+            for (int c = 0; c < 32; ++c)
+              if (here >> (c / 16) & 1) s[c] = -CUDART_INF_F;
           }
-          if (fresh) {
-            float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+        };
+        const auto max32 = [&](const float (&s)[32]) {
+          float mx0 = s[0], mx1 = s[1];
 #pragma unroll
-            for (int c = 4; c < kKeys - 4; c += 8) {
-              mx0 = fmax3(mx0, s[c], s[c + 1]);
-              mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
-              mx2 = fmax3(mx2, s[c + 4], s[c + 5]);
-              mx3 = fmax3(mx3, s[c + 6], s[c + 7]);
-            }
-            mx0 = fmax3(mx0, s[kKeys - 4], s[kKeys - 3]);
-            mx1 = fmax3(mx1, s[kKeys - 2], s[kKeys - 1]);
-            const float mn = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc);
-            alpha = start || mn == m ? 1.f : fast_exp2(m - mn);
-            m = mn;
+          for (int c = 2; c < 30; c += 4) {
+            mx0 = fmax3(mx0, s[c], s[c + 1]);
+            mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
           }
-          const float nm = m == -CUDART_INF_F ? 0.f : -m;
-          sum0 = 0.f;
-          sum1 = 0.f;
+          return fmax3(fmaxf(mx0, mx1), s[30], s[31]);
+        };
+        float s[32];
+        scores(0, s);
+        float top = max32(s);
+        scores(32, s);
+        top = fmaxf(top, max32(s));
+        top = fmaxf(top, other(top)) * sc;
+        // The reference m moves to the row's maximum only when that has passed it by 2^8, so
+        // that O is rarely rescaled.
+        float alpha = 1.f;
+        if (top > m + 8.f) {
+          alpha = fast_exp2(m - top);
+          m = top;
+        }
+        const float nm = m == -CUDART_INF_F ? 0.f : -m;
+        float sum0 = 0.f, sum1 = 0.f;
+        const auto weights = [&](const float (&s)[32], uint32_t (&pk)[16]) {
 #pragma unroll
-          for (int c = 0; c < kKeys; c += 2) {
+          for (int c = 0; c < 32; c += 2) {
             float x0, x1;
             ffma2(x0, x1, s[c], s[c + 1], sc, sc, nm, nm);
             const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
             fadd2(sum0, sum1, sum0, sum1, p0, p1);
             pk[c / 2] = pack2<T>(p0, p1);
           }
-          if (fresh || !__any_sync(0xffffffffu, !(sum0 + sum1 <= 256.f))) break;
-          fresh = true;
-        }
+        };
+        // (the second 32 first, whose scores are at hand; no P is stored before the first 32
+        // have been read again, over whose place it goes)
+        uint32_t pk1[16], pk0[16];
+        weights(s, pk1);
+        scores(0, s);
+        weights(s, pk0);
         __syncwarp();
-        tmem_st64(t_s, pk);
+        tmem_st16(t_s, pk0);
+        tmem_st16(t_s + 16, pk1);
+        tmem_wait_st();
         l = l * alpha + (sum0 + sum1);
-        if (!start && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (kt != pc.kt0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < D / 64; ++c) {
             float v[32];
             tmem_ld32(t_o + c * 32, v);
 #pragma unroll
@@ -504,19 +541,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int own0 = max(pc.pos + 1 - key0, 0);
           const int end = pc.pos + pc.n_tok - key0;
           uint4* v = reinterpret_cast<uint4*>(sm.v[kv & 1]);
-          for (int i = r; i < kBlocks * 8 * kKeys; i += 128) {
-            const int row = i / 8 % kKeys;
+          // (chunks of the rows from own0 on)
+          const int rows = kKeys - own0;
+          for (int i = half * 128 + r; i < kBlocks * 8 * rows; i += 256) {
+            const int row = own0 + i / 8 % rows, at = i / 8 / rows * kKeys * 8 + row * 8 + i % 8;
             if (row >= end) {
-              v[i] = make_uint4(0, 0, 0, 0);
-            } else if (row >= own0) {
-              uint4 x = v[i];
+              v[at] = make_uint4(0, 0, 0, 0);
+            } else {
+              uint4 x = v[at];
               if (non_finite2<T>(x.x) || non_finite2<T>(x.y) || non_finite2<T>(x.z) ||
                   non_finite2<T>(x.w)) {
                 x.x = drop_non_finite2<T>(x.x);
                 x.y = drop_non_finite2<T>(x.y);
                 x.z = drop_non_finite2<T>(x.z);
                 x.w = drop_non_finite2<T>(x.w);
-                v[i] = x;
+                v[at] = x;
                 *reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) = rd;
               }
             }
@@ -532,97 +571,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++done;
       if (!ok) break;
       tc_fence_after();
-      float o[D];
-      if constexpr (D == 128) {
-        tmem_ld128(t_o, o);
-      } else {
-        float lo[32];
-        tmem_ld32(t_o, lo);
+      l += other(l);
+      const bool poisoned = *reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) == rd;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const int t = g * kTok + r / G;
+      const bool whole = pc.slot < 0, mine = r < kTok * G && t < pc.n_tok;
+      T* dst = static_cast<T*>(p.out) + (long long)(pc.tok + t) * p.out_stride +
+               (long long)(pc.head * G + r % G) * D + D / 2 * half;
+      const long long at = ((long long)pc.slot * 2 + g) * kRowsTile + r;
+      if (!whole && half == 0) part.chunk_ml[at] = make_float2(m, l);
+      float* part_dst = part.chunk_o + at * D + D / 2 * half;
+#pragma unroll 1
+      for (int c = 0; c < D / 2; c += 32) {
+        float o[32];
+        tmem_ld32(t_o + c, o);
+        if (poisoned) {
+          const int k0 = max(pc.pos + 1, pc.kt0 * kKeys);
+          for (int key = k0; key <= limit && key < pc.kt1 * kKeys; ++key) {
+            const int page = page_of(p.kv, pc.seq, key);
+            if (page < 0) continue;
+            const T* row = static_cast<const T*>(p.kv.v) + row_offset(p.kv, page, pc.head, key) +
+                           D / 2 * half + c;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = lo[e];
-        tmem_ld32(t_o + 32, lo);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[32 + e] = lo[e];
-      }
-      if (*reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) == rd) {
-        const int k0 = max(pc.pos + 1, pc.kt0 * kKeys);
-        for (int key = k0; key <= limit && key < pc.kt1 * kKeys; ++key) {
-          const int page = page_of(p.kv, pc.seq, key);
-          if (page < 0) continue;
-          const uint4* row = reinterpret_cast<const uint4*>(
-              static_cast<const T*>(p.kv.v) + row_offset(p.kv, page, pc.head, key));
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 x = row[c];
-            const T* e = reinterpret_cast<const T*>(&x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float f = Elem<T>::get(e[j]);
-              if (!(fabsf(f) < CUDART_INF_F)) o[c * 8 + j] += f;
+            for (int e = 0; e < 32; ++e) {
+              const float f = Elem<T>::get(row[e]);
+              if (!(fabsf(f) < CUDART_INF_F)) o[e] += f;
             }
           }
         }
-      }
-      // Rows leave through the warp's 4 KB: written a row per thread, read back so that
-      // eight lanes cover 128 bytes of a row (16-byte chunk c of row i at c ^ (i % 8)).
-      const int row_base = (warp & 3) * 32;
-      if (pc.slot < 0) {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        uint32_t x[8];
+        if (!whole) {
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
+          for (int e = 0; e < 32; e += 8) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint4 x;
-            const float* f = o + b * 64 + c * 8;
-            x.x = pack2<T>(f[0] * inv, f[1] * inv);
-            x.y = pack2<T>(f[2] * inv, f[3] * inv);
-            x.z = pack2<T>(f[4] * inv, f[5] * inv);
-            x.w = pack2<T>(f[6] * inv, f[7] * inv);
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = x;
+            for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(o[e + j]);
+            st_global_32(part_dst + c + e, x);
           }
-          __syncwarp();
+        } else if (mine) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rr = i * 4 + (lane >> 3), c = lane & 7;
-            const int row = row_base + rr, t = g * kTok + row / G;
-            if (row < kTok * G && t < pc.n_tok) {
-              const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 128 +
-                                                              ((c ^ (rr & 7)) << 4));
-              T* dst = static_cast<T*>(p.out) + (long long)(pc.tok + t) * p.out_stride +
-                       (long long)(pc.head * G + row % G) * D + b * 64 + c * 8;
-              *reinterpret_cast<uint4*>(dst) = x;
+          for (int e = 0; e < 32; e += 16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = pack2<T>(o[e + 2 * j] * inv, o[e + 2 * j + 1] * inv);
+            if (wide_out) {
+              st_global_32(dst + c + e, x);
+            } else {
+              *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(x[0], x[1], x[2], x[3]);
+              *reinterpret_cast<uint4*>(dst + c + e + 8) = make_uint4(x[4], x[5], x[6], x[7]);
             }
           }
-          __syncwarp();
-        }
-      } else {
-        const long long base = ((long long)pc.slot * 2 + g) * kRowsTile + row_base;
-        part.chunk_ml[base + lane] = make_float2(m, l);
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                make_float4(o[b * 32 + 4 * c], o[b * 32 + 4 * c + 1], o[b * 32 + 4 * c + 2],
-                            o[b * 32 + 4 * c + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rr = i * 4 + (lane >> 3), c = lane & 7;
-            *reinterpret_cast<float4*>(part.chunk_o + (base + rr) * D + b * 32 + c * 4) =
-                *reinterpret_cast<const float4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
-          }
-          __syncwarp();
         }
       }
     }
-    if (!ok) atomicOr(&sm.err, 1);
+    if (!ok) {
+      atomicOr(&sm.err, 1);
+      asm volatile("bar.arrive %0, %1;" ::"r"(meeting), "r"(64) : "memory");
+    }
   }
 
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && sm.err) atomicOr(p.status, kStatusWaitTimeout);
-  if (warp == 9) {
+  if (warp == kMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
                  ::"r"(tmem), "r"(512) : "memory");
@@ -686,7 +695,7 @@ cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int 
       ((long long)p.plan.n_tokens / (2 * tile_tokens<G>()) + p.plan.n_seq) * p.n_kv;
   const long long tiles = units * ((p.max_len + kKeys - 1) / kKeys);
   const int grid = (int)std::min<long long>(n_sm, tiles);
-  e = launch_with_pdl(paged_chunk_kernel<T, D, G>, dim3(grid), kThreads, sizeof(Smem<D>) + 1024,
+  e = launch_with_pdl(paged_chunk_kernel<T, D, G>, dim3(grid), kThreads, sizeof(Smem<D, G>) + 1024,
                       st, true, p, part, maps, hnd, box_rows);
   if (e != cudaSuccess) return e;
   return launch_with_pdl(paged_chunk_merge_kernel<T, D, G>,
@@ -697,7 +706,7 @@ template <typename T, int D, int G>
 cudaError_t prepare_one() {
   return cudaFuncSetAttribute((const void*)paged_chunk_kernel<T, D, G>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)sizeof(Smem<D>) + 1024);
+                              (int)sizeof(Smem<D, G>) + 1024);
 }
 
 }  // namespace

@@ -57,8 +57,11 @@ __device__ __forceinline__ int unit_tiles(int n_new, int len, int unit) {
 }
 template <int U, int KEYS>
 __device__ __forceinline__ long long chunk_tiles(int n_new, int len) {
-  long long sum = 0;
-  for (int u = 0; u * U < n_new; ++u) sum += unit_tiles<U, KEYS>(n_new, len, u);
+  long long sum = (len + KEYS - 1) / KEYS;  // the last unit
+  unsigned x = len - n_new + U + KEYS - 1;
+  const unsigned end = len + KEYS - 1;
+#pragma unroll 4
+  for (; x < end; x += U) sum += x / KEYS;
   return sum;
 }
 
@@ -68,8 +71,9 @@ template <typename T, int D, int G>
 __global__ void __launch_bounds__(256) rotate_q_kernel(const PagedAttnParams p) {
   using V = Vec16<T>;
   constexpr int kChunks = D / 2 / V::n;
-  pdl_launch_dependents();
   pdl_wait();
+  // (after the wait: what runs early beside this kernel may read all but its output)
+  pdl_launch_dependents();
   const int per_token = p.n_kv * kChunks;
   const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long last = (long long)p.plan.n_tokens * per_token - 1;
@@ -112,78 +116,132 @@ __global__ void __launch_bounds__(256) rotate_q_kernel(const PagedAttnParams p) 
 template <int U, int KEYS>
 struct Walk {
   long long tile, first, last, total, n;
-  long long seq_first;  // first tile of sequence seq
   int seq;
+  // the sequence (n_new 0: still to be read) and the unit that holds `tile`
+  int tok, n_new, len;
+  int head, unit, tiles;
+  long long at;  // first tile of the unit
 
-  // This CTA's share of the tiles of all units, by the whole block (scan: a word per warp).
-  __device__ void begin(const PagedAttnParams& p, const PagedPartials& part, long long* scan) {
-    const int tid = threadIdx.x, n_threads = blockDim.x;
+  // This CTA's share of the tiles of all units and the unit of its first tile, by the whole
+  // block.  found: two words of shared memory, scan: one per warp.
+  __device__ void begin(const PagedAttnParams& p, const PagedPartials& part, long long* scan,
+                        long long* found) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_threads = blockDim.x;
+    if (tid == 0) {
+      part.chunk_jobs[blockIdx.x].n_parts = 0;
+      found[0] = p.plan.n_seq;
+    }
+    const auto tiles_of = [&](int s) -> long long {
+      int a, b, c;
+      if (s >= p.plan.n_seq) return 0;
+      return chunk_of(p, s, a, b, c) ? chunk_tiles<U, KEYS>(b, c) * p.n_kv : 0;
+    };
     long long mine = 0;
     for (int s = tid; s < p.plan.n_seq; s += n_threads) {
-      int tok, n_new, len;
-      if (chunk_of(p, s, tok, n_new, len))
-        mine += chunk_tiles<U, KEYS>(n_new, len);
-      else if (blockIdx.x == 0 && p.plan.q_starts[s + 1] - (long long)p.plan.q_starts[s] > 1)
+      const long long x = tiles_of(s);
+      mine += x;
+      if (x == 0 && blockIdx.x == 0 &&
+          p.plan.q_starts[s + 1] - (long long)p.plan.q_starts[s] > 1)
         atomicOr(p.status, kStatusBadLength);
     }
+    const long long own = mine;
 #pragma unroll
     for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    if (tid % 32 == 0) scan[tid / 32] = mine;
-    if (tid == 0) part.chunk_jobs[blockIdx.x].n_parts = 0;
+    if (lane == 0) scan[warp] = mine;
     __syncthreads();
     total = 0;
     for (int w = 0; w < n_threads / 32; ++w) total += scan[w];
-    total *= p.n_kv;
     n = min((long long)gridDim.x, total);
     first = last = 0;
     if (blockIdx.x < n) {
       first = blockIdx.x * total / n;
       last = (blockIdx.x + 1) * total / n;
     }
+    // the sequence of the first tile
+    long long before = 0;
+    for (int s0 = 0; s0 < p.plan.n_seq && first < last; s0 += n_threads) {
+      const long long x = p.plan.n_seq <= n_threads ? own : tiles_of(s0 + tid);
+      long long incl = x;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      __syncthreads();
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      long long sum = 0;
+      for (int w = 0; w < n_threads / 32; ++w) {
+        if (w == warp) incl += before + sum;
+        sum += scan[w];
+      }
+      if (incl - x <= first && first < incl) {
+        found[0] = s0 + tid;
+        found[1] = incl - x;
+      }
+      before += sum;
+      if (first < before) break;
+    }
+    __syncthreads();
     tile = first;
-    seq_first = 0;
-    seq = 0;
-  }
-
-  __device__ bool next(const PagedAttnParams& p, const PagedPartials& part, Piece& out) {
-    while (tile < last && seq < p.plan.n_seq) {
-      int tok, n_new, len;
-      if (!chunk_of(p, seq, tok, n_new, len)) {
-        ++seq;
-        continue;
-      }
+    seq = (int)found[0];
+    at = found[1];
+    n_new = 0;
+    if (seq < p.plan.n_seq && first < last && chunk_of(p, seq, tok, n_new, len)) {
       const long long per_head = chunk_tiles<U, KEYS>(n_new, len);
-      if (tile >= seq_first + per_head * p.n_kv) {
-        seq_first += per_head * p.n_kv;
-        ++seq;
-        continue;
-      }
-      const int h = (int)((tile - seq_first) / per_head);
-      long long at = seq_first + h * per_head;  // first tile of the unit
-      int u = 0, tiles = unit_tiles<U, KEYS>(n_new, len, 0);
+      head = (int)((tile - at) / per_head);
+      at += head * per_head;
+      unit = 0;
+      tiles = unit_tiles<U, KEYS>(n_new, len, 0);
       while (tile >= at + tiles) {
         at += tiles;
-        tiles = unit_tiles<U, KEYS>(n_new, len, ++u);
+        tiles = unit_tiles<U, KEYS>(n_new, len, ++unit);
       }
-      out.seq = seq;
-      out.head = h;
-      out.tok = tok + u * U;
-      out.n_tok = min(U, n_new - u * U);
-      out.pos = len - n_new + u * U;
-      out.len = len;
-      out.kt0 = (int)(tile - at);
-      out.kt1 = (int)min((long long)tiles, last - at);
-      const bool whole = out.kt0 == 0 && out.kt1 == tiles;
-      out.slot = whole ? -1 : 2 * (int)blockIdx.x + (tile == first ? 0 : 1);
-      if (!whole && out.kt0 == 0) {
-        const int last_cta = (int)(((at + tiles) * n + total - 1) / total) - 1;
-        part.chunk_jobs[blockIdx.x] = PagedChunkJob{out.tok, out.n_tok, h, out.slot,
-                                                    last_cta - (int)blockIdx.x + 1};
-      }
-      tile = at + out.kt1;
-      return true;
     }
-    return false;
+  }
+
+  // The next piece; false when the share is done.
+  __device__ bool next(const PagedAttnParams& p, const PagedPartials& part, Piece& out) {
+    if (tile >= last) return false;
+    while (n_new == 0) {
+      if (seq >= p.plan.n_seq) return false;
+      if (!chunk_of(p, seq, tok, n_new, len)) {
+        n_new = 0;
+        ++seq;
+        continue;
+      }
+      head = unit = 0;
+      tiles = unit_tiles<U, KEYS>(n_new, len, 0);
+    }
+    out.seq = seq;
+    out.head = head;
+    out.tok = tok + unit * U;
+    out.n_tok = min(U, n_new - unit * U);
+    out.pos = len - n_new + unit * U;
+    out.len = len;
+    out.kt0 = (int)(tile - at);
+    out.kt1 = (int)min((long long)tiles, last - at);
+    const bool whole = out.kt0 == 0 && out.kt1 == tiles;
+    out.slot = whole ? -1 : 2 * (int)blockIdx.x + (tile == first ? 0 : 1);
+    if (!whole && out.kt0 == 0) {
+      const int last_cta = (int)(((at + tiles) * n + total - 1) / total) - 1;
+      part.chunk_jobs[blockIdx.x] = PagedChunkJob{out.tok, out.n_tok, head, out.slot,
+                                                  last_cta - (int)blockIdx.x + 1};
+    }
+    tile = at + out.kt1;
+    if (out.kt1 == tiles) {  // on to the next unit, head or sequence
+      at += tiles;
+      ++unit;
+      if (unit * U >= n_new) {
+        unit = 0;
+        if (++head == p.n_kv) {
+          n_new = 0;
+          ++seq;
+        }
+      }
+      if (n_new) tiles = unit_tiles<U, KEYS>(n_new, len, unit);
+    }
+    return true;
   }
 };
 

@@ -44,7 +44,7 @@ struct alignas(1024) Smem {
   uint64_t item_full[4], item_empty[4];
   uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty;
   uint64_t s_full[2], p_full, o_full, o_empty, drain;
-  long long scan[kThreads / 32];
+  long long scan[kThreads / 32], found[2];
   Walk<tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
   uint32_t tmem_base;
   int err;
@@ -75,16 +75,6 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t (&t)[kTerms]) 
   x -= __uint_as_float(t[1] << 16);
   y -= __uint_as_float(t[1] & 0xffff0000u);
   t[2] = pack_bf16(x, y);
-}
-
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-        "r"(v[7]) : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // Four floats of column c (a multiple of 4) of row r as three terms, at their place in an
@@ -141,12 +131,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                  ::"r"(smem_addr(&sm.tmem_base)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();
+  // The kernel before this one waited for all that came before it and wrote only q: the plan,
+  // the pages and the slots can be used before it is done.
   pdl_launch_dependents();
   tc_fence_before();
   {
     Walk<kTok, kKeys> walk;
-    walk.begin(p, part, sm.scan);
+    walk.begin(p, part, sm.scan, sm.found);
     if (tid == 128) sm.walk = walk;  // (the thread that walks)
   }
   tc_fence_after();
@@ -168,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kLoads = 16 / kSide;     // loads of a warp's 16 rows
     const int sub = lane / kLanes, col = lane % kLanes * 4;
     int t = 0;
-    bool ok = true;
+    bool ok = true, waited = false;
     for (int rd = 0; ok; ++rd) {
       const int place = rd & 3;
       if (w == 0) {  // this warp hands the pieces out
@@ -216,6 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       load(p.kv.k, pc.kt0, xk);
 
       // Q (rotated, in the rows of out)
+      if (!waited) pdl_wait();
+      waited = true;
       if (rd > 0) ok = wait_or_abort(&sm.q_empty, (rd - 1) & 1, err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -278,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&sm.v_full);
       }
     }
+    if (!waited) pdl_wait();  // (the grid must not end before the one whose q it stands for)
     if (!ok) atomicOr(&sm.err, 1);
   } else if (warp >= 8) {
     // ---- MMA issuer ----
