@@ -26,7 +26,9 @@
 // Warps 0-7 / 8-15: softmax of tile A / B, two threads per row (64 keys each: with one thread a
 // row, two warps a scheduler waited for their own instructions, 1800 clocks a tile against 1024
 // of the exponential unit); 16: loader (TMA of the pages); 17: MMA.  Tensor memory: S_A | S_B |
-// O_A | O_B, the P of each half of the keys over the first half of its scores.
+// O_A | O_B, the P of each half of the keys over the first half of its scores.  (One MMA warp
+// per tile measured slower, 64 against 58 us for 512 tokens over 8192 rows: the products of the
+// two interleave and both finish late.)
 // Every wait is bounded; a wait that runs out sets the status bit, and the CTA drains
 // what it issued and returns its tensor memory.
 #include <cuda.h>
@@ -58,7 +60,8 @@ struct alignas(1024) Smem {
   uint64_t item_full[4], item_empty[4];
   uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_final[2], drain;
-  long long scan[kThreads / 32], found[2];
+  long long scan[kThreads / 32];
+  WalkStart start;
   Walk<2 * tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
   uint32_t tmem_base;
   int err;
@@ -115,6 +118,47 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// Whether key tile kt holds rows past the piece's first token, which not all its rows see.
+__device__ __forceinline__ bool clears_v(const Piece& pc, int kt) {
+  return (kt + 1) * kKeys > pc.pos + 1;
+}
+
+// Scores whose bit is set become -inf.
+__device__ __forceinline__ void hide(float (&s)[32], unsigned hidden) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c)
+    if (hidden >> c & 1) s[c] = -CUDART_INF_F;
+}
+
+// The largest of 64 scores of this thread's row.  (Not inlined: needed on a piece's first tile
+// and when a maximum moves; the loop over the tiles has to fit the instruction cache beside the
+// MMA warp's.)
+__device__ __noinline__ float max64(uint32_t t_s, unsigned long long hidden) {
+  float top = -CUDART_INF_F;
+#pragma unroll 1
+  for (int c0 = 0; c0 < 64; c0 += 32) {
+    float s[32];
+    tmem_ld32(t_s + c0, s);
+    hide(s, (unsigned)(hidden >> c0));
+    float mx0 = s[0], mx1 = s[1];
+#pragma unroll
+    for (int c = 2; c < 30; c += 4) {
+      mx0 = fmax3(mx0, s[c], s[c + 1]);
+      mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+    }
+    top = fmax3(top, fmax3(mx0, s[30], s[31]), mx1);
+  }
+  return top;
+}
+
+// wait_or_abort with everything but the first look out of line, for the same reason.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, int* err) {
+  return wait_or_abort(bar, parity, err);
+}
+__device__ __forceinline__ bool wait_lean(uint64_t* bar, uint32_t parity, int* err) {
+  return mbar_try_wait(bar, parity) || wait_long(bar, parity, err);
+}
+
 // A pair of 16-bit values with an infinity or a NaN among them.
 template <typename T>
 __device__ __forceinline__ bool non_finite2(uint32_t x) {
@@ -149,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < 4; ++s) {
       mbar_init(&sm.item_full[s], 1);
-      mbar_init(&sm.item_empty[s], 1 + kSoftmaxWarps);  // the MMA thread and the softmax warps
+      mbar_init(&sm.item_empty[s], 1 + kSoftmaxWarps);  // the MMA and the softmax warps
       sm.poison[s] = -1;
     }
     for (int s = 0; s < 2; ++s) {
@@ -184,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   {
     Walk<2 * kTok, kKeys> walk;
-    walk.begin(p, part, sm.scan, sm.found);
+    walk.begin(p, part, sm.scan, &sm.start, kLoader * 32);
     if (tid == kLoader * 32) sm.walk = walk;
   }
   tc_fence_after();
@@ -300,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kMma) {
     // ---- MMA issuer (the whole warp, one lane issues) ----
     const auto all_wait = [&](uint64_t* bar, uint32_t parity, volatile int* e) {
-      return (bool)__all_sync(0xffffffffu, wait_or_abort(bar, parity, e));
+      return (bool)__all_sync(0xffffffffu, wait_lean(bar, parity, &sm.err));
     };
     {
       const auto issue_s = [&](int g, int kv) {
@@ -440,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int done = 0;
     bool ok = true;
     for (int rd = 0; ok; ++rd) {
-      ok = wait_or_abort(&sm.item_full[rd & 3], (rd >> 2) & 1, err);
+      ok = wait_lean(&sm.item_full[rd & 3], (rd >> 2) & 1, &sm.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const Piece pc = sm.ring[rd & 3];
@@ -455,52 +499,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first_limit = pc.pos + g * kTok;                       // of the tile's first row
       float m = -CUDART_INF_F, l = 0.f;
       for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++tc, ++kv) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&sm.s_full[g], tc & 1, err));
+        ok = __all_sync(0xffffffffu, wait_lean(&sm.s_full[g], tc & 1, &sm.err));
         if (!ok) break;
         tc_fence_after();
         const int key0 = kt * kKeys;
         const unsigned bad = sm.bad_rows[kv & 3];
-        // 32 scores at a time, masked
-        const auto scores = [&](int c0, float (&s)[32]) {
-          tmem_ld32(t_s + c0, s);
-          if (key0 + kKeys - 1 > first_limit) {
-            const int lim = limit - key0 - 64 * half - c0;
+        // Keys of this half that the row does not see: those past its own position, and rows
+        // without a page.
+        const bool edge = key0 + kKeys - 1 > first_limit || bad;
+        unsigned long long hidden = 0;
+        if (edge) {
+          const int seen = limit - key0 - 64 * half + 1;
+          hidden = seen >= 64 ? 0ull : ~0ull << max(seen, 0);
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (c > lim) s[c] = -CUDART_INF_F;
-          }
-          if (bad) {
-            const unsigned here = bad >> (4 * half + c0 / 16);
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (here >> (c / 16) & 1) s[c] = -CUDART_INF_F;
-          }
-        };
-        const auto max32 = [&](const float (&s)[32]) {
-          float mx0 = s[0], mx1 = s[1];
-#pragma unroll
-          for (int c = 2; c < 30; c += 4) {
-            mx0 = fmax3(mx0, s[c], s[c + 1]);
-            mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
-          }
-          return fmax3(fmaxf(mx0, mx1), s[30], s[31]);
-        };
-        float s[32];
-        scores(0, s);
-        float top = max32(s);
-        scores(32, s);
-        top = fmaxf(top, max32(s));
-        top = fmaxf(top, other(top)) * sc;
-        // The reference m moves to the row's maximum only when that has passed it by 2^8, so
-        // that O is rarely rescaled.
-        float alpha = 1.f;
-        if (top > m + 8.f) {
-          alpha = fast_exp2(m - top);
-          m = top;
+          for (int i = 0; i < 4; ++i)
+            if (bad >> (4 * half + i) & 1) hidden |= 0xffffull << (16 * i);
         }
-        const float nm = m == -CUDART_INF_F ? 0.f : -m;
-        float sum0 = 0.f, sum1 = 0.f;
-        const auto weights = [&](const float (&s)[32], uint32_t (&pk)[16]) {
+        // Weights against the running reference m, which is moved to the row's maximum (in a
+        // second pass over the scores) only on the piece's first tile, or when the weights of
+        // the tile add up to more than 2^10 in some row; the two halves of a row agree on it by
+        // their sums.  No P is stored before that, as it goes over the scores.
+        uint32_t pk0[16], pk1[16];
+        float alpha = 1.f, sum0, sum1;
+        const auto weights = [&](int c0, uint32_t (&pk)[16]) {
+          float s[32];
+          tmem_ld32(t_s + c0, s);
+          if (edge) hide(s, (unsigned)(hidden >> c0));
+          const float nm = m == -CUDART_INF_F ? 0.f : -m;
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             float x0, x1;
@@ -510,12 +535,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             pk[c / 2] = pack2<T>(p0, p1);
           }
         };
-        // (the second 32 first, whose scores are at hand; no P is stored before the first 32
-        // have been read again, over whose place it goes)
-        uint32_t pk1[16], pk0[16];
-        weights(s, pk1);
-        scores(0, s);
-        weights(s, pk0);
+        bool move = __any_sync(0xffffffffu, m == -CUDART_INF_F);
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          if (move) {
+            const float top = max64(t_s, hidden);
+            const float mn = fmaxf(m, fmaxf(top, other(top)) * sc);
+            alpha = mn == m ? 1.f : fast_exp2(m - mn);
+            m = mn;
+          }
+          sum0 = sum1 = 0.f;
+          weights(0, pk0);
+          weights(32, pk1);
+          if (move) break;
+          const float sum = sum0 + sum1;
+          move = __any_sync(0xffffffffu, !(sum + other(sum) <= 1024.f));
+          if (!move) break;
+        }
         __syncwarp();
         tmem_st16(t_s, pk0);
         tmem_st16(t_s + 16, pk1);
@@ -535,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // unit's last token are cleared; in those of its own tokens, which only some of its
         // rows see, what is not finite is cleared here and added to the rows that do see it
         // at the end.
-        if (g == 0 && key0 + kKeys > pc.pos + 1) {
-          ok = __all_sync(0xffffffffu, wait_or_abort(&sm.v_full[kv & 1], (kv >> 1) & 1, err));
+        if (g == 0 && clears_v(pc, kt)) {
+          ok = __all_sync(0xffffffffu, wait_lean(&sm.v_full[kv & 1], (kv >> 1) & 1, &sm.err));
           if (!ok) break;
           const int own0 = max(pc.pos + 1 - key0, 0);
           const int end = pc.pos + pc.n_tok - key0;
@@ -567,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&sm.p_full[g]);
       }
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, wait_or_abort(&sm.o_final[g], done & 1, err));
+      ok = __all_sync(0xffffffffu, wait_lean(&sm.o_final[g], done & 1, &sm.err));
       ++done;
       if (!ok) break;
       tc_fence_after();

@@ -112,91 +112,140 @@ __global__ void __launch_bounds__(256) rotate_q_kernel(const PagedAttnParams p) 
   }
 }
 
+// A share's start: the sequence of its first tile.
+struct WalkStart {
+  int seq, tok, n_new, len;
+  long long before, per_head;  // tiles of the sequences before it, and of one of its heads
+};
+
+// Equal shares of `total` tiles over n CTAs (the first few one larger), in 32 bits where that
+// is enough: a 64-bit division takes some 500 clocks of every CTA's start.
+struct Shares {
+  long long total;
+  int n;
+  long long each, rest;
+  __device__ static long long divide(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+  }
+  __device__ void set(long long tiles, int grid) {
+    total = tiles;
+    n = (int)min((long long)grid, tiles);
+    each = n ? divide(tiles, n) : 0;
+    rest = tiles - each * n;
+  }
+  __device__ long long first(int cta) const { return cta * each + min((long long)cta, rest); }
+  __device__ int cta_of(long long tile) const {
+    const long long big = rest * (each + 1);
+    return (int)(tile < big ? divide(tile, each + 1) : rest + divide(tile - big, each));
+  }
+};
+
 // The pieces of a CTA's share, in order.
 template <int U, int KEYS>
 struct Walk {
-  long long tile, first, last, total, n;
+  Shares shares;
+  long long tile, first, last;
   int seq;
   // the sequence (n_new 0: still to be read) and the unit that holds `tile`
   int tok, n_new, len;
   int head, unit, tiles;
   long long at;  // first tile of the unit
 
-  // This CTA's share of the tiles of all units and the unit of its first tile, by the whole
-  // block.  found: two words of shared memory, scan: one per warp.
+  // This CTA's share of the tiles of all units and the sequence of its first tile, by the
+  // whole block (scan: a word of shared memory per warp); `walker` then looks up the unit.
   __device__ void begin(const PagedAttnParams& p, const PagedPartials& part, long long* scan,
-                        long long* found) {
+                        WalkStart* start, int walker) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_threads = blockDim.x;
+    const int n_warps = n_threads / 32;
     if (tid == 0) {
       part.chunk_jobs[blockIdx.x].n_parts = 0;
-      found[0] = p.plan.n_seq;
+      start->n_new = 0;
     }
-    const auto tiles_of = [&](int s) -> long long {
-      int a, b, c;
-      if (s >= p.plan.n_seq) return 0;
-      return chunk_of(p, s, a, b, c) ? chunk_tiles<U, KEYS>(b, c) * p.n_kv : 0;
-    };
-    long long mine = 0;
-    for (int s = tid; s < p.plan.n_seq; s += n_threads) {
-      const long long x = tiles_of(s);
-      mine += x;
-      if (x == 0 && blockIdx.x == 0 &&
-          p.plan.q_starts[s + 1] - (long long)p.plan.q_starts[s] > 1)
+    // (one round for up to a block of sequences: their numbers stay in registers)
+    WalkStart mine{};
+    const auto read = [&](int s) {
+      mine.seq = s;
+      mine.per_head = 0;
+      if (s < p.plan.n_seq && chunk_of(p, s, mine.tok, mine.n_new, mine.len))
+        mine.per_head = chunk_tiles<U, KEYS>(mine.n_new, mine.len);
+      else if (s < p.plan.n_seq && blockIdx.x == 0 &&
+               p.plan.q_starts[s + 1] - (long long)p.plan.q_starts[s] > 1)
         atomicOr(p.status, kStatusBadLength);
-    }
-    const long long own = mine;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    if (lane == 0) scan[warp] = mine;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < n_threads / 32; ++w) total += scan[w];
-    n = min((long long)gridDim.x, total);
-    first = last = 0;
-    if (blockIdx.x < n) {
-      first = blockIdx.x * total / n;
-      last = (blockIdx.x + 1) * total / n;
-    }
-    // the sequence of the first tile
-    long long before = 0;
-    for (int s0 = 0; s0 < p.plan.n_seq && first < last; s0 += n_threads) {
-      const long long x = p.plan.n_seq <= n_threads ? own : tiles_of(s0 + tid);
-      long long incl = x;
+    };
+    // sum of x over the block and, in `incl`, over the threads up to this one
+    const auto scan_block = [&](long long x, long long& incl) {
+      incl = x;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += y;
       }
-      __syncthreads();
       if (lane == 31) scan[warp] = incl;
       __syncthreads();
-      long long sum = 0;
-      for (int w = 0; w < n_threads / 32; ++w) {
-        if (w == warp) incl += before + sum;
-        sum += scan[w];
+      long long w = lane < n_warps ? scan[lane] : 0, upto = w;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
       }
-      if (incl - x <= first && first < incl) {
-        found[0] = s0 + tid;
-        found[1] = incl - x;
+      incl += __shfl_sync(0xffffffffu, upto - w, warp);
+      return __shfl_sync(0xffffffffu, upto, 31);
+    };
+    long long incl, sum = 0;
+    if (p.plan.n_seq <= n_threads) {
+      read(tid);
+      sum = scan_block(mine.per_head * p.n_kv, incl);
+    } else {
+      for (int s0 = 0; s0 < p.plan.n_seq; s0 += n_threads) {
+        read(s0 + tid);
+        sum += scan_block(mine.per_head * p.n_kv, incl);
+        __syncthreads();
       }
-      before += sum;
-      if (first < before) break;
+    }
+    shares.set(sum, gridDim.x);
+    first = last = 0;
+    if (blockIdx.x < shares.n) {
+      first = shares.first(blockIdx.x);
+      last = shares.first(blockIdx.x + 1);
+    }
+    const auto offer = [&](long long upto) {
+      const long long x = mine.per_head * p.n_kv;
+      if (upto - x <= first && first < upto && first < last) {
+        mine.before = upto - x;
+        *start = mine;
+      }
+    };
+    if (p.plan.n_seq <= n_threads) {
+      offer(incl);
+    } else {
+      long long before = 0;
+      for (int s0 = 0; s0 < p.plan.n_seq && before <= first; s0 += n_threads) {
+        read(s0 + tid);
+        __syncthreads();
+        const long long all = scan_block(mine.per_head * p.n_kv, incl);
+        offer(before + incl);
+        before += all;
+      }
     }
     __syncthreads();
+    if (tid != walker) return;
     tile = first;
-    seq = (int)found[0];
-    at = found[1];
-    n_new = 0;
-    if (seq < p.plan.n_seq && first < last && chunk_of(p, seq, tok, n_new, len)) {
-      const long long per_head = chunk_tiles<U, KEYS>(n_new, len);
-      head = (int)((tile - at) / per_head);
-      at += head * per_head;
-      unit = 0;
-      tiles = unit_tiles<U, KEYS>(n_new, len, 0);
-      while (tile >= at + tiles) {
-        at += tiles;
-        tiles = unit_tiles<U, KEYS>(n_new, len, ++unit);
-      }
+    seq = start->seq;
+    tok = start->tok;
+    n_new = start->n_new;
+    len = start->len;
+    at = start->before;
+    if (n_new == 0 || first >= last) {
+      last = first;
+      return;
+    }
+    head = (int)Shares::divide(tile - at, start->per_head);
+    at += head * start->per_head;
+    unit = 0;
+    tiles = unit_tiles<U, KEYS>(n_new, len, 0);
+    while (tile >= at + tiles) {
+      at += tiles;
+      tiles = unit_tiles<U, KEYS>(n_new, len, ++unit);
     }
   }
 
@@ -224,7 +273,7 @@ struct Walk {
     const bool whole = out.kt0 == 0 && out.kt1 == tiles;
     out.slot = whole ? -1 : 2 * (int)blockIdx.x + (tile == first ? 0 : 1);
     if (!whole && out.kt0 == 0) {
-      const int last_cta = (int)(((at + tiles) * n + total - 1) / total) - 1;
+      const int last_cta = shares.cta_of(at + tiles - 1);
       part.chunk_jobs[blockIdx.x] = PagedChunkJob{out.tok, out.n_tok, head, out.slot,
                                                   last_cta - (int)blockIdx.x + 1};
     }

@@ -44,7 +44,8 @@ struct alignas(1024) Smem {
   uint64_t item_full[4], item_empty[4];
   uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty;
   uint64_t s_full[2], p_full, o_full, o_empty, drain;
-  long long scan[kThreads / 32], found[2];
+  long long scan[kThreads / 32];
+  WalkStart start;
   Walk<tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
   uint32_t tmem_base;
   int err;
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   {
     Walk<kTok, kKeys> walk;
-    walk.begin(p, part, sm.scan, sm.found);
+    walk.begin(p, part, sm.scan, &sm.start, 128);
     if (tid == 128) sm.walk = walk;  // (the thread that walks)
   }
   tc_fence_after();
