@@ -1743,11 +1743,14 @@ int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv,
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
   p.status = c->status;
   cudaStream_t st = (cudaStream_t)stream;
-  if (max_new > 1 && kv->dtype == GQA_F32)
-    GQA_CUDA(launch_paged_chunk32(p, c->paged, hd, c->n_sm, st, c->pdl != 0));
-  else if (max_new > 1)
-    GQA_CUDA(launch_paged_chunk16(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));
-  GQA_CUDA(launch_paged_decode(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0));
+  const bool chunks = max_new > 1, f32 = kv->dtype == GQA_F32;
+  int n_decode = 0, n_chunk = 0;
+  GQA_CUDA(launch_paged_decode(p, c->paged, kv->dtype, hd, c->n_sm, st, c->pdl != 0, chunks,
+                               &n_decode));
+  if (chunks)
+    GQA_CUDA(f32 ? launch_paged_chunk32(p, c->paged, hd, c->n_sm, st, &n_chunk)
+                 : launch_paged_chunk16(p, c->paged, kv->dtype, hd, c->n_sm, st, &n_chunk));
+  GQA_CUDA(launch_paged_merge(p, c->paged, kv->dtype, hd, n_decode, n_chunk, st));
   return GQA_OK;
 }
 

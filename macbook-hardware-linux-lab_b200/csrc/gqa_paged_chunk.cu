@@ -17,7 +17,7 @@
 // leaves its parts in two slots per CTA, merged by a second kernel.  So a short chunk
 // over a long cache uses every SM, and the triangle of a whole prompt is balanced.
 //
-// q is rotated for its position by a first kernel, which puts it where the result of the
+// q is rotated for its position by the kernel before this one, which puts it where the result of the
 // same token will be (every unit reads its q before it writes its output, and parts are
 // merged after all units), so no workspace grows with the batch.  Rounding it to the type
 // there is what the projection before it would do with a rotated q; scores and sums are
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm.q[b / kBlocks][(b % kBlocks) * kRowsTile * 64 + (kTok * G + r) * 64 + x] = 0;
   }
   fence_proxy_async_smem();
-  // The kernel before this one waited for all that came before it and wrote only q: the plan,
-  // the pages and the slots can be used before it is done.
+  // The kernel before this one waited for all that came before it; of what it writes this one
+  // uses only q: the plan, the pages and the slots can be used before it is done.
   pdl_launch_dependents();
   tc_fence_before();
   {
@@ -689,8 +689,7 @@ PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
 
 template <typename T, int D, int G>
 cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int n_sm,
-                       cudaStream_t st, bool pdl) {
-  using V = Vec16<T>;
+                       cudaStream_t st, int* grid) {
   PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
   if (!encode) return cudaErrorNotSupported;
   ChunkMaps maps;
@@ -723,19 +722,12 @@ cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
 
-  const long long items = (long long)p.plan.n_tokens * p.n_kv * (D / 2 / V::n);
-  cudaError_t e = launch_with_pdl(rotate_q_kernel<T, D, G>, dim3((unsigned)((items + 255) / 256)),
-                                  256, 0, st, pdl, p);
-  if (e != cudaSuccess) return e;
   const long long units =
       ((long long)p.plan.n_tokens / (2 * tile_tokens<G>()) + p.plan.n_seq) * p.n_kv;
   const long long tiles = units * ((p.max_len + kKeys - 1) / kKeys);
-  const int grid = (int)std::min<long long>(n_sm, tiles);
-  e = launch_with_pdl(paged_chunk_kernel<T, D, G>, dim3(grid), kThreads, sizeof(Smem<D, G>) + 1024,
-                      st, true, p, part, maps, hnd, box_rows);
-  if (e != cudaSuccess) return e;
-  return launch_with_pdl(paged_chunk_merge_kernel<T, D, G>,
-                         dim3(grid, ((2 * tile_tokens<G>()) * G + 7) / 8), 256, 0, st, true, p, part);
+  *grid = (int)std::min<long long>({(long long)n_sm, part.n_chunk_ctas, tiles});
+  return launch_with_pdl(paged_chunk_kernel<T, D, G>, dim3(*grid), kThreads,
+                         sizeof(Smem<D, G>) + 1024, st, true, p, part, maps, hnd, box_rows);
 }
 
 template <typename T, int D, int G>
@@ -756,13 +748,13 @@ cudaError_t prepare_paged_chunk16() {
 }
 
 cudaError_t launch_paged_chunk16(const PagedAttnParams& p, const PagedPartials& part, int dtype,
-                                 int head_dim, int n_sm, cudaStream_t st, bool pdl) {
+                                 int head_dim, int n_sm, cudaStream_t st, int* grid) {
   const bool wide = head_dim == 128;
   if (dtype == kDtypeBf16)
-    return wide ? launch_one<__nv_bfloat16, 128, 6>(p, part, n_sm, st, pdl)
-                : launch_one<__nv_bfloat16, 64, 7>(p, part, n_sm, st, pdl);
-  return wide ? launch_one<__half, 128, 6>(p, part, n_sm, st, pdl)
-              : launch_one<__half, 64, 7>(p, part, n_sm, st, pdl);
+    return wide ? launch_one<__nv_bfloat16, 128, 6>(p, part, n_sm, st, grid)
+                : launch_one<__nv_bfloat16, 64, 7>(p, part, n_sm, st, grid);
+  return wide ? launch_one<__half, 128, 6>(p, part, n_sm, st, grid)
+              : launch_one<__half, 64, 7>(p, part, n_sm, st, grid);
 }
 
 }  // namespace gqa

@@ -1,6 +1,6 @@
 // Shared parts of the chunk kernels of the paged attention (gqa_paged_chunk.cu in 16 bits,
 // gqa_paged_chunk32.cu in fp32): units and pieces of the work, q rotated into the rows of the
-// output, the merge of parts, and the matrix instruction.
+// output, and the matrix instruction.
 #pragma once
 
 #include <math_constants.h>
@@ -10,8 +10,6 @@
 #include "gqa_tc.cuh"
 
 namespace gqa {
-
-constexpr int kChunkRows = 128;  // rows of a tile: token * G + head
 
 template <int G>
 __host__ __device__ constexpr int tile_tokens() { return kChunkRows / G; }
@@ -65,50 +63,49 @@ __device__ __forceinline__ long long chunk_tiles(int n_new, int len) {
   return sum;
 }
 
-// q rotated into the rows of out: one thread per (token, KV head, 16-byte chunk of the
-// first half of a row), all heads of the group.
+// q of the chunks' tokens rotated into the rows of out: an item is (token, KV head, 16-byte chunk
+// of the first half of a row), all heads of the group; the whole grid takes part.
 template <typename T, int D, int G>
-__global__ void __launch_bounds__(256) rotate_q_kernel(const PagedAttnParams p) {
+__device__ void rotate_q(const PagedAttnParams& p) {
   using V = Vec16<T>;
   constexpr int kChunks = D / 2 / V::n;
-  pdl_wait();
-  // (after the wait: what runs early beside this kernel may read all but its output)
-  pdl_launch_dependents();
   const int per_token = p.n_kv * kChunks;
-  const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long last = (long long)p.plan.n_tokens * per_token - 1;
-  const int tok = (int)(min(item, last) / per_token);
-  const int tok0 = __shfl_sync(0xffffffffu, tok, 0);
-  int s = find_sequence(p.plan.q_starts, p.plan.n_seq, tok0);
-  while (s + 1 < p.plan.n_seq && p.plan.q_starts[s + 1] <= tok) ++s;
-  if (item > last) return;
-  int first, n_new, len;
-  if (!chunk_of(p, s, first, n_new, len) || tok < first || tok >= first + n_new) {
-    return;  // (another kernel's sequence, or one that is reported there)
-  }
-  const int pos = len - n_new + tok - first;
-  const int rem = (int)(item - (long long)tok * per_token);
-  const int h = rem / kChunks, c = rem % kChunks;
-  float co[V::n], si[V::n];
+  const long long items = (long long)p.plan.n_tokens * per_token;
+  const long long step = (long long)gridDim.x * blockDim.x;
+  for (long long i0 = (long long)blockIdx.x * blockDim.x + threadIdx.x / 32 * 32; i0 < items;
+       i0 += step) {
+    const long long item = i0 + threadIdx.x % 32;
+    const int tok = (int)(min(item, items - 1) / per_token);
+    // the warp looks up its first token; its others are in that or a later sequence
+    int s = find_sequence(p.plan.q_starts, p.plan.n_seq, __shfl_sync(0xffffffffu, tok, 0));
+    while (s + 1 < p.plan.n_seq && p.plan.q_starts[s + 1] <= tok) ++s;
+    int first, n_new, len;
+    if (item >= items || !chunk_of(p, s, first, n_new, len) || tok < first || tok >= first + n_new)
+      continue;  // (a single token, or a sequence that is reported elsewhere)
+    const int pos = len - n_new + tok - first;
+    const int rem = (int)(item - (long long)tok * per_token);
+    const int h = rem / kChunks, c = rem % kChunks;
+    float co[V::n], si[V::n];
 #pragma unroll
-  for (int e = 0; e < V::n; ++e) rope_cos_sin(pos, p.turns[c * V::n + e], co[e], si[e]);
-  const T* src = static_cast<const T*>(p.qkv) + (long long)tok * p.qkv_stride +
-                 (long long)h * G * D + c * V::n;
-  T* dst = static_cast<T*>(p.out) + (long long)tok * p.out_stride + (long long)h * G * D +
-           c * V::n;
+    for (int e = 0; e < V::n; ++e) rope_cos_sin(pos, p.turns[c * V::n + e], co[e], si[e]);
+    const T* src = static_cast<const T*>(p.qkv) + (long long)tok * p.qkv_stride +
+                   (long long)h * G * D + c * V::n;
+    T* dst = static_cast<T*>(p.out) + (long long)tok * p.out_stride + (long long)h * G * D +
+             c * V::n;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const V a = *reinterpret_cast<const V*>(src + g * D);
-    const V b = *reinterpret_cast<const V*>(src + g * D + D / 2);
-    V y0, y1;
+    for (int g = 0; g < G; ++g) {
+      const V a = *reinterpret_cast<const V*>(src + g * D);
+      const V b = *reinterpret_cast<const V*>(src + g * D + D / 2);
+      V y0, y1;
 #pragma unroll
-    for (int e = 0; e < V::n; ++e) {
-      const float x = Elem<T>::get(a.e[e]), y = Elem<T>::get(b.e[e]);
-      y0.e[e] = Elem<T>::put(x * co[e] - y * si[e]);
-      y1.e[e] = Elem<T>::put(x * si[e] + y * co[e]);
+      for (int e = 0; e < V::n; ++e) {
+        const float x = Elem<T>::get(a.e[e]), y = Elem<T>::get(b.e[e]);
+        y0.e[e] = Elem<T>::put(x * co[e] - y * si[e]);
+        y1.e[e] = Elem<T>::put(x * si[e] + y * co[e]);
+      }
+      *reinterpret_cast<V*>(dst + g * D) = y0;
+      *reinterpret_cast<V*>(dst + g * D + D / 2) = y1;
     }
-    *reinterpret_cast<V*>(dst + g * D) = y0;
-    *reinterpret_cast<V*>(dst + g * D + D / 2) = y1;
   }
 }
 
@@ -293,60 +290,5 @@ struct Walk {
     return true;
   }
 };
-
-// Merges the parts of units that crossed shares: a warp per row, blocks of 8 rows.
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(256) paged_chunk_merge_kernel(const PagedAttnParams p,
-                                                                const PagedPartials part) {
-  pdl_wait();
-  const PagedChunkJob job = part.chunk_jobs[blockIdx.x];
-  if (job.n_parts == 0) return;
-  constexpr int kTok = tile_tokens<G>(), E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int idx = blockIdx.y * 8 + (threadIdx.x >> 5);  // row of the unit's tokens
-  const int t = idx / G, g = idx % G;
-  if (t >= job.n_tok) return;
-  const int row = t < kTok ? idx : kChunkRows + (t - kTok) * G + g;
-  const auto at = [&](int i) {
-    return (long long)(i == 0 ? job.slot : 2 * ((int)blockIdx.x + i)) * kChunkSlotRows + row;
-  };
-  // the parts' weights, a part per lane; then loads that depend on nothing
-  float m = -CUDART_INF_F, l = 0.f, o[E];
-  for (int i = lane; i < job.n_parts; i += 32) {
-    const float2 ml = part.chunk_ml[at(i)];
-    if (ml.y != 0.f) m = fmaxf(m, ml.x);
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i0 = 0; i0 < job.n_parts; i0 += 32) {
-    float2 ml = make_float2(0.f, 0.f);
-    if (i0 + lane < job.n_parts) ml = part.chunk_ml[at(i0 + lane)];
-    const float weight = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
-    l += weight * ml.y;
-    for (int i = i0; i < min(i0 + 32, job.n_parts); i += 8) {
-      float x[8][E];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          x[u][e] = i + u < job.n_parts ? part.chunk_o[at(i + u) * D + lane * E + e] : 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float a = __shfl_sync(0xffffffffu, weight, i - i0 + u);
-        if (a != 0.f)
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += a * x[u][e];
-      }
-    }
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  T* out = static_cast<T*>(p.out) + (long long)(job.tok + t) * p.out_stride +
-           (long long)(job.head * G + g) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = Elem<T>::put(l != 0.f ? o[e] / l : 0.f);
-}
 
 }  // namespace gqa

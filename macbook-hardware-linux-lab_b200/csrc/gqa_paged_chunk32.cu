@@ -14,8 +14,9 @@
 // Rows, units and shares are as in gqa_paged_chunk.cu, with one tile of 126 rows per unit and
 // 64 keys per tile (three terms of Q, K and V fill the shared memory).
 //
-// Warps 0-3: softmax (a row per thread, its output in registers); 4-7: read Q, K and V from
-// the pages, split them and write the operands; 8: MMA (9-11 only give their registers).  K and V have one place each: the
+// Warps 0-3: softmax (a row per thread, its output in registers); 4-11: read Q, K and V from
+// the pages, split them and write the operands (with four warps that took twice the MMA's time);
+// 12: MMA (13-15 only give their registers).  K and V have one place each: the
 // next tile is read into registers while this one is worked on.  Tensor memory: two S, two P
 // of three terms, one O of a single tile.
 #include "gqa_paged_chunk.cuh"
@@ -25,10 +26,12 @@ namespace gqa {
 namespace {
 
 constexpr int kKeys = 64;
-constexpr int kThreads = 384;
-// Registers of a thread in each group of four warps; three groups of 168 at the launch.
-constexpr int kRegsSoftmax = 240, kRegsOperands = 184, kRegsMma = 80;
-static_assert(kRegsSoftmax + kRegsOperands + kRegsMma == 3 * 168, "the launch's registers");
+constexpr int kOperandWarps = 8, kFirstOperand = 4, kMma = 12;
+constexpr int kThreads = 512;
+// Registers of a thread in each group of four warps; four groups of 128 at the launch.
+constexpr int kRegsSoftmax = 232, kRegsOperands = 104, kRegsMma = 72;
+static_assert(kRegsSoftmax + 2 * kRegsOperands + kRegsMma == 4 * 128, "the launch's registers");
+constexpr int kRowsWarp = kKeys / kOperandWarps;  // rows of K and V of an operand warp
 constexpr int kTerms = 3;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 320;  // S: 2 x 64, P: 2 x 96, O: D
 
@@ -109,12 +112,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < 4; ++s) {
       mbar_init(&sm.item_full[s], 1);
-      mbar_init(&sm.item_empty[s], 9);  // the MMA thread, the softmax and the operand warps
+      mbar_init(&sm.item_empty[s], 5 + kOperandWarps);  // MMA thread, softmax, operand warps
       sm.poison[s] = -1;
     }
-    mbar_init(&sm.q_full, 4);
-    mbar_init(&sm.k_full, 4);
-    mbar_init(&sm.v_full, 4);
+    mbar_init(&sm.q_full, kOperandWarps);
+    mbar_init(&sm.k_full, kOperandWarps);
+    mbar_init(&sm.v_full, kOperandWarps);
     mbar_init(&sm.p_full, 4);
     mbar_init(&sm.o_empty, 4);
     mbar_init(&sm.q_empty, 1);
@@ -127,13 +130,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm.err = 0;
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_addr(&sm.tmem_base)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // The kernel before this one waited for all that came before it and wrote only q: the plan,
-  // the pages and the slots can be used before it is done.
+  // The kernel before this one waited for all that came before it; of what it writes this one
+  // uses only q: the plan, the pages and the slots can be used before it is done.
   pdl_launch_dependents();
   tc_fence_before();
   {
@@ -151,13 +154,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     return true;
   };
 
-  if (warp >= 4 && warp < 8) {
+  if (warp >= kFirstOperand && warp < kMma) {
     // ---- operands ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOperands));
-    const int w = warp - 4;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOperands));
+    const int w = warp - kFirstOperand;
     constexpr int kLanes = D / 4;          // lanes that cover a row
     constexpr int kSide = 32 / kLanes;     // rows side by side in a load
-    constexpr int kLoads = 16 / kSide;     // loads of a warp's 16 rows
+    constexpr int kLoads = kRowsWarp / kSide;  // loads of a warp's rows
     const int sub = lane / kLanes, col = lane % kLanes * 4;
     int t = 0;
     bool ok = true, waited = false;
@@ -183,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // K or V rows of the warp's part of key tile kt into registers.
       int page = 0;
       const auto look_up = [&](int kt) {
-        const int row = kt * kKeys + w * 16;
+        const int row = kt * kKeys + w * kRowsWarp;
         page = p.kv.n_pages;  // (nothing there)
         if (row < pc.pos + pc.n_tok) {
           page = page_of(p.kv, pc.seq, row);
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       const auto load = [&](const void* pool, int kt, float4 (&x)[kLoads]) {
-        const int row0 = kt * kKeys + w * 16;
+        const int row0 = kt * kKeys + w * kRowsWarp;
         const bool there = page >= 0 && page < p.kv.n_pages;
         const float* src = static_cast<const float*>(pool) +
                            (there ? row_offset(p.kv, page, pc.head, row0) : 0);
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (rd > 0) ok = wait_or_abort(&sm.q_empty, (rd - 1) & 1, err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      for (int r0 = w * 32; r0 < w * 32 + 32; r0 += kSide * 4) {
+      for (int r0 = w * 16; r0 < w * 16 + 16; r0 += kSide * 4) {
         float4 x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -237,8 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) put4(sm.k, kKeys, w * 16 + i * kSide + sub, col, xk[i]);
-        if (lane == 0) sm.bad[t & 3][w] = page < 0;
+        for (int i = 0; i < kLoads; ++i) put4(sm.k, kKeys, w * kRowsWarp + i * kSide + sub, col, xk[i]);
+        if (lane == 0) sm.bad[t & 3][w * kRowsWarp / 16] = page < 0;  // (alike in two warps)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.k_full);
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) put4(sm.v, kKeys, w * 16 + i * kSide + sub, col, xv[i]);
+        for (int i = 0; i < kLoads; ++i) put4(sm.v, kKeys, w * kRowsWarp + i * kSide + sub, col, xv[i]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.v_full);
@@ -274,10 +277,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!waited) pdl_wait();  // (the grid must not end before the one whose q it stands for)
     if (!ok) atomicOr(&sm.err, 1);
-  } else if (warp >= 8) {
+  } else if (warp >= kMma) {
     // ---- MMA issuer ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-    if (warp == 8 && lane == 0) {
+    if (warp == kMma && lane == 0) {
       // Pairs of terms, small products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), a digit each.
       // (Not unrolled: the descriptors of all products would not fit the registers.)
       constexpr uint32_t kA = 0x001102, kB = 0x010120;
@@ -442,8 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t pk[kTerms][8];
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float p0 = exp2f(fmaf(s[c + e], sc, -ref));
-              const float p1 = exp2f(fmaf(s[c + e + 1], sc, -ref));
+              const float p0 = fast_exp2(fmaf(s[c + e], sc, -ref));
+              const float p1 = fast_exp2(fmaf(s[c + e + 1], sc, -ref));
               sum0 += p0;
               sum1 += p1;
               uint32_t x[kTerms];
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && sm.err) atomicOr(p.status, kStatusWaitTimeout);
-  if (warp == 8) {
+  if (warp == kMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
                  ::"r"(tmem), "r"(512) : "memory");
@@ -534,20 +537,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D, int G>
 cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int n_sm,
-                       cudaStream_t st, bool pdl) {
+                       cudaStream_t st, int* grid) {
   constexpr int kTok = tile_tokens<G>();
-  const long long items = (long long)p.plan.n_tokens * p.n_kv * (D / 2 / Vec16<float>::n);
-  cudaError_t e = launch_with_pdl(rotate_q_kernel<float, D, G>,
-                                  dim3((unsigned)((items + 255) / 256)), 256, 0, st, pdl, p);
-  if (e != cudaSuccess) return e;
   const long long units = ((long long)p.plan.n_tokens / kTok + p.plan.n_seq) * p.n_kv;
   const long long tiles = units * ((p.max_len + kKeys - 1) / kKeys);
-  const int grid = (int)std::min<long long>(n_sm, tiles);
-  e = launch_with_pdl(paged_chunk32_kernel<D, G>, dim3(grid), kThreads, sizeof(Smem<D, G>) + 1024, st,
-                      true, p, part);
-  if (e != cudaSuccess) return e;
-  return launch_with_pdl(paged_chunk_merge_kernel<float, D, G>, dim3(grid, (kTok * G + 7) / 8), 256,
-                         0, st, true, p, part);
+  *grid = (int)std::min<long long>({(long long)n_sm, part.n_chunk_ctas, tiles});
+  return launch_with_pdl(paged_chunk32_kernel<D, G>, dim3(*grid), kThreads,
+                         sizeof(Smem<D, G>) + 1024, st, true, p, part);
 }
 
 template <int D, int G>
@@ -566,9 +562,9 @@ cudaError_t prepare_paged_chunk32() {
 }
 
 cudaError_t launch_paged_chunk32(const PagedAttnParams& p, const PagedPartials& part, int head_dim,
-                                 int n_sm, cudaStream_t st, bool pdl) {
-  return head_dim == 128 ? launch_one<128, 6>(p, part, n_sm, st, pdl)
-                         : launch_one<64, 7>(p, part, n_sm, st, pdl);
+                                 int n_sm, cudaStream_t st, int* grid) {
+  return head_dim == 128 ? launch_one<128, 6>(p, part, n_sm, st, grid)
+                         : launch_one<64, 7>(p, part, n_sm, st, grid);
 }
 
 }  // namespace gqa

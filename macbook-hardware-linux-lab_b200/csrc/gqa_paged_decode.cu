@@ -17,10 +17,12 @@
 // filled by 16-byte asynchronous copies (rows past the end are filled with zeros, so
 // that what stands there never meets a weight), its own softmax state, and no
 // barrier until the piece is done.
+//
+// In a call with chunks the kernel also rotates their q, for the chunks' kernel after it.
 #include <math_constants.h>
 
-#include "gqa_paged.cuh"
-#include "gqa_paged_launch.cuh"
+#include "gqa_paged_chunk.cuh"
+#include "gqa_paged_merge.cuh"
 
 namespace gqa {
 
@@ -386,8 +388,8 @@ __device__ __forceinline__ long long block_sum(long long x, long long (&part)[kW
 }
 
 template <typename T, int D, int G>
-__global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedAttnParams p,
-                                                                   const PagedPartials part) {
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_decode_kernel(const PagedAttnParams p, const PagedPartials part, const int rotate) {
   extern __shared__ unsigned char smem_raw[];
   using S = Smem<T, D>;
   S& sm = *reinterpret_cast<S*>(smem_raw);
@@ -395,7 +397,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedAt
   constexpr int kChunks = D * (int)sizeof(T) / 16;  // of a row
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
+  // (after the wait: the chunks' kernel behind this one may read all but this one's output early)
   pdl_launch_dependents();
+  if (rotate) rotate_q<T, D, G>(p);
 
   // Tiles of all pairs, and this CTA's share [first, last) of them.
   long long mine = 0;
@@ -581,84 +585,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedAt
   }
 }
 
-// Merges the parts of a pair: one block per (CTA that holds a first part, query head).  The
-// parts' weights first (a part per thread), so that the loads of the outputs depend on nothing
-// and go out together.
-constexpr int kMergeWarps = 8;
-constexpr int kMaxParts = 512;  // two CTAs on each SM of the largest parts, and some
-
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(kMergeWarps * 32)
-    paged_merge_kernel(const PagedAttnParams p, const PagedPartials part) {
-  __shared__ float weight[kMaxParts], red[2][kMergeWarps], so[kMergeWarps][D];
-  pdl_wait();
-  const PagedJob job = part.jobs[blockIdx.x];
-  if (job.n_parts == 0) return;
-  const int g = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // the first part's slot, then slot 0 of each CTA after it
-  const auto slot_of = [&](int i) { return i == 0 ? job.slot : 2 * ((int)blockIdx.x + i); };
-  constexpr int kOwn = kMaxParts / (kMergeWarps * 32);
-  float2 ml[kOwn];
-  float m = -CUDART_INF_F;
-#pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    const int i = tid + j * kMergeWarps * 32;
-    ml[j] = i < job.n_parts ? part.ml[slot_of(i) * G + g] : make_float2(-CUDART_INF_F, 0.f);
-    if (ml[j].y != 0.f) m = fmaxf(m, ml[j].x);
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (lane == 0) red[0][warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, red[0][w]);
-  float l = 0.f;
-#pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    const float a = ml[j].y != 0.f ? exp2f(ml[j].x - m) : 0.f;
-    l += a * ml[j].y;
-    weight[tid + j * kMergeWarps * 32] = a;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) l += red[1][w];
-  constexpr int E = D / 32;
-  float o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i0 = warp; i0 < job.n_parts; i0 += 8 * kMergeWarps) {
-    float x[8][E], a[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = min(i0 + u * kMergeWarps, job.n_parts - 1);
-      a[u] = i0 + u * kMergeWarps < job.n_parts ? weight[i] : 0.f;
-      const float* src = part.o + ((long long)slot_of(i) * G + g) * D + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[u][e] = src[e];
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (a[u] != 0.f)  // (a part without a row holds nothing to be added)
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += a[u] * x[u][e];
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
-  __syncthreads();
-  T* out = static_cast<T*>(p.out) + (long long)job.tok * p.out_stride +
-           (long long)(job.head * G + g) * D;
-  for (int e = tid; e < D; e += kMergeWarps * 32) {
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) sum += so[w][e];
-    out[e] = Elem<T>::put(l != 0.f ? sum / l : 0.f);
-  }
-}
-
 template <typename T, int D, int G>
 cudaError_t prepare_one() {
   return cudaFuncSetAttribute((const void*)paged_decode_kernel<T, D, G>,
@@ -668,16 +594,21 @@ cudaError_t prepare_one() {
 
 template <typename T, int D, int G>
 cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int n_sm,
-                       cudaStream_t st, bool pdl) {
+                       cudaStream_t st, bool pdl, bool rotate, int* grid) {
   const long long tiles =
       (long long)p.plan.n_seq * p.n_kv * ((p.max_len + tile_rows<T>() - 1) / tile_rows<T>());
-  const long long most = std::min<long long>({2LL * n_sm, part.n_ctas, kMaxParts});
-  const int grid = (int)std::min(most, tiles);
-  cudaError_t e = launch_with_pdl(paged_decode_kernel<T, D, G>, dim3(grid), kThreads,
-                                  sizeof(Smem<T, D>), st, pdl, p, part);
-  if (e != cudaSuccess) return e;
-  return launch_with_pdl(paged_merge_kernel<T, D, G>, dim3(grid, G), kMergeWarps * 32, 0, st, true,
-                         p, part);
+  const long long items = (long long)p.plan.n_tokens * p.n_kv * (D / 2 / Vec16<T>::n);
+  const long long want = rotate ? std::max(tiles, (items + kThreads - 1) / kThreads) : tiles;
+  *grid = (int)std::min<long long>({2LL * n_sm, part.n_ctas, kMaxDecodeCtas, want});
+  return launch_with_pdl(paged_decode_kernel<T, D, G>, dim3(*grid), kThreads, sizeof(Smem<T, D>),
+                         st, pdl, p, part, (int)rotate);
+}
+
+template <typename T, int D, int G>
+cudaError_t merge_one(const PagedAttnParams& p, const PagedPartials& part, int n_decode,
+                      int n_chunk, cudaStream_t st) {
+  return launch_with_pdl(paged_merge_kernel<T, D, G>, dim3(n_decode * G + n_chunk * kUnitSlabs),
+                         kMergeWarps * 32, 0, st, true, p, part, n_decode);
 }
 
 }  // namespace
@@ -693,16 +624,30 @@ cudaError_t prepare_paged_decode() {
 }
 
 cudaError_t launch_paged_decode(const PagedAttnParams& p, const PagedPartials& part, int dtype,
-                                int head_dim, int n_sm, cudaStream_t st, bool pdl) {
+                                int head_dim, int n_sm, cudaStream_t st, bool pdl, bool rotate,
+                                int* grid) {
   const bool wide = head_dim == 128;
   if (dtype == kDtypeF32)
-    return wide ? launch_one<float, 128, 6>(p, part, n_sm, st, pdl)
-                : launch_one<float, 64, 7>(p, part, n_sm, st, pdl);
+    return wide ? launch_one<float, 128, 6>(p, part, n_sm, st, pdl, rotate, grid)
+                : launch_one<float, 64, 7>(p, part, n_sm, st, pdl, rotate, grid);
   if (dtype == kDtypeBf16)
-    return wide ? launch_one<__nv_bfloat16, 128, 6>(p, part, n_sm, st, pdl)
-                : launch_one<__nv_bfloat16, 64, 7>(p, part, n_sm, st, pdl);
-  return wide ? launch_one<__half, 128, 6>(p, part, n_sm, st, pdl)
-              : launch_one<__half, 64, 7>(p, part, n_sm, st, pdl);
+    return wide ? launch_one<__nv_bfloat16, 128, 6>(p, part, n_sm, st, pdl, rotate, grid)
+                : launch_one<__nv_bfloat16, 64, 7>(p, part, n_sm, st, pdl, rotate, grid);
+  return wide ? launch_one<__half, 128, 6>(p, part, n_sm, st, pdl, rotate, grid)
+              : launch_one<__half, 64, 7>(p, part, n_sm, st, pdl, rotate, grid);
+}
+
+cudaError_t launch_paged_merge(const PagedAttnParams& p, const PagedPartials& part, int dtype,
+                               int head_dim, int n_decode, int n_chunk, cudaStream_t st) {
+  const bool wide = head_dim == 128;
+  if (dtype == kDtypeF32)
+    return wide ? merge_one<float, 128, 6>(p, part, n_decode, n_chunk, st)
+                : merge_one<float, 64, 7>(p, part, n_decode, n_chunk, st);
+  if (dtype == kDtypeBf16)
+    return wide ? merge_one<__nv_bfloat16, 128, 6>(p, part, n_decode, n_chunk, st)
+                : merge_one<__nv_bfloat16, 64, 7>(p, part, n_decode, n_chunk, st);
+  return wide ? merge_one<__half, 128, 6>(p, part, n_decode, n_chunk, st)
+              : merge_one<__half, 64, 7>(p, part, n_decode, n_chunk, st);
 }
 
 }  // namespace gqa

@@ -22,6 +22,8 @@ struct PagedChunkJob {
   int n_parts;
 };
 constexpr int kChunkSlotRows = 256;
+constexpr int kChunkRows = 128;      // rows of a chunk's tile: token * G + head
+constexpr int kMaxDecodeCtas = 512;  // of the single tokens' grid (and parts of a pair)
 struct PagedPartials {
   float* o;
   float2* ml;
@@ -52,13 +54,18 @@ cudaError_t launch_with_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t
 cudaError_t prepare_paged_decode();
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int head_dim,
                                 cudaStream_t st, bool pdl);
+// The attention's launches, in this order: single tokens (and, `rotate`, q of the chunks), chunks
+// (max_new > 1), merge.  *grid gets the CTAs launched.
 cudaError_t launch_paged_decode(const PagedAttnParams& p, const PagedPartials& part, int dtype,
-                                int head_dim, int n_sm, cudaStream_t st, bool pdl);
+                                int head_dim, int n_sm, cudaStream_t st, bool pdl, bool rotate,
+                                int* grid);
 cudaError_t prepare_paged_chunk16();
 cudaError_t launch_paged_chunk16(const PagedAttnParams& p, const PagedPartials& part, int dtype,
-                                 int head_dim, int n_sm, cudaStream_t st, bool pdl);
+                                 int head_dim, int n_sm, cudaStream_t st, int* grid);
 cudaError_t prepare_paged_chunk32();
 cudaError_t launch_paged_chunk32(const PagedAttnParams& p, const PagedPartials& part, int head_dim,
-                                 int n_sm, cudaStream_t st, bool pdl);
+                                 int n_sm, cudaStream_t st, int* grid);
+cudaError_t launch_paged_merge(const PagedAttnParams& p, const PagedPartials& part, int dtype,
+                               int head_dim, int n_decode, int n_chunk, cudaStream_t st);
 
 }  // namespace gqa
