@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kMma) {
     // ---- MMA issuer (the whole warp, one lane issues) ----
-    const auto all_wait = [&](uint64_t* bar, uint32_t parity, volatile int* e) {
+    const auto all_wait = [&](uint64_t* bar, uint32_t parity) {
       return (bool)__all_sync(0xffffffffu, wait_lean(bar, parity, &sm.err));
     };
     {
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   desc_mn_major(v + ks * 2048), kIdO, acc || ks > 0);
       };
       const auto take = [&](int n, Piece& pc) {
-        if (!all_wait(&sm.item_full[n & 3], (n >> 2) & 1, err)) return false;
+        if (!all_wait(&sm.item_full[n & 3], (n >> 2) & 1)) return false;
         pc = sm.ring[n & 3];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.item_empty[n & 3]);
@@ -382,30 +382,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       int rd = 0, kv = 0, nq[2] = {0, 0}, nt[2] = {0, 0};  // Q tiles, S tiles of A and B
       bool ok = take(0, pc);
       bool two = pc.n_tok > kTok;
-      // S of the first key tile of a piece or of the next one
-      const auto first_s = [&](int g, bool start) {
-        if (start) {
-          if (!all_wait(&sm.q_full[g], nq[g] & 1, err)) return false;
-          ++nq[g];
-        }
-        return true;
-      };
-      if (ok && pc.n_tok > 0) {
-        const bool lone = pc.kt1 - pc.kt0 == 1;
-        ok = all_wait(&sm.k_full[0], 0, err) && first_s(0, true);
-        if (ok) {
+      // S of a piece's first key tile
+      const auto first_s = [&](int kv, bool both, bool lone) {
+        if (!all_wait(&sm.q_full[0], nq[0] & 1) || !all_wait(&sm.k_full[kv & 1], (kv >> 1) & 1))
+          return false;
+        ++nq[0];
+        tc_fence_after();
+        issue_s(0, kv);
+        if (lone) commit(&sm.q_empty[0]);
+        if (both) {
+          if (!all_wait(&sm.q_full[1], nq[1] & 1)) return false;
+          ++nq[1];
           tc_fence_after();
-          issue_s(0, 0);
-          if (lone) commit(&sm.q_empty[0]);
-          if (two) ok = first_s(1, true);
-        }
-        if (ok && two) {
-          tc_fence_after();
-          issue_s(1, 0);
+          issue_s(1, kv);
           if (lone) commit(&sm.q_empty[1]);
         }
-        if (ok) commit(&sm.k_empty[0]);
-      }
+        commit(&sm.k_empty[kv & 1]);
+        return true;
+      };
+      if (ok && pc.n_tok > 0) ok = first_s(0, two, pc.kt1 - pc.kt0 == 1);
       int kt = pc.kt0;
       while (ok && pc.n_tok > 0) {
         // the key tile after this one: of the same piece, or the next one's first
@@ -421,33 +416,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool n_last = kt_n + 1 == nx.kt1;
         const int kv_n = kv + 1;
         // What the loader brings is waited for first, while the softmax is still at work: the
-        // products then follow the weights at once, P V of this tile and S of the next.
-        ok = all_wait(&sm.v_full[kv & 1], (kv >> 1) & 1, err);
-        if (ok && more)
-          ok = first_s(0, last) && all_wait(&sm.k_full[kv_n & 1], (kv_n >> 1) & 1, err);
-        if (!ok || !all_wait(&sm.p_full[0], nt[0] & 1, err)) { ok = false; break; }
+        // products then follow the weights at once, P V of this tile and S of the next (of the
+        // next piece only after the commits: its Q may be long in coming).
+        ok = all_wait(&sm.v_full[kv & 1], (kv >> 1) & 1);
+        if (ok && !last) ok = all_wait(&sm.k_full[kv_n & 1], (kv_n >> 1) & 1);
+        if (!ok || !all_wait(&sm.p_full[0], nt[0] & 1)) { ok = false; break; }
         ++nt[0];
         tc_fence_after();
         issue_pv(0, kv, kt > pc.kt0);
-        if (more) issue_s(0, kv_n);
+        if (!last) issue_s(0, kv_n);
         if (!two) commit(&sm.v_empty[kv & 1]);
         if (last) commit(&sm.o_final[0]);
-        if (more && n_last) commit(&sm.q_empty[0]);
-        if (more && two_n && !first_s(1, last)) { ok = false; break; }
+        if (!last && n_last) commit(&sm.q_empty[0]);
         if (two) {
-          if (!all_wait(&sm.p_full[1], nt[1] & 1, err)) { ok = false; break; }
+          if (!all_wait(&sm.p_full[1], nt[1] & 1)) { ok = false; break; }
           ++nt[1];
           tc_fence_after();
           issue_pv(1, kv, kt > pc.kt0);
-        }
-        if (more && two_n) issue_s(1, kv_n);
-        if (two) {
+          if (!last) issue_s(1, kv_n);
           commit(&sm.v_empty[kv & 1]);
           if (last) commit(&sm.o_final[1]);
+          if (!last && n_last) commit(&sm.q_empty[1]);
         }
-        if (more) {
-          if (two_n && n_last) commit(&sm.q_empty[1]);
+        if (!last) {
           commit(&sm.k_empty[kv_n & 1]);
+        } else if (more) {
+          ok = first_s(kv_n, two_n, n_last);
+          if (!ok) break;
         }
         pc = nx;
         two = two_n;

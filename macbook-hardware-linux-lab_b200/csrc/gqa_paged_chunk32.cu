@@ -1,9 +1,9 @@
 // Attention of chunks of new tokens over a paged KV cache in fp32, on the
 // 5th-generation tensor cores.
 //
-// Each fp32 number enters as three bf16 terms (x = h + m + l, 8 significant bits each, to
-// 2^-25 of x), and a product of two as the six products of terms that matter (hh, hm, mh, mm,
-// hl, lh; the rest is below 2^-24): six bf16 matrix products in place of one, 279 TFLOP/s at
+// Each fp32 number enters as three bf16 terms (x = h + m + l, 8 significant bits each,
+// exactly), and a product of two as the six products of terms that matter (hh, hm, mh, mm,
+// hl, lh; the rest is below 2^-22, and some 2^-25 on average): six bf16 matrix products in place of one, 279 TFLOP/s at
 // the measured bf16 rate against some 70 of the fp32 units, with fp32's accuracy.  bf16 terms
 // rather than fp16 ones (which would do with three products) because they have fp32's range:
 // no scales, and columns of V of very different size keep their digits.  The products of
@@ -70,15 +70,19 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// x and y as three bf16 pairs.
+// x and y as three bf16 pairs: the upper halves of the number, of what is left and of what is
+// left of that.  Cut off rather than rounded, each takes eight bits or more, so the three hold
+// all 24 exactly; no conversion instruction is needed.
 __device__ __forceinline__ void split3(float x, float y, uint32_t (&t)[kTerms]) {
-  t[0] = pack_bf16(x, y);
-  x -= __uint_as_float(t[0] << 16);
-  y -= __uint_as_float(t[0] & 0xffff0000u);
-  t[1] = pack_bf16(x, y);
-  x -= __uint_as_float(t[1] << 16);
-  y -= __uint_as_float(t[1] & 0xffff0000u);
-  t[2] = pack_bf16(x, y);
+#pragma unroll
+  for (int i = 0; i < kTerms; ++i) {
+    t[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    if (i + 1 < kTerms) {
+      const float hx = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+      const float hy = __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+      ffma2(x, y, hx, hy, -1.f, -1.f, x, y);
+    }
+  }
 }
 
 // Four floats of column c (a multiple of 4) of row r as three terms, at their place in an
@@ -95,6 +99,19 @@ __device__ __forceinline__ void put4(uint16_t (*term)[N], int rows, int r, int c
 }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < CUDART_INF_F; }
+
+// Adds the infinities and NaN in V of the piece's keys up to `limit` to a row of output.
+template <int D>
+__device__ __noinline__ void add_non_finite(const PagedAttnParams& p, const Piece& pc, int limit,
+                                            float* row) {
+  for (int key = pc.kt0 * kKeys; key <= limit && key < pc.kt1 * kKeys; ++key) {
+    const int page = page_of(p.kv, pc.seq, key);
+    if (page < 0) continue;
+    const float* v = static_cast<const float*>(p.kv.v) + row_offset(p.kv, page, pc.head, key);
+    for (int e = 0; e < D; ++e)
+      if (!finite(v[e])) row[e] += v[e];
+  }
+}
 
 template <int D, int G>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -183,17 +200,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&sm.item_empty[place]);
       if (pc.n_tok == 0) break;
 
-      // K or V rows of the warp's part of key tile kt into registers.
-      int page = 0;
-      const auto look_up = [&](int kt) {
+      // The warp's rows of a key tile: their page (-1: a bad one; n_pages: past the unit), and
+      // K or V of them into registers.
+      const auto page_at = [&](int kt) {
         const int row = kt * kKeys + w * kRowsWarp;
-        page = p.kv.n_pages;  // (nothing there)
-        if (row < pc.pos + pc.n_tok) {
-          page = page_of(p.kv, pc.seq, row);
-          if (page < 0 && lane == 0) atomicOr(p.status, kStatusBadPage);
-        }
+        if (kt >= pc.kt1 || row >= pc.pos + pc.n_tok) return p.kv.n_pages;
+        const int page = page_of(p.kv, pc.seq, row);
+        if (page < 0 && lane == 0) atomicOr(p.status, kStatusBadPage);
+        return page;
       };
-      const auto load = [&](const void* pool, int kt, float4 (&x)[kLoads]) {
+      const auto load = [&](const void* pool, int kt, int page, float4 (&x)[kLoads]) {
         const int row0 = kt * kKeys + w * kRowsWarp;
         const bool there = page >= 0 && page < p.kv.n_pages;
         const float* src = static_cast<const float*>(pool) +
@@ -206,48 +222,58 @@ __global__ void __launch_bounds__(kThreads, 1)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       };
-      float4 xk[kLoads], xv[kLoads];
-      look_up(pc.kt0);
-      load(p.kv.k, pc.kt0, xk);
-
-      // Q (rotated, in the rows of out)
-      if (!waited) pdl_wait();
-      waited = true;
-      if (rd > 0) ok = wait_or_abort(&sm.q_empty, (rd - 1) & 1, err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      for (int r0 = w * 16; r0 < w * 16 + 16; r0 += kSide * 4) {
-        float4 x[4];
+      const auto put_k = [&](int n, int page, const float4 (&x)[kLoads]) {
+        if (n > 0 && !__all_sync(0xffffffffu, wait_or_abort(&sm.k_empty, (n - 1) & 1, err)))
+          return false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = r0 + i * kSide + sub, tk = r / G;
-          x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (r < kTok * G && tk < pc.n_tok)
-            x[i] = *reinterpret_cast<const float4*>(
-                static_cast<const float*>(p.out) + (long long)(pc.tok + tk) * p.out_stride +
-                (long long)(pc.head * G + r % G) * D + col);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put4(sm.q, kChunkRows, r0 + i * kSide + sub, col, x[i]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_full);
-
-      for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++t) {
-        load(p.kv.v, kt, xv);
-        if (t > 0) ok = wait_or_abort(&sm.k_empty, (t - 1) & 1, err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) put4(sm.k, kKeys, w * kRowsWarp + i * kSide + sub, col, xk[i]);
-        if (lane == 0) sm.bad[t & 3][w * kRowsWarp / 16] = page < 0;  // (alike in two warps)
+        for (int i = 0; i < kLoads; ++i)
+          put4(sm.k, kKeys, w * kRowsWarp + i * kSide + sub, col, x[i]);
+        if (lane == 0) sm.bad[n & 3][w * kRowsWarp / 16] = page < 0;  // (alike in two warps)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.k_full);
+        return true;
+      };
+      // K runs one tile ahead of V, as S runs ahead of P V; Q comes between the first K and V.
+      float4 xk[kLoads], xv[kLoads];
+      int page = page_at(pc.kt0), page_n = page;
+      load(p.kv.k, pc.kt0, page, xk);
+      load(p.kv.v, pc.kt0, page, xv);
+      for (int kt = pc.kt0 - 1; kt < pc.kt1; ++kt) {
+        // (here xk holds tile kt + 1 and xv tile kt, or kt + 1 at first)
         if (kt + 1 < pc.kt1) {
-          look_up(kt + 1);
-          load(p.kv.k, kt + 1, xk);
+          ok = put_k(t + (kt >= pc.kt0), page_n, xk);
+          if (!ok) break;
+          page = page_n;
+          page_n = page_at(kt + 2);
+          load(p.kv.k, kt + 2, page_n, xk);
+        }
+        if (kt < pc.kt0) {
+          // Q (rotated, in the rows of out)
+          if (!waited) pdl_wait();
+          waited = true;
+          if (rd > 0) ok = wait_or_abort(&sm.q_empty, (rd - 1) & 1, err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+#pragma unroll 1
+          for (int r0 = w * 16; r0 < w * 16 + 16; r0 += kSide * 4) {
+            float4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = r0 + i * kSide + sub, tk = r / G;
+              x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (r < kTok * G && tk < pc.n_tok)
+                x[i] = *reinterpret_cast<const float4*>(
+                    static_cast<const float*>(p.out) + (long long)(pc.tok + tk) * p.out_stride +
+                    (long long)(pc.head * G + r % G) * D + col);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put4(sm.q, kChunkRows, r0 + i * kSide + sub, col, x[i]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.q_full);
+          continue;
         }
         // A weight of zero does not cancel an infinity or a NaN (and the terms of a weight
         // have signs): what is not finite stays out of the product, and is added at the end to
@@ -255,24 +281,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          float4& x = xv[i];
-          if (!(finite(x.x) && finite(x.y) && finite(x.z) && finite(x.w))) {
-            odd = true;
+          const float4 x = xv[i];
+          odd |= !(finite(x.x) && finite(x.y) && finite(x.z) && finite(x.w));
+        }
+        if (odd) {
+          *reinterpret_cast<volatile int*>(&sm.poison[place]) = rd;
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            float4& x = xv[i];
             x.x = finite(x.x) ? x.x : 0.f;
             x.y = finite(x.y) ? x.y : 0.f;
             x.z = finite(x.z) ? x.z : 0.f;
             x.w = finite(x.w) ? x.w : 0.f;
           }
         }
-        if (odd) *reinterpret_cast<volatile int*>(&sm.poison[place]) = rd;
         if (t > 0) ok = wait_or_abort(&sm.v_empty, (t - 1) & 1, err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) put4(sm.v, kKeys, w * kRowsWarp + i * kSide + sub, col, xv[i]);
+        for (int i = 0; i < kLoads; ++i)
+          put4(sm.v, kKeys, w * kRowsWarp + i * kSide + sub, col, xv[i]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.v_full);
+        load(p.kv.v, kt + 1, kt + 1 < pc.kt1 ? page : p.kv.n_pages, xv);
+        ++t;
       }
     }
     if (!waited) pdl_wait();  // (the grid must not end before the one whose q it stands for)
@@ -280,82 +313,93 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= kMma) {
     // ---- MMA issuer ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-    if (warp == kMma && lane == 0) {
+    if (warp == kMma) {  // (the whole warp, one lane issues)
+      const auto all_wait = [&](uint64_t* bar, uint32_t parity) {
+        return (bool)__all_sync(0xffffffffu, wait_or_abort(bar, parity, err));
+      };
+      const auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+        __syncwarp();
+      };
+      // Descriptors differ in their low words alone, by constants.
+      const uint32_t q0 = (uint32_t)smem_desc(smem_addr(sm.q[0]), 16);
+      const uint32_t k0 = (uint32_t)smem_desc(smem_addr(sm.k[0]), 16);
+      const uint32_t v0 = (uint32_t)smem_desc(smem_addr(sm.v[0]), kKeys * 128);
+      const uint32_t high = (uint32_t)(smem_desc(0, 0) >> 32);
+      const auto desc = [&](uint32_t low) {
+        uint64_t d;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+        return d;
+      };
       // Pairs of terms, small products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), a digit each.
-      // (Not unrolled: the descriptors of all products would not fit the registers.)
+      // One pair unrolled: the loops of all roles have to fit the instruction cache together.
       constexpr uint32_t kA = 0x001102, kB = 0x010120;
       const auto issue_s = [&](int t) {
-        bool acc = false;
+        const uint32_t d = tmem + kColS + 64 * (t & 1);
+        if (elect_one()) {
 #pragma unroll 1
-        for (int i = 0; i < 6; ++i) {
-          const uint32_t q = smem_addr(sm.q[kA >> 4 * i & 15]);
-          const uint32_t k = smem_addr(sm.k[kB >> 4 * i & 15]);
+          for (int i = 0; i < 24; i += 4) {
+            const uint32_t q = q0 + (kA >> i & 15) * (kChunkRows * D * 2 / 16);
+            const uint32_t k = k0 + (kB >> i & 15) * (kKeys * D * 2 / 16);
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t in = (ks & 3) * 32;
-            umma_ss(tmem + kColS + 64 * (t & 1),
-                    smem_desc(q + (ks >> 2) * (kChunkRows * 128) + in, 16),
-                    smem_desc(k + (ks >> 2) * (kKeys * 128) + in, 16), kIdS, acc);
-            acc = true;
+            for (int ks = 0; ks < D / 16; ++ks)
+              umma_ss(d, desc(q + ((ks >> 2) * kChunkRows * 128 + (ks & 3) * 32) / 16),
+                      desc(k + ((ks >> 2) * kKeys * 128 + (ks & 3) * 32) / 16), kIdS, i + ks > 0);
           }
+          umma_commit(&sm.s_full[t & 1]);
+          umma_commit(&sm.k_empty);
         }
-        umma_commit(&sm.s_full[t & 1]);
-        umma_commit(&sm.k_empty);
+        __syncwarp();
       };
       const auto issue_pv = [&](int t) {
-        bool acc = false;
+        const uint32_t at = tmem + kColP + 96 * (t & 1);
+        if (elect_one()) {
 #pragma unroll 1
-        for (int i = 0; i < 6; ++i) {
-          const uint32_t v = smem_addr(sm.v[kB >> 4 * i & 15]);
-          const uint32_t p_at = tmem + kColP + 96 * (t & 1) + 32 * (kA >> 4 * i & 15);
+          for (int i = 0; i < 24; i += 4) {
+            const uint32_t w = at + 32 * (kA >> i & 15);
+            const uint32_t v = v0 + (kB >> i & 15) * (kKeys * D * 2 / 16);
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks) {
-            umma_ts(tmem + kColO, p_at + ks * 8, smem_desc(v + ks * 2048, kKeys * 128), kIdO, acc);
-            acc = true;
+            for (int ks = 0; ks < kKeys / 16; ++ks)
+              umma_ts(tmem + kColO, w + ks * 8, desc(v + ks * 2048 / 16), kIdO, i + ks > 0);
           }
+          umma_commit(&sm.o_full);
+          umma_commit(&sm.v_empty);
         }
-        umma_commit(&sm.o_full);
-        umma_commit(&sm.v_empty);
+        __syncwarp();
+      };
+      const auto get = [&](int n, Piece& pc) {
+        const bool good = __all_sync(0xffffffffu, take(n, pc));
+        __syncwarp();
+        if (good && lane == 0) mbar_arrive(&sm.item_empty[n & 3]);
+        return good;
       };
       Piece pc{};
-      int rd = 0, t = 0;
-      bool ok = take(0, pc);
-      if (ok) mbar_arrive(&sm.item_empty[0]);
-      if (ok && pc.n_tok > 0) {
-        ok = wait_or_abort(&sm.q_full, 0, err) && wait_or_abort(&sm.k_full, 0, err);
-        if (ok) {
-          tc_fence_after();
-          issue_s(0);
-          if (pc.kt1 - pc.kt0 == 1) umma_commit(&sm.q_empty);
-        }
-      }
-      int kt = pc.kt0;
+      int rd = 0, t = 0;  // pieces; tiles whose P V is issued
+      bool ok = get(0, pc);
       while (ok && pc.n_tok > 0) {
-        Piece nx = pc;
-        int kt_n = kt + 1;
-        const bool last = kt_n == pc.kt1;
-        if (last) {
-          ok = take(++rd, nx);
-          if (!ok) break;
-          mbar_arrive(&sm.item_empty[rd & 3]);
-          kt_n = nx.kt0;
+        const int tiles = pc.kt1 - pc.kt0;
+        // S runs one tile ahead of P V (the first of a piece follows the last P V of the one
+        // before: its Q may be long in coming).
+        for (int j = 0; j <= tiles; ++j) {
+          if (j < tiles) {
+            ok = (j > 0 || all_wait(&sm.q_full, rd & 1)) && all_wait(&sm.k_full, (t + (j > 0)) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(t + (j > 0));
+            if (j + 1 == tiles) commit(&sm.q_empty);
+          }
+          if (j > 0) {
+            ok = all_wait(&sm.v_full, t & 1) && (t == 0 || all_wait(&sm.o_empty, (t - 1) & 1)) &&
+                 all_wait(&sm.p_full, t & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t);
+            ++t;
+          }
         }
-        if (nx.n_tok > 0) {
-          if ((last && !wait_or_abort(&sm.q_full, rd & 1, err)) ||
-              !wait_or_abort(&sm.k_full, (t + 1) & 1, err)) { ok = false; break; }
-          tc_fence_after();
-          issue_s(t + 1);
-          if (kt_n + 1 == nx.kt1) umma_commit(&sm.q_empty);
-        }
-        if (!wait_or_abort(&sm.p_full, t & 1, err) || !wait_or_abort(&sm.v_full, t & 1, err) ||
-            (t > 0 && !wait_or_abort(&sm.o_empty, (t - 1) & 1, err))) { ok = false; break; }
-        tc_fence_after();
-        issue_pv(t);
-        pc = nx;
-        kt = kt_n;
-        ++t;
+        if (ok) ok = get(++rd, pc);
       }
-      umma_commit(&sm.drain);  // no MMA may be running when tensor memory is freed
+      commit(&sm.drain);  // no MMA may be running when tensor memory is freed
       mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
     }
     __syncwarp();
@@ -379,119 +423,105 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -CUDART_INF_F, l = 0.f, o[D];
 #pragma unroll
       for (int e = 0; e < D; ++e) o[e] = 0.f;
-      // Adds the product of tile n to the row.
-      const auto add_o = [&](int n) {
-        const bool good = __all_sync(0xffffffffu, wait_or_abort(&sm.o_full, n & 1, err));
-        if (!good) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          float v[32];
-          tmem_ld32(t_lane + kColO + c * 32, v);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[c * 32 + e] += v[e];
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.o_empty);
-        return true;
-      };
-      for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++t) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&sm.s_full[t & 1], (t >> 1) & 1, err));
-        if (!ok) break;
-        tc_fence_after();
-        const int lim = limit - kt * kKeys;
-        const uint32_t bad = *reinterpret_cast<const uint32_t*>(sm.bad[t & 3]);
-        // Half a row of scores at a time (read twice: a whole one beside the output's
-        // registers would not fit).
-        const auto scores = [&](int half, float (&s)[32]) {
-          tmem_ld32(t_lane + kColS + 64 * (t & 1) + 32 * half, s);
-          if (lim < 32 * half + 31) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (32 * half + c > lim) s[c] = -CUDART_INF_F;
-          }
+      // Turn j: weights of tile j, then the product of tile j - 1 is added to the row.
+      const int tiles = pc.kt1 - pc.kt0;
+      for (int j = 0; j <= tiles; ++j) {
+        float alpha = 1.f;
+        if (j < tiles) {
+          ok = __all_sync(0xffffffffu, wait_or_abort(&sm.s_full[t & 1], (t >> 1) & 1, err));
+          if (!ok) break;
+          tc_fence_after();
+          // Keys that the row does not see: past its own position, or without a page.
+          const int seen = limit - (pc.kt0 + j) * kKeys + 1;
+          unsigned long long hidden = seen >= kKeys ? 0ull : ~0ull << max(seen, 0);
+          const uint32_t bad = *reinterpret_cast<const uint32_t*>(sm.bad[t & 3]);
           if (bad) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (bad >> ((2 * half + c / 16) * 8) & 1) s[c] = -CUDART_INF_F;
+            for (int i = 0; i < 4; ++i)
+              if (bad >> (8 * i) & 1) hidden |= 0xffffull << (16 * i);
           }
-        };
-        float top = -CUDART_INF_F;
+          // Sixteen scores at a time, twice: the largest, then the weights.  (A row of scores
+          // beside the row of output would not fit the registers, nor all of it unrolled the
+          // instruction cache.)
+          const uint32_t t_s = t_lane + kColS + 64 * (t & 1), t_p = t_lane + kColP + 96 * (t & 1);
+          const auto scores = [&](int c0, float (&s)[16]) {
+            tmem_ld16(t_s + c0, s);
+            const unsigned h = (unsigned)(hidden >> c0) & 0xffffu;
+            if (__any_sync(0xffffffffu, h != 0)) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float s[32];
-          scores(half, s);
-          float mx0 = s[0], mx1 = s[1];
+              for (int c = 0; c < 16; ++c)
+                if (h >> c & 1) s[c] = -CUDART_INF_F;
+            }
+          };
+          float top = -CUDART_INF_F;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kKeys; c0 += 16) {
+            float s[16];
+            scores(c0, s);
+            float mx0 = s[0], mx1 = s[1];
 #pragma unroll
-          for (int c = 2; c < 30; c += 4) {
-            mx0 = fmax3(mx0, s[c], s[c + 1]);
-            mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+            for (int c = 2; c < 14; c += 4) {
+              mx0 = fmax3(mx0, s[c], s[c + 1]);
+              mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+            }
+            top = fmax3(top, fmax3(mx0, s[14], s[15]), mx1);
           }
-          top = fmax3(top, fmax3(mx0, s[30], s[31]), mx1);
-        }
-        const float mn = fmaxf(m, top * sc);
-        const float alpha = mn == m ? 1.f : exp2f(m - mn);
-        m = mn;
-        const float ref = m == -CUDART_INF_F ? 0.f : m;
-        float sum0 = 0.f, sum1 = 0.f;
-        __syncwarp();
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float s[32];
-          scores(half, s);
-#pragma unroll
-          for (int c = 0; c < 32; c += 16) {
+          const float mn = fmaxf(m, top * sc);
+          alpha = mn == m ? 1.f : fast_exp2(m - mn);
+          m = mn;
+          const float neg = m == -CUDART_INF_F ? 0.f : -m;
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kKeys; c0 += 16) {
+            float s[16];
             uint32_t pk[kTerms][8];
+            scores(c0, s);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float p0 = fast_exp2(fmaf(s[c + e], sc, -ref));
-              const float p1 = fast_exp2(fmaf(s[c + e + 1], sc, -ref));
-              sum0 += p0;
-              sum1 += p1;
+              float x0, x1;
+              ffma2(x0, x1, s[e], s[e + 1], sc, sc, neg, neg);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              fadd2(sum0, sum1, sum0, sum1, p0, p1);
               uint32_t x[kTerms];
               split3(p0, p1, x);
 #pragma unroll
               for (int i = 0; i < kTerms; ++i) pk[i][e / 2] = x[i];
             }
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < kTerms; ++i)
-              tmem_st8(t_lane + kColP + 96 * (t & 1) + 32 * i + 16 * half + c / 2, pk[i]);
+            for (int i = 0; i < kTerms; ++i) tmem_st8(t_p + 32 * i + c0 / 2, pk[i]);
           }
+          tmem_wait_st();
+          l = l * alpha + (sum0 + sum1);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full);
+          ++t;
         }
-        tmem_wait_st();
-        l = l * alpha + (sum0 + sum1);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full);
-        if (kt > pc.kt0) {
-          ok = add_o(t - 1);
+        if (j > 0) {
+          const int n = t - 1 - (j < tiles);  // the tile before
+          ok = __all_sync(0xffffffffu, wait_or_abort(&sm.o_full, n & 1, err));
           if (!ok) break;
-        }
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+          tc_fence_after();
 #pragma unroll
-          for (int e = 0; e < D; ++e) o[e] *= alpha;
-        }
-      }
-      if (!ok) break;
-      ok = add_o(t - 1);
-      if (!ok) break;
-      if (*reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) == rd) {
-        for (int key = pc.kt0 * kKeys; key <= limit && key < pc.kt1 * kKeys; ++key) {
-          const int page = page_of(p.kv, pc.seq, key);
-          if (page < 0) continue;
-          const float4* row = reinterpret_cast<const float4*>(
-              static_cast<const float*>(p.kv.v) + row_offset(p.kv, page, pc.head, key));
+          for (int c = 0; c < D; c += 32) {
+            float v[32];
+            tmem_ld32(t_lane + kColO + c, v);
 #pragma unroll
-          for (int c = 0; c < D / 4; ++c) {
-            const float4 x = row[c];
-            if (!finite(x.x)) o[4 * c] += x.x;
-            if (!finite(x.y)) o[4 * c + 1] += x.y;
-            if (!finite(x.z)) o[4 * c + 2] += x.z;
-            if (!finite(x.w)) o[4 * c + 3] += x.w;
+            for (int e = 0; e < 32; e += 2)
+              fadd2(o[c + e], o[c + e + 1], o[c + e], o[c + e + 1], v[e], v[e + 1]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.o_empty);
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < D; e += 2)
+              ffma2(o[e], o[e + 1], o[e], o[e + 1], alpha, alpha, 0.f, 0.f);
           }
         }
       }
+      if (!ok) break;
       // Rows leave through the warp's 4 KB: written a row per thread, read back so that eight
       // lanes cover 128 bytes of a row (16-byte chunk c of row i at c ^ (i % 8)).
       const bool whole = pc.slot < 0;
@@ -519,6 +549,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                                        (long long)(pc.tok + tk) * p.out_stride +
                                        (long long)(pc.head * G + row % G) * D + b * 32 + c * 4) = x;
         }
+        __syncwarp();
+      }
+      if (*reinterpret_cast<volatile int*>(&sm.poison[rd & 3]) == rd) {
+        // what was kept out of the product, to this thread's row where it was written
+        const int tk = r / G;
+        float* row = whole ? static_cast<float*>(p.out) +
+                                 (long long)(pc.tok + tk) * p.out_stride +
+                                 (long long)(pc.head * G + r % G) * D
+                           : part.chunk_o + (base + lane) * D;
+        if (r < kTok * G && tk < pc.n_tok) add_non_finite<D>(p, pc, limit, row);
         __syncwarp();
       }
     }
