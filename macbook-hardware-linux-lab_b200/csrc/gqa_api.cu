@@ -659,7 +659,7 @@ int check_paged(const gqa_ctx* c, const gqa_paged_kv* kv, int n_seq, int n_token
 cudaError_t alloc_paged(gqa_ctx* c, int group) {
   PagedPartials& w = c->paged;
   const size_t d = c->cfg.head_dim;
-  w.n_ctas = 2 * c->n_sm;
+  w.n_ctas = std::min(2 * c->n_sm, kMaxDecodeCtas);
   w.n_chunk_ctas = c->n_sm;
   const size_t rows = (size_t)2 * w.n_ctas * group;
   const size_t chunk_rows = (size_t)2 * w.n_chunk_ctas * kChunkSlotRows;

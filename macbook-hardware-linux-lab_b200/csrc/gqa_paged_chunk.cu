@@ -346,112 +346,81 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto all_wait = [&](uint64_t* bar, uint32_t parity) {
       return (bool)__all_sync(0xffffffffu, wait_lean(bar, parity, &sm.err));
     };
-    {
-      const auto issue_s = [&](int g, int kv) {
-        const uint32_t q = smem_addr(sm.q[g]), k = smem_addr(sm.k[kv & 1]);
-        if (!elect_one()) return;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
-          umma_ss(tmem + 128 * g, desc_k_major(q + off), desc_k_major(k + off), kIdS, ks > 0);
-        }
-        umma_commit(&sm.s_full[g]);
-      };
-      const auto issue_pv = [&](int g, int kv, bool acc) {
-        const uint32_t v = smem_addr(sm.v[kv & 1]);
-        if (!elect_one()) return;
-#pragma unroll
-        for (int ks = 0; ks < kKeys / 16; ++ks)
-          umma_ts(tmem + 256 + 128 * g, tmem + 128 * g + (ks & 3) * 8 + (ks >> 2) * 64,
-                  desc_mn_major(v + ks * 2048), kIdO, acc || ks > 0);
-      };
-      const auto take = [&](int n, Piece& pc) {
-        if (!all_wait(&sm.item_full[n & 3], (n >> 2) & 1)) return false;
-        pc = sm.ring[n & 3];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.item_empty[n & 3]);
-        return true;
-      };
-      // (after the matrix instructions before it, whichever lane issued them: the elected lane
-      // is the same one throughout)
-      const auto commit = [&](uint64_t* bar) {
-        if (elect_one()) umma_commit(bar);
-        __syncwarp();
-      };
-      Piece pc{};
-      int rd = 0, kv = 0, nq[2] = {0, 0}, nt[2] = {0, 0};  // Q tiles, S tiles of A and B
-      bool ok = take(0, pc);
-      bool two = pc.n_tok > kTok;
-      // S of a piece's first key tile
-      const auto first_s = [&](int kv, bool both, bool lone) {
-        if (!all_wait(&sm.q_full[0], nq[0] & 1) || !all_wait(&sm.k_full[kv & 1], (kv >> 1) & 1))
-          return false;
-        ++nq[0];
-        tc_fence_after();
-        issue_s(0, kv);
-        if (lone) commit(&sm.q_empty[0]);
-        if (both) {
-          if (!all_wait(&sm.q_full[1], nq[1] & 1)) return false;
-          ++nq[1];
-          tc_fence_after();
-          issue_s(1, kv);
-          if (lone) commit(&sm.q_empty[1]);
-        }
-        commit(&sm.k_empty[kv & 1]);
-        return true;
-      };
-      if (ok && pc.n_tok > 0) ok = first_s(0, two, pc.kt1 - pc.kt0 == 1);
-      int kt = pc.kt0;
-      while (ok && pc.n_tok > 0) {
-        // the key tile after this one: of the same piece, or the next one's first
-        Piece nx = pc;
-        int kt_n = kt + 1;
-        const bool last = kt_n == pc.kt1;
-        if (last) {
-          ok = take(++rd, nx);
-          if (!ok) break;
-          kt_n = nx.kt0;
-        }
-        const bool more = nx.n_tok > 0, two_n = nx.n_tok > kTok;
-        const bool n_last = kt_n + 1 == nx.kt1;
-        const int kv_n = kv + 1;
+    // (the elected lane is the same one throughout, so a commit covers all products before it)
+    const auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    const auto take = [&](int n, Piece& pc) {
+      if (!all_wait(&sm.item_full[n & 3], (n >> 2) & 1)) return false;
+      pc = sm.ring[n & 3];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[n & 3]);
+      return true;
+    };
+    // Descriptors differ in their low words alone.
+    const uint32_t q_low = (uint32_t)desc_k_major(smem_addr(sm.q[0]));
+    const uint32_t k_low = (uint32_t)desc_k_major(smem_addr(sm.k[0]));
+    const uint32_t v_low = (uint32_t)desc_mn_major(smem_addr(sm.v[0]));
+    const uint32_t high = (uint32_t)(desc_k_major(0) >> 32);
+    const auto desc = [&](uint32_t low) {
+      uint64_t d;
+      asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+      return d;
+    };
+    Piece pc{};
+    int rd = 0, kv = 0;              // pieces; key tiles whose P V is issued
+    uint32_t q_turn = 0, p_turn = 0; // parities of Q and P, a bit for each of A and B
+    bool ok = take(0, pc);
+    while (ok && pc.n_tok > 0) {
+      const int tiles = pc.kt1 - pc.kt0, both = pc.n_tok > kTok;
+      // Turn j: P V of tile j - 1 and S of tile j, of A, then of B.  Written once and looped
+      // over, as the loops of all roles have to fit the instruction cache together.
+      for (int j = 0; j <= tiles && ok; ++j) {
         // What the loader brings is waited for first, while the softmax is still at work: the
-        // products then follow the weights at once, P V of this tile and S of the next (of the
-        // next piece only after the commits: its Q may be long in coming).
-        ok = all_wait(&sm.v_full[kv & 1], (kv >> 1) & 1);
-        if (ok && !last) ok = all_wait(&sm.k_full[kv_n & 1], (kv_n >> 1) & 1);
-        if (!ok || !all_wait(&sm.p_full[0], nt[0] & 1)) { ok = false; break; }
-        ++nt[0];
-        tc_fence_after();
-        issue_pv(0, kv, kt > pc.kt0);
-        if (!last) issue_s(0, kv_n);
-        if (!two) commit(&sm.v_empty[kv & 1]);
-        if (last) commit(&sm.o_final[0]);
-        if (!last && n_last) commit(&sm.q_empty[0]);
-        if (two) {
-          if (!all_wait(&sm.p_full[1], nt[1] & 1)) { ok = false; break; }
-          ++nt[1];
-          tc_fence_after();
-          issue_pv(1, kv, kt > pc.kt0);
-          if (!last) issue_s(1, kv_n);
-          commit(&sm.v_empty[kv & 1]);
-          if (last) commit(&sm.o_final[1]);
-          if (!last && n_last) commit(&sm.q_empty[1]);
-        }
-        if (!last) {
-          commit(&sm.k_empty[kv_n & 1]);
-        } else if (more) {
-          ok = first_s(kv_n, two_n, n_last);
+        // products then follow the weights at once.
+        const int kn = kv + (j > 0);
+        ok = (j == 0 || all_wait(&sm.v_full[kv & 1], (kv >> 1) & 1)) &&
+             (j == tiles || all_wait(&sm.k_full[kn & 1], (kn >> 1) & 1));
+#pragma unroll 1
+        for (int g = 0; g <= both && ok; ++g) {
+          uint32_t& turn = j == 0 ? q_turn : p_turn;
+          ok = all_wait(j == 0 ? &sm.q_full[g] : &sm.p_full[g], turn >> g & 1);
           if (!ok) break;
+          turn ^= 1u << g;
+          tc_fence_after();
+          if (elect_one()) {
+            if (j > 0) {
+              const uint32_t v = v_low + (kv & 1) * (kKeys * D * 2 / 16);
+              const uint32_t at = tmem + 128 * g;
+#pragma unroll
+              for (int ks = 0; ks < kKeys / 16; ++ks)
+                umma_ts(tmem + 256 + 128 * g, at + (ks & 3) * 8 + (ks >> 2) * 64,
+                        desc(v + ks * 2048 / 16), kIdO, j > 1 || ks > 0);
+            }
+            if (j < tiles) {
+              const uint32_t q = q_low + g * (kRowsTile * D * 2 / 16);
+              const uint32_t k = k_low + (kn & 1) * (kKeys * D * 2 / 16);
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks) {
+                const uint32_t off = ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32) / 16;
+                umma_ss(tmem + 128 * g, desc(q + off), desc(k + off), kIdS, ks > 0);
+              }
+              umma_commit(&sm.s_full[g]);
+            }
+            if (j == tiles) umma_commit(&sm.o_final[g]);
+            if (j + 1 == tiles) umma_commit(&sm.q_empty[g]);
+          }
+          __syncwarp();
         }
-        pc = nx;
-        two = two_n;
-        kt = kt_n;
-        kv = kv_n;
+        if (ok && j > 0) commit(&sm.v_empty[kv & 1]);
+        if (ok && j < tiles) commit(&sm.k_empty[kn & 1]);
+        kv += j > 0;
       }
-      commit(&sm.drain);  // no MMA may be running when tensor memory is freed
-      mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
+      if (ok) ok = take(++rd, pc);
     }
+    commit(&sm.drain);  // no MMA may be running when tensor memory is freed
+    mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
     __syncwarp();
   } else {
     // ---- softmax of tile g: row r (token r / G, head r % G), keys 64 half .. 64 half + 63 ----

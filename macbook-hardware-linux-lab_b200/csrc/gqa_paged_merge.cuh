@@ -8,68 +8,71 @@
 
 namespace gqa {
 
-// Merges the parts of a pair: one block per (CTA that holds a first part, query head).  The
-// parts' weights first (a part per thread), so that the loads of the outputs depend on nothing
-// and go out together.
+// A warp's merge of every `step`-th part of a pair from `first` on, for one query head.  (m, l) and
+// outputs are loaded together (nothing waits for a weight), up to 8 parts at once.
 constexpr int kMergeWarps = 8;
-constexpr int kMaxParts = kMaxDecodeCtas;
+constexpr int kPartsAtOnce = 8;
 
-template <typename T, int D, int G>
-__device__ void merge_pair(const PagedAttnParams& p, const PagedPartials& part, int cta, int g) {
-  __shared__ float weight[kMaxParts], red[2][kMergeWarps], so[kMergeWarps][D];
-  const PagedJob job = part.jobs[cta];
-  if (job.n_parts == 0) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+template <int D, int G>
+__device__ __forceinline__ void merge_parts(const PagedPartials& part, const PagedJob& job, int cta,
+                                            int g, int first, int step, float& m, float& l,
+                                            float (&o)[D / 32]) {
+  const int lane = threadIdx.x & 31;
   // the first part's slot, then slot 0 of each CTA after it
   const auto slot_of = [&](int i) { return i == 0 ? job.slot : 2 * (cta + i); };
-  constexpr int kOwn = kMaxParts / (kMergeWarps * 32);
-  float2 ml[kOwn];
-  float m = -CUDART_INF_F;
-#pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    const int i = tid + j * kMergeWarps * 32;
-    ml[j] = i < job.n_parts ? part.ml[slot_of(i) * G + g] : make_float2(-CUDART_INF_F, 0.f);
-    if (ml[j].y != 0.f) m = fmaxf(m, ml[j].x);
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (lane == 0) red[0][warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, red[0][w]);
-  float l = 0.f;
-#pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    const float a = ml[j].y != 0.f ? exp2f(ml[j].x - m) : 0.f;
-    l += a * ml[j].y;
-    weight[tid + j * kMergeWarps * 32] = a;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
+  constexpr int E = D / 32, kAtOnce = kPartsAtOnce;
+  m = -CUDART_INF_F;
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) l += red[1][w];
-  constexpr int E = D / 32;
-  float o[E];
-#pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i0 = warp; i0 < job.n_parts; i0 += 8 * kMergeWarps) {
-    float x[8][E], a[8];
+  for (int i0 = first; i0 < job.n_parts; i0 += kAtOnce * step) {
+    const int own = i0 + (lane & (kAtOnce - 1)) * step;  // the part of this lane's (m, l)
+    const float2 ml =
+        own < job.n_parts ? part.ml[slot_of(own) * G + g] : make_float2(-CUDART_INF_F, 0.f);
+    float x[kAtOnce][E];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = min(i0 + u * kMergeWarps, job.n_parts - 1);
-      a[u] = i0 + u * kMergeWarps < job.n_parts ? weight[i] : 0.f;
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * step;
       const float* src = part.o + ((long long)slot_of(i) * G + g) * D + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[u][e] = src[e];
+      for (int e = 0; e < E; ++e) x[u][e] = i < job.n_parts ? src[e] : 0.f;
     }
+    float mx = ml.y != 0.f ? ml.x : -CUDART_INF_F;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (a[u] != 0.f)  // (a part without a row holds nothing to be added)
+    for (int d = kAtOnce / 2; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    mx = fmaxf(m, mx);
+    if (mx == -CUDART_INF_F) continue;  // (nothing in any of them; alike in the warp's lanes)
+    const float a = exp2f(m - mx), w = ml.y != 0.f ? exp2f(ml.x - mx) : 0.f;
+    float add = w * ml.y;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += a[u] * x[u][e];
+    for (int d = kAtOnce / 2; d; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+    m = mx;
+    l = l * a + add;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= a;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float wu = __shfl_sync(0xffffffffu, w, u);
+      if (wu != 0.f)  // (a part without a row holds nothing to be added)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += wu * x[u][e];
+    }
+  }
+}
+
+// A pair's query head, by a block.
+template <typename T, int D, int G>
+__device__ void merge_by_block(const PagedAttnParams& p, const PagedPartials& part,
+                               const PagedJob& job, int cta, int g) {
+  __shared__ float sm[kMergeWarps], sl[kMergeWarps], so[kMergeWarps][D];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int E = D / 32;
+  float m, l, o[E];
+  merge_parts<D, G>(part, job, cta, g, warp, kMergeWarps, m, l, o);
+  __syncthreads();
+  if (lane == 0) {
+    sm[warp] = m;
+    sl[warp] = l;
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
@@ -77,83 +80,111 @@ __device__ void merge_pair(const PagedAttnParams& p, const PagedPartials& part, 
   T* out = static_cast<T*>(p.out) + (long long)job.tok * p.out_stride +
            (long long)(job.head * G + g) * D;
   for (int e = tid; e < D; e += kMergeWarps * 32) {
-    float sum = 0.f;
+    float mm = -CUDART_INF_F;
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) sum += so[w][e];
-    out[e] = Elem<T>::put(l != 0.f ? sum / l : 0.f);
+    for (int w = 0; w < kMergeWarps; ++w) mm = fmaxf(mm, sm[w]);
+    float ll = 0.f, oo = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+      if (sl[w] == 0.f) continue;
+      const float a = exp2f(sm[w] - mm);
+      ll += a * sl[w];
+      oo += a * so[w][e];
+    }
+    out[e] = Elem<T>::put(ll != 0.f ? oo / ll : 0.f);
   }
 }
 
-// Merges the parts of a unit that crossed shares: a warp per row.
-template <typename T, int D, int G>
-__device__ void merge_unit_row(const PagedAttnParams& p, const PagedPartials& part,
-                               const PagedChunkJob& job, int cta, int idx) {
-  constexpr int kTok = kChunkRows / G, E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int t = idx / G, g = idx % G;
-  if (t >= job.n_tok) return;
-  const int row = t < kTok ? idx : kChunkRows + (t - kTok) * G + g;
-  const auto at = [&](int i) {
+// Merges the parts of a unit that crossed shares: R rows at a time per warp, two parts at once,
+// all loads of which go out together.
+template <typename T, int D, int G, int R>
+__device__ void merge_unit_rows(const PagedAttnParams& p, const PagedPartials& part,
+                                const PagedChunkJob& job, int cta, int idx0, int step) {
+  constexpr int kTok = kChunkRows / G, E = D / 32, kAtOnce = 2;
+  const int lane = threadIdx.x & 31, rows = job.n_tok * G;
+  const auto at = [&](int i, int r) {
+    const int idx = min(idx0 + r * step, rows - 1), t = idx / G;
+    const int row = t < kTok ? idx : kChunkRows + idx - kTok * G;
     return (long long)(i == 0 ? job.slot : 2 * (cta + i)) * kChunkSlotRows + row;
   };
-  // the parts' weights, a part per lane; then loads that depend on nothing
-  float m = -CUDART_INF_F, l = 0.f, o[E];
-  for (int i = lane; i < job.n_parts; i += 32) {
-    const float2 ml = part.chunk_ml[at(i)];
-    if (ml.y != 0.f) m = fmaxf(m, ml.x);
+  float m[R], l[R], o[R][E];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -CUDART_INF_F;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[r][e] = 0.f;
   }
+  for (int i0 = 0; i0 < job.n_parts; i0 += kAtOnce) {
+    float2 ml[R][kAtOnce];
+    float x[R][kAtOnce][E];
 #pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i0 = 0; i0 < job.n_parts; i0 += 32) {
-    float2 ml = make_float2(0.f, 0.f);
-    if (i0 + lane < job.n_parts) ml = part.chunk_ml[at(i0 + lane)];
-    const float weight = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
-    l += weight * ml.y;
-    for (int i = i0; i < min(i0 + 32, job.n_parts); i += 8) {
-      float x[8][E];
+      for (int u = 0; u < kAtOnce; ++u) {
+        const bool on = i0 + u < job.n_parts;
+        const long long a = at(on ? i0 + u : 0, r);
+        ml[r][u] = on ? part.chunk_ml[a] : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+        for (int e = 0; e < E; ++e) x[r][u][e] = on ? part.chunk_o[a * D + lane * E + e] : 0.f;
+      }
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          x[u][e] = i + u < job.n_parts ? part.chunk_o[at(i + u) * D + lane * E + e] : 0.f;
+    for (int r = 0; r < R; ++r) {
+      float mx = m[r];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float a = __shfl_sync(0xffffffffu, weight, i - i0 + u);
-        if (a != 0.f)
+      for (int u = 0; u < kAtOnce; ++u)
+        if (ml[r][u].y != 0.f) mx = fmaxf(mx, ml[r][u].x);
+      if (mx == -CUDART_INF_F) continue;
+      const float a = exp2f(m[r] - mx);
+      m[r] = mx;
+      l[r] *= a;
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += a * x[u][e];
+      for (int e = 0; e < E; ++e) o[r][e] *= a;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (ml[r][u].y == 0.f) continue;
+        const float w = exp2f(ml[r][u].x - mx);
+        l[r] += w * ml[r][u].y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] += w * x[r][u][e];
       }
     }
   }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  T* out = static_cast<T*>(p.out) + (long long)(job.tok + t) * p.out_stride +
-           (long long)(job.head * G + g) * D + lane * E;
+  for (int r = 0; r < R; ++r) {
+    const int idx = idx0 + r * step;
+    if (idx >= rows) break;
+    T* out = static_cast<T*>(p.out) + (long long)(job.tok + idx / G) * p.out_stride +
+             (long long)(job.head * G + idx % G) * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = Elem<T>::put(l != 0.f ? o[e] / l : 0.f);
+    for (int e = 0; e < E; ++e) out[e] = Elem<T>::put(l[r] != 0.f ? o[r][e] / l[r] : 0.f);
+  }
 }
 
 // Blocks: one per (decode CTA, query head), then kUnitSlabs per chunk CTA.  Most find nothing to
-// merge and leave.
-constexpr int kUnitSlabs = 32;
+// merge and leave, so registers are kept to what lets four share an SM: with 16 parts at once and
+// three, 64 sequences took 63 us in place of 59.7, a batch with chunks among them 100 in place of 96.5; one
+// token over 32768 rows gains 2 us from blocks of 16 warps, the others lose 1 to 4.  (One list of
+// the jobs, made by every block for itself and dealt out evenly, took 104 us in place of 97 for
+// four whole prompts.)
+constexpr int kUnitSlabs = 8, kUnitRows = 2;
 
 template <typename T, int D, int G>
-__global__ void __launch_bounds__(kMergeWarps * 32)
+__global__ void __launch_bounds__(kMergeWarps * 32, 4)
     paged_merge_kernel(const PagedAttnParams p, const PagedPartials part, const int n_decode) {
   pdl_wait();
   const int b = blockIdx.x;
   if (b < n_decode * G) {
-    merge_pair<T, D, G>(p, part, b / G, b % G);
+    const PagedJob job = part.jobs[b / G];
+    if (job.n_parts > 0) merge_by_block<T, D, G>(p, part, job, b / G, b % G);
     return;
   }
   const int cta = (b - n_decode * G) / kUnitSlabs, slab = (b - n_decode * G) % kUnitSlabs;
   const PagedChunkJob job = part.chunk_jobs[cta];
   if (job.n_parts == 0) return;
-  for (int i = slab * kMergeWarps + (threadIdx.x >> 5); i < job.n_tok * G;
-       i += kUnitSlabs * kMergeWarps)
-    merge_unit_row<T, D, G>(p, part, job, cta, i);
+  constexpr int kStep = kUnitSlabs * kMergeWarps;
+  for (int i = slab * kMergeWarps + (threadIdx.x >> 5); i < job.n_tok * G; i += kUnitRows * kStep)
+    merge_unit_rows<T, D, G, kUnitRows>(p, part, job, cta, i, kStep);
 }
 
 }  // namespace gqa
