@@ -505,6 +505,22 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int g = 0; g < kStages - 1; ++g) flight[g] = issue(g);
 
+    const bool whole = t0 == 0 && t1 == tiles;
+    if (!whole && tid == kThreads - 1) {
+      // what the merge's block of this CTA's number does (the divisions while rows arrive)
+      // Query heads of many parts are listed apart from one another: neighbours' blocks would
+      // share an SM, whose reads then bound them (3 us more over 32768 rows).  Never under the
+      // last CTA, which may list its next pair.
+      static_assert(kFewParts >= G, "a CTA per query head, and one more");
+      const auto cta_of = [&](long long t) { return (int)(((t + 1) * n - 1) / total); };
+      const int c0 = cta_of(pair_first), n_parts = cta_of(pair_first + tiles - 1) - c0 + 1;
+      const int i = (int)blockIdx.x - c0, apart = n_parts > kFewParts ? n_parts / G : 1;
+      const int slot0 = 2 * c0 + (pair_first == c0 * total / n ? 0 : 1);
+      if (i == 0 || (n_parts > kFewParts && i % apart == 0 && i / apart < G))
+        part.jobs[blockIdx.x] =
+            PagedJob{tok, h, c0, slot0, n_parts, n_parts > kFewParts ? i / apart : -1};
+    }
+
     // q of the token, rotated for its position and scaled, while the first rows arrive
     const T* q = static_cast<const T*>(p.qkv) + (long long)tok * p.qkv_stride +
                  (long long)h * G * D;
@@ -550,7 +566,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     static_assert(sizeof(sm.k[0]) >= sizeof(float) * kHeads * D, "room for the warp's output");
     st.end(sm, warp, lane, so);
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
     const int slot = 2 * blockIdx.x + (tile == first ? 0 : 1);
     T* out = static_cast<T*>(p.out) + (long long)tok * p.out_stride + (long long)h * G * D;
     for (int i = tid; i < G * D; i += kThreads) {
@@ -573,12 +588,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         part.o[(long long)slot * G * D + i] = oo;
         if (i % D == 0) part.ml[slot * G + g] = make_float2(mm, ll);
       }
-    }
-    if (!whole && t0 == 0 && tid == 0) {
-      // this CTA holds the pair's first part: the merge is listed under it
-      const long long end = pair_first + tiles;
-      const int last_cta = (int)((end * n + total - 1) / total) - 1;
-      part.jobs[blockIdx.x] = PagedJob{tok, h, slot, last_cta - (int)blockIdx.x + 1};
     }
     tile = pair_first + t1;
     __syncthreads();
@@ -607,7 +616,7 @@ cudaError_t launch_one(const PagedAttnParams& p, const PagedPartials& part, int 
 template <typename T, int D, int G>
 cudaError_t merge_one(const PagedAttnParams& p, const PagedPartials& part, int n_decode,
                       int n_chunk, cudaStream_t st) {
-  return launch_with_pdl(paged_merge_kernel<T, D, G>, dim3(n_decode * G + n_chunk * kUnitSlabs),
+  return launch_with_pdl(paged_merge_kernel<T, D, G>, dim3(n_decode + n_chunk * kUnitSlabs),
                          kMergeWarps * 32, 0, st, true, p, part, n_decode);
 }
 

@@ -10,12 +10,16 @@
 namespace gqa {
 
 // Parts of (token, KV head) pairs whose rows were split over CTAs: two slots per CTA, each
-// [G][D] un-normalised outputs and [G] (m in log2 units, l), and under the CTA that holds a
-// pair's first part what is to be merged.
-struct PagedJob {
-  int tok, head, slot;
-  int n_parts;  // CTAs from this one on (0: nothing to merge)
+// [G][D] un-normalised outputs and [G] (m in log2 units, l), and what the merge's block of the
+// same number does: all query heads of a pair of few parts, listed under the CTA that holds its
+// first; else one of them, listed under one of the pair's first G CTAs each.
+struct alignas(16) PagedJob {
+  int tok, head;
+  int cta, slot;  // of the first part
+  int n_parts;    // CTAs from `cta` on (0: nothing to merge)
+  int q_head;     // -1: all
 };
+constexpr int kFewParts = 8;  // of a pair whose query heads a warp each merges
 // The same for chunks: units of some tokens, 256 rows a slot.
 struct PagedChunkJob {
   int tok, n_tok, head, slot;

@@ -11,16 +11,15 @@ namespace gqa {
 // A warp's merge of every `step`-th part of a pair from `first` on, for one query head.  (m, l) and
 // outputs are loaded together (nothing waits for a weight), up to 8 parts at once.
 constexpr int kMergeWarps = 8;
-constexpr int kPartsAtOnce = 8;
 
 template <int D, int G>
-__device__ __forceinline__ void merge_parts(const PagedPartials& part, const PagedJob& job, int cta,
-                                            int g, int first, int step, float& m, float& l,
+__device__ __forceinline__ void merge_parts(const PagedPartials& part, const PagedJob& job, int g,
+                                            int first, int step, float& m, float& l,
                                             float (&o)[D / 32]) {
   const int lane = threadIdx.x & 31;
   // the first part's slot, then slot 0 of each CTA after it
-  const auto slot_of = [&](int i) { return i == 0 ? job.slot : 2 * (cta + i); };
-  constexpr int E = D / 32, kAtOnce = kPartsAtOnce;
+  const auto slot_of = [&](int i) { return i == 0 ? job.slot : 2 * (job.cta + i); };
+  constexpr int E = D / 32, kAtOnce = kFewParts;
   m = -CUDART_INF_F;
   l = 0.f;
 #pragma unroll
@@ -60,15 +59,28 @@ __device__ __forceinline__ void merge_parts(const PagedPartials& part, const Pag
   }
 }
 
-// A pair's query head, by a block.
+// A pair of few parts, a query head by a warp.
+template <typename T, int D, int G>
+__device__ __forceinline__ void merge_by_warp(const PagedAttnParams& p, const PagedPartials& part,
+                                              const PagedJob& job, int g) {
+  constexpr int E = D / 32;
+  float m, l, o[E];
+  merge_parts<D, G>(part, job, g, 0, 1, m, l, o);
+  T* out = static_cast<T*>(p.out) + (long long)job.tok * p.out_stride +
+           (long long)(job.head * G + g) * D + (threadIdx.x & 31) * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = Elem<T>::put(l != 0.f ? o[e] / l : 0.f);
+}
+
+// A query head of many, by a block.
 template <typename T, int D, int G>
 __device__ void merge_by_block(const PagedAttnParams& p, const PagedPartials& part,
-                               const PagedJob& job, int cta, int g) {
+                               const PagedJob& job, int g) {
   __shared__ float sm[kMergeWarps], sl[kMergeWarps], so[kMergeWarps][D];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int E = D / 32;
   float m, l, o[E];
-  merge_parts<D, G>(part, job, cta, g, warp, kMergeWarps, m, l, o);
+  merge_parts<D, G>(part, job, g, warp, kMergeWarps, m, l, o);
   __syncthreads();
   if (lane == 0) {
     sm[warp] = m;
@@ -161,12 +173,13 @@ __device__ void merge_unit_rows(const PagedAttnParams& p, const PagedPartials& p
   }
 }
 
-// Blocks: one per (decode CTA, query head), then kUnitSlabs per chunk CTA.  Most find nothing to
-// merge and leave, so registers are kept to what lets four share an SM: with 16 parts at once and
-// three, 64 sequences took 63 us in place of 59.7, a batch with chunks among them 100 in place of 96.5; one
-// token over 32768 rows gains 2 us from blocks of 16 warps, the others lose 1 to 4.  (One list of
-// the jobs, made by every block for itself and dealt out evenly, took 104 us in place of 97 for
-// four whole prompts.)
+// Blocks: one per decode CTA, which does what that CTA listed, then kUnitSlabs per chunk CTA.  All
+// of a decode's fit on the device at once (a block per CTA and query head, most of which found
+// nothing, took three waves: 58.6 us in place of 56.6 for 64 sequences), and registers are kept to
+// what lets four share an SM: with 16 parts at once and three, 64 sequences took 3 us more.  The
+// merge is 4.5 us of the 12 and 21 of one token over 4096 and 32768 rows in fp32, and is bound by
+// the chain of its loads.  (One list of the jobs, made by every block for itself and dealt out
+// evenly, took 104 us in place of 97 for four whole prompts.)
 constexpr int kUnitSlabs = 8, kUnitRows = 2;
 
 template <typename T, int D, int G>
@@ -174,12 +187,17 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 4)
     paged_merge_kernel(const PagedAttnParams p, const PagedPartials part, const int n_decode) {
   pdl_wait();
   const int b = blockIdx.x;
-  if (b < n_decode * G) {
-    const PagedJob job = part.jobs[b / G];
-    if (job.n_parts > 0) merge_by_block<T, D, G>(p, part, job, b / G, b % G);
+  if (b < n_decode) {
+    static_assert(kMergeWarps >= G, "a warp per query head");
+    const PagedJob job = part.jobs[b];
+    if (job.n_parts == 0) return;
+    if (job.q_head >= 0)
+      merge_by_block<T, D, G>(p, part, job, job.q_head);
+    else if ((threadIdx.x >> 5) < G)
+      merge_by_warp<T, D, G>(p, part, job, threadIdx.x >> 5);
     return;
   }
-  const int cta = (b - n_decode * G) / kUnitSlabs, slab = (b - n_decode * G) % kUnitSlabs;
+  const int cta = (b - n_decode) / kUnitSlabs, slab = (b - n_decode) % kUnitSlabs;
   const PagedChunkJob job = part.chunk_jobs[cta];
   if (job.n_parts == 0) return;
   constexpr int kStep = kUnitSlabs * kMergeWarps;
