@@ -19,7 +19,7 @@
 //
 // A row belongs to a cluster of CTAs, each with a contiguous slice of it in shared
 // memory (logits past what fits are read again from memory), so a row is read from
-// memory once.  The last kept element is found in two steps: a histogram over 2048
+// memory once.  The last kept element is found in two steps: a histogram over 4096
 // equal steps of the exponent (they hold few elements each, wherever the logits lie,
 // and equal logits fall together), merged over the cluster by reads of the other CTAs'
 // shared memory, gives the step; its few elements are listed and ranked by comparing all
@@ -39,7 +39,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;       // four per thread
+constexpr int kBins = 4096;       // eight per thread
 constexpr int kList = 512;
 // A top_k up to which the row's first k are looked for by way of the threads' largest logits.
 constexpr int kSmallK = 256;
@@ -49,24 +49,29 @@ constexpr int kBlock = kThreads * 4;  // elements of one turn of the CTA's threa
 using u64 = unsigned long long;
 
 constexpr int kGroups = 64;                 // of the steps, for the first look over the cluster
-constexpr int kInGroup = kBins / kGroups;   // 32: a warp's lanes
+constexpr int kInGroup = kBins / kGroups;   // 64: two per lane of a warp
+constexpr int kSums = (1 << 20) / kMaxCluster / 128 + kWarps;  // of the largest slice
 
 struct alignas(16) Shared {  // (the slice of the row follows it)
   union {
     uint32_t hist[kBins];
-    u64 sums[kBins / 2 + kWarps];  // for the pick: weights of 128 elements each
+    u64 sums[kSums];  // for the pick: weights of 128 elements each
+    struct {          // for the finish, by rank
+      u64 ord[kList], w[kList], i[kList], kept[kList];
+    } by_rank;
   };
   alignas(16) u64 group[kGroups];      // sums of the histogram's groups
-  u64 list_ord[kList], list_w[kList];  // this CTA's elements of the step
-  u64 over_ord[kList], over_w[kList];  // and those before it, while they fit
+  u64 list_ord[kList];                 // this CTA's elements of the step
+  u64 over_ord[kList];                 // and those before it, while they fit
   u64 all_ord[kList], all_w[kList];    // the cluster's
   u64 x[2][4];                         // values exchanged over the cluster
   u64 got[kMaxCluster][4];
   u64 red[kWarps][4];
   double pow2[64];                     // 2^(j / 64 + wshift)
   u64 found_before, found_all, cut;
-  int found;
+  int found, row;
   uint32_t n_list, n_over;
+  alignas(16) u64 counts[kWarps];  // rows of each class by warp, ten bits a class
 };
 
 // Keys in the order of the logits: larger logit, larger key.
@@ -78,7 +83,7 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 // -0 as 0, NaN as -inf.
-__device__ __forceinline__ float clean(float x) { return x != x ? -CUDART_INF_F : x + 0.0f; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -CUDART_INF_F) + 0.0f; }
 
 __device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
   u64 v;
@@ -87,6 +92,10 @@ __device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
 }
 __device__ __forceinline__ void ld_cluster_v2(uint32_t addr, u64 (&v)[2]) {
   asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ld_cluster_v2(uint32_t addr, uint32_t (&v)[2]) {
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr)
                : "memory");
 }
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
@@ -286,7 +295,10 @@ struct Row {
   }
 
   __device__ void clear_hist() {
-    *reinterpret_cast<uint4*>(&sm.hist[4 * tid]) = make_uint4(0, 0, 0, 0);
+    static_assert(kBins == 8 * kThreads, "eight steps a thread");
+#pragma unroll
+    for (int j = 0; j < 8; j += 4)
+      *reinterpret_cast<uint4*>(&sm.hist[8 * tid + j]) = make_uint4(0, 0, 0, 0);
     if (tid == 0) sm.n_list = sm.n_over = 0;
     __syncthreads();
   }
@@ -300,13 +312,13 @@ struct Row {
   // Puts the sums of the histogram's groups beside it (before an exchange).
   __device__ void sum_groups(bool by_weight) {
     __syncthreads();
-    const int s = 4 * tid;
+    const int s = 8 * tid;
     u64 x = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x += (u64)sm.hist[s + j] << (by_weight ? shift_of(s + j) : 0);
+    for (int j = 0; j < 8; ++j) x += (u64)sm.hist[s + j] << (by_weight ? shift_of(s + j) : 0);
 #pragma unroll
-    for (int d = kInGroup / 8; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    if (tid % (kInGroup / 4) == 0) sm.group[tid / (kInGroup / 4)] = x;
+    for (int d = kInGroup / 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    if (tid % (kInGroup / 8) == 0) sm.group[tid / (kInGroup / 8)] = x;
   }
 
   // After the exchange: the step of the cluster's histogram at which the running sum reaches
@@ -334,18 +346,28 @@ struct Row {
       if (g[1] && (double)b1 < want) at = 2 * lane + 1;
       const int gr = max(__reduce_max_sync(0xffffffffu, at), 0);
       u64 before = __shfl_sync(0xffffffffu, gr & 1 ? b1 : b0, gr >> 1);
-      const int s = gr * kInGroup + lane;
-      uint32_t ph[kMaxCluster];
-      u64 h = 0;
+      const int s = gr * kInGroup + 2 * lane;
+      uint32_t ph[kMaxCluster][2];
+      u64 h[2] = {0, 0};
 #pragma unroll
       for (int r = 0; r < kMaxCluster; ++r)
-        ph[r] = ld_cluster_u32(cluster_map(&sm.hist[s], min(r, ranks - 1)));
+        ld_cluster_v2(cluster_map(&sm.hist[s], min(r, ranks - 1)), ph[r]);
 #pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r) h += r < ranks ? ph[r] : 0;
-      if (by_weight) h <<= shift_of(s);
-      const u64 b = before + warp_scan(h, lane) - h;
-      const int in = max(__reduce_max_sync(0xffffffffu, h && (double)b < want ? lane : -1), 0);
-      before = __shfl_sync(0xffffffffu, b, in);
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < ranks) {
+          h[0] += ph[r][0];
+          h[1] += ph[r][1];
+        }
+      if (by_weight) {
+        h[0] <<= shift_of(s);
+        h[1] <<= shift_of(s + 1);
+      }
+      const u64 c0 = before + warp_scan(h[0] + h[1], lane) - h[0] - h[1], c1 = c0 + h[0];
+      at = -1;
+      if (h[0] && (double)c0 < want) at = 2 * lane;
+      if (h[1] && (double)c1 < want) at = 2 * lane + 1;
+      const int in = max(__reduce_max_sync(0xffffffffu, at), 0);
+      before = __shfl_sync(0xffffffffu, in & 1 ? c1 : c0, in >> 1);
       if (lane == 0) {
         sm.found = gr * kInGroup + in;
         sm.found_before = before;
@@ -371,10 +393,9 @@ struct Row {
   }
 
   // Appends an element to a list of the CTA.
-  __device__ __forceinline__ static int put(uint32_t& count, u64* list, u64 o) {
+  __device__ __forceinline__ static void put(uint32_t& count, u64* list, u64 o) {
     const uint32_t at = atomicAdd(&count, 1u);
     if (at < kList) list[at] = o;
-    return (int)min(at, 1u << 30);
   }
 
   // The cluster's lists of the step into sm.all_* (counts in the exchange's last value: the
@@ -385,10 +406,12 @@ struct Row {
       const int c = (int)(uint32_t)sm.got[r][3], o = over ? (int)(sm.got[r][3] >> 32) : 0;
       for (int i = tid; i < c + o; i += kThreads) {
         const u64* from = i < c ? &sm.list_ord[i] : &sm.over_ord[i - c];
-        sm.all_ord[at + i] = ld_cluster_u64(cluster_map(from, r));
+        const u64 e = ld_cluster_u64(cluster_map(from, r));
+        sm.all_ord[at + i] = e;
         if (weights) {
-          from = i < c ? &sm.list_w[i] : &sm.over_w[i - c];
-          sm.all_w[at + i] = ld_cluster_u64(cluster_map(from, r));
+          const float x = key_logit((uint32_t)(e >> 32));
+          double w64;
+          sm.all_w[at + i] = weight(x, x > floor_x, w64);
         }
       }
       at += c + o;
@@ -434,14 +457,14 @@ struct Row {
       const float x = key_logit((uint32_t)(o >> 32));
       double w64;
       const u64 w = weight(x, x > floor_x, w64);
-      sm.over_ord[at] = o;
+      sm.by_rank.ord[at] = o;
       // the weight, and whether min_p leaves it out in the top bit (weights stay below 2^51)
-      sm.over_w[at] = w | (u64)(w64 < (double)min_p * most && at > 0) << 63;
+      sm.by_rank.w[at] = w | (u64)(w64 < (double)min_p * most && at > 0) << 63;
     }
     __syncthreads();
     // cumulative weight in rank order, one rank a thread
     static_assert(kList <= kThreads, "a thread per element");
-    const u64 marked = tid < m ? sm.over_w[tid] : 0;
+    const u64 marked = tid < m ? sm.by_rank.w[tid] : 0;
     const u64 w = marked & (~0ull >> 1);
     u64 incl = warp_scan(w, lane);
     if (lane == 31) sm.red[warp][0] = incl;
@@ -457,18 +480,18 @@ struct Row {
                        (tid == 0 || !(share < 1.0) || (double)(incl - w) < target);
     u64 mass[1] = {stays ? w : 0};
     if (tid < m) {
-      sm.list_ord[tid] = stays ? 0xffffffffu - (uint32_t)sm.over_ord[tid] : 0xffffffffu;
-      sm.list_w[tid] = mass[0];
+      sm.by_rank.i[tid] = stays ? 0xffffffffu - (uint32_t)sm.by_rank.ord[tid] : 0xffffffffu;
+      sm.by_rank.kept[tid] = mass[0];
     }
     block_reduce<false, 1>(mass);
     u = u > 0.f ? u : 0.f;
     const double ut = (double)u * (double)mass[0];
     const u64 pick = ut < (double)mass[0] ? (u64)ut : mass[0] - 1;
     if (stays && w) {
-      const u64 me = sm.list_ord[tid];
+      const u64 me = sm.by_rank.i[tid];
       u64 run = 0;
 #pragma unroll 8
-      for (int j = 0; j < m; ++j) run += sm.list_ord[j] <= me ? sm.list_w[j] : 0;
+      for (int j = 0; j < m; ++j) run += sm.by_rank.i[j] <= me ? sm.by_rank.kept[j] : 0;
       if (run > pick && run - w <= pick) *token = (int)me;
     }
   }
@@ -501,7 +524,7 @@ struct Row {
     u64 want = k - sm.found_before;  // rank within the interval
     u64 first = 0, last = ~0ull;     // ords of the interval
     bool by_step = true;
-    // (each turn narrows the interval to one of 2048 parts: 64 bits take six)
+    // (each turn narrows the interval to one of 4096 parts: 64 bits take six)
     for (int guard = 0; guard < 16; ++guard) {
       u64 mm[2] = {0, 0};  // largest ord, largest ~ord
       each(by_step ? below(step) : below(kBins), [&](float x, int i) {
@@ -529,7 +552,7 @@ struct Row {
       }
       narrow(first, last);
       by_step = false;
-      const int shift = max(0, 53 - __clzll(last - first));  // (last - first) >> shift < kBins
+      const int shift = max(0, 52 - __clzll(last - first));  // (last - first) >> shift < kBins
       clear_hist();
       each(below(kBins), [&](float x, int i) {
         const u64 o = ord(x, i);
@@ -594,14 +617,10 @@ struct Row {
         const u64 w = weight(x, x > floor_x, w64);
         if (b < step) {
           s[0] += w;
-          if (shift < 0 && *(volatile uint32_t*)&sm.n_over < kList) {
-            const int at = put(sm.n_over, sm.over_ord, o);
-            if (at < kList) sm.over_w[at] = w;
-          }
+          if (shift < 0 && *(volatile uint32_t*)&sm.n_over < kList) put(sm.n_over, sm.over_ord, o);
         } else {
           s[1] += w;
-          const int at = put(sm.n_list, sm.list_ord, o);
-          if (at < kList) sm.list_w[at] = w;
+          put(sm.n_list, sm.list_ord, o);
         }
       });
       block_reduce<false, 2>(s);
@@ -652,7 +671,7 @@ struct Row {
       exchange(mm[0], mm[1]);
       narrow(first, last);
       above = before;
-      shift = max(0, 53 - __clzll(last - first));
+      shift = max(0, 52 - __clzll(last - first));
       clear_hist();
       double largest;
       weight(key_logit((uint32_t)(last >> 32)), true, largest);
@@ -766,12 +785,6 @@ __device__ void load_slice(const T* base, int skip, int n, int n_held, float* he
   constexpr int V = 16 / (int)sizeof(T), kAhead = 4;
   best = -CUDART_INF_F;
   at = 0;
-  const auto see = [&](float v, int i) {
-    if (v > best || (v == best && i < at)) {
-      best = v;
-      at = i;
-    }
-  };
   const int tid = threadIdx.x;
   const int g0 = skip ? 1 : 0, g1 = max(g0, min(n, n_held) / V);  // whole vectors
   for (int g = g0 + tid; g < g1; g += kAhead * kThreads) {
@@ -787,9 +800,13 @@ __device__ void load_slice(const T* base, int skip, int n, int n_held, float* he
         const T* e = reinterpret_cast<const T*>(&r[u]);
         float v[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          v[j] = clean(Elem<T>::get(e[j]));
-          see(v[j], i + j);
+        for (int j = 0; j < V; ++j) v[j] = clean(Elem<T>::get(e[j]));
+        float most = v[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) most = fmaxf(most, v[j]);
+        if (most > best) {
+          best = most;
+          at = i;  // (of the vector; the element is looked up below)
         }
 #pragma unroll
         for (int j = 0; j < V; j += 4)
@@ -797,31 +814,83 @@ __device__ void load_slice(const T* base, int skip, int n, int n_held, float* he
       }
     }
   }
+  if (best > -CUDART_INF_F) {
+    const int i = at;
+#pragma unroll
+    for (int j = V - 1; j >= 0; --j)
+      if (held[i + j] == best) at = i + j;
+  }
   const auto one = [&](int i) {
     const float v = i >= skip && i < n ? clean(Elem<T>::get(base[i])) : -CUDART_INF_F;
     if (i < n_held) held[i] = v;
-    see(v, i);
+    if (v > best || (v == best && i < at)) {
+      best = v;
+      at = i;
+    }
   };
   for (int i = tid; i < g0 * V; i += kThreads) one(i);
   for (int i = g1 * V + tid; i < max(n, n_held); i += kThreads) one(i);
 }
 
+// The row of cluster q when there are more clusters than run at once: within each 512 rows those
+// of the costliest settings come first, so that no long row starts when the others are done.
+__device__ int ordered_row(const SampleParams& p, Shared& sm, int q) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int base = q / kThreads * kThreads, row = base + tid;
+  int cls = -1;
+  if (row < p.n_rows) {
+    const float temp = p.temperature ? p.temperature[row] : 1.f;
+    const int k = p.top_k ? p.top_k[row] : 0;
+    const float top_p = p.top_p ? p.top_p[row] : 1.f;
+    const bool by_count = k > 0 && k < p.vocab;
+    cls = !(temp > 0.f) ? 0
+          : by_count && k <= kSmallK ? 1
+                                     : 2 + (top_p < 1.f ? 1 : 0) + (by_count ? 2 : 0);
+  }
+  static_assert(kThreads < 1024, "ten bits hold a class's rows");
+  u64 packed = 0;
+  int mine = 0;  // rows that come before the thread's
+#pragma unroll
+  for (int c = 0; c < 6; ++c) {
+    const unsigned in = __ballot_sync(0xffffffffu, cls == c);
+    packed |= (u64)__popc(in) << (10 * c);
+    if (cls == c) mine = __popc(in & ((1u << lane) - 1));
+  }
+  if (lane == 0) sm.counts[warp] = packed;
+  __syncthreads();
+  u64 all = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const u64 x = sm.counts[w];
+    all += x;
+    before += w < warp ? x : 0;
+  }
+  if (cls >= 0) mine += (int)(before >> (10 * cls)) & 1023;
+#pragma unroll
+  for (int c = 1; c < 6; ++c) mine += c > cls ? (int)(all >> (10 * c)) & 1023 : 0;
+  if (cls >= 0 && mine == q - base) sm.row = row;
+  __syncthreads();
+  return sm.row;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
-    sample_kernel(const SampleParams p, const int ranks, const int per, const int room) {
+    sample_kernel(const SampleParams p, const int ranks, const int per, const int room,
+                  const bool order) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& sm = *reinterpret_cast<Shared*>(smem_raw);
   float* held = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = blockIdx.x % ranks, row = blockIdx.x / ranks;
+  const int rank = blockIdx.x % ranks;
+  if (tid < 64) sm.pow2[tid] = exp2(tid / 64.0 + p.wshift);
+  pdl_wait();
+  const int row = order ? ordered_row(p, sm, blockIdx.x / ranks) : blockIdx.x / ranks;
   const int lo = min(rank * per, p.vocab);
   const T* x = static_cast<const T*>(p.logits) + (long long)row * p.logits_stride + lo;
   const int skip = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
   const int n = lo < p.vocab ? min(per, p.vocab - lo) + skip : 0;
   static_assert(sizeof(Shared) % 16 == 0, "the slice is read 16 bytes at a time");
   const int n_held = min((n + 7) & ~7, room);
-  if (tid < 64) sm.pow2[tid] = exp2(tid / 64.0 + p.wshift);
-  pdl_wait();
 
   float best;
   int at;
@@ -881,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 template <typename T>
 cudaError_t launch_one(const SampleParams& p, int ranks, int per, int room, size_t smem,
-                       cudaStream_t st, bool pdl) {
+                       bool order, cudaStream_t st, bool pdl) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.n_rows * ranks));
   cfg.blockDim = dim3(kThreads);
@@ -896,7 +965,7 @@ cudaError_t launch_one(const SampleParams& p, int ranks, int per, int room, size
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p, ranks, per, room);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p, ranks, per, room, order);
 }
 
 constexpr int kMaxSmem = 227 * 1024;
@@ -927,10 +996,17 @@ cudaError_t launch_sample(const SampleParams& p, int dtype, int n_sm, cudaStream
   const int per = ((p.vocab + ranks - 1) / ranks + 7) & ~7;
   // (a slice that starts off a 16-byte boundary is held from that boundary on)
   const int room = std::min(per + 8, (kMaxSmem - (int)sizeof(Shared)) / 4 & ~7);
-  const size_t smem = sizeof(Shared) + (size_t)room * 4;
-  if (dtype == kDtypeF32) return launch_one<float>(p, ranks, per, room, smem, st, pdl);
-  if (dtype == kDtypeBf16) return launch_one<__nv_bfloat16>(p, ranks, per, room, smem, st, pdl);
-  return launch_one<__half>(p, ranks, per, room, smem, st, pdl);
+  size_t smem = sizeof(Shared) + (size_t)room * 4;
+  // Few clusters would share SMs while others are idle: each CTA asks for more than half of one.
+  // (Not as soon as the CTAs outnumber half the SMs: a cluster lies within one of the device's
+  // parts, which then holds fewer of them.  16 rows took 25 us in place of 19.)
+  constexpr int kHalf = kMaxSmem / 2 - 1024;
+  const long long ctas = (long long)p.n_rows * ranks;
+  if (ctas <= n_sm / 2) smem = std::max<size_t>(smem, kMaxSmem / 2 + 1024);
+  const bool order = ctas > (long long)n_sm * (smem <= kHalf ? 2 : 1);
+  if (dtype == kDtypeF32) return launch_one<float>(p, ranks, per, room, smem, order, st, pdl);
+  if (dtype == kDtypeBf16) return launch_one<__nv_bfloat16>(p, ranks, per, room, smem, order, st, pdl);
+  return launch_one<__half>(p, ranks, per, room, smem, order, st, pdl);
 }
 
 }  // namespace gqa
