@@ -387,3 +387,158 @@ def test_refusals(pkg, cuda):
         ctx.paged_attention(r.kv, 2, 0, None, r.lens, 1, 30, r.qkv, out)
     with make_ctx(pkg, 64) as ctx, bad:
         ctx.paged_append(r.kv, 2, 2, None, r.lens, r.qkv)              # heads of another size
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_padded_pages(pkg, cuda, dtype, layout):
+    """Pages, heads and rows with gaps between them, which are not touched."""
+    b = Batch(dtype, 128, [40, 1, 2], [70, 90, 33], page=32, n_kv=2, layout=layout, seed=16)
+    ks, vs, tols = b.appended()
+    r = Run(pkg, b)
+    wide = []
+    for x in (r.kp, r.vp):
+        w = cuda.full((x.shape[0], x.shape[1] + 1, x.shape[2] + 3, 128 + 8), 7.0, dtype=b.td,
+                      device="cuda")
+        w[:, :x.shape[1], :x.shape[2], :128] = x
+        wide.append(w)
+    view = [w[:, :x.shape[1], :x.shape[2], :128] for w, x in zip(wide, (r.kp, r.vp))]
+    r.kv = pkg.paged_kv_of(*view, r.table, layout=layout)
+    with make_ctx(pkg, 128) as ctx:
+        r.append(ctx)
+        out = r.attend(ctx)
+        assert ctx.device_status() == 0
+    for w, v in zip(wide, view):
+        v_bits = v.clone()
+        v.fill_(7.0)
+        assert (w == 7).all()
+        v.copy_(v_bits)
+    kp, vp = (v.cpu() for v in view)
+    for s in range(3):
+        assert (np.abs(b.unpool(kp, s) - ks[s]) <= tols[s]).all()
+        np.testing.assert_array_equal(b.unpool(vp, s), vs[s])
+    b.set_appended()
+    check_attention(b, out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_more_sequences_than_threads(pkg, cuda, dtype):
+    """700 sequences, some of them empty or not advanced, single tokens and chunks."""
+    g = np.random.default_rng(17)
+    news = g.choice([0, 1, 1, 1, 2, 5], 700).tolist()
+    news[:3], news[-2:] = [0, 0, 1], [30, 0]
+    lens = [n + int(t) for n, t in zip(news, g.integers(0, 40, 700))]
+    b = Batch(dtype, 64, news, lens, page=16, n_kv=1, seed=18)
+    b.set_appended()
+    r = Run(pkg, b)
+    before = r.kp.clone()
+    with make_ctx(pkg, 64, 1) as ctx:
+        out = r.attend(ctx)
+        r.append(ctx)
+        assert ctx.device_status() == 0
+    check_attention(b, out)
+    kp = r.kp.cpu()
+    for s in range(0, 700, 13):
+        assert (np.abs(b.unpool(kp, s) - b.k[s]) <=
+                cuda.finfo(b.td).eps * np.abs(b.k[s]) + 1e-5).all()
+    assert int(r.kp.isnan().sum()) == int(before.isnan().sum())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d,n_kv", [(128, 2), (64, 8)])
+def test_long_beside_short(pkg, cuda, dtype, d, n_kv):
+    """Single tokens whose rows many CTAs share beside some that one CTA holds."""
+    b = Batch(dtype, d, [1] * 6, [9000, 20, 5000, 1, 700, 6001], page=64, n_kv=n_kv, seed=19)
+    b.set_appended()
+    r = Run(pkg, b)
+    with make_ctx(pkg, d, n_kv) as ctx:
+        out = r.attend(ctx)
+        assert ctx.device_status() == 0
+    check_attention(b, out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_output_rows_apart(pkg, cuda, dtype):
+    """Rows of the output 16 bytes off a sector's start; what lies between them stays."""
+    b = Batch(dtype, 128, [50, 1, 300], [50, 400, 330], page=16, seed=20)
+    b.set_appended()
+    r = Run(pkg, b)
+    pad = 16 // b.qkv.element_size()
+    wide = cuda.full((b.n_tokens, b.n_q * 128 + pad), 7.0, dtype=b.td, device="cuda")
+    with make_ctx(pkg, 128) as ctx:
+        r.attend(ctx, out=wide[:, :b.n_q * 128])
+        want = r.attend(ctx)
+        assert ctx.device_status() == 0
+    check_attention(b, wide)
+    assert (wide[:, b.n_q * 128:] == 7).all()
+    assert cuda.equal(wide[:, :b.n_q * 128], want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_offsets_past_32_bits(pkg, cuda, dtype):
+    """Pages that lie more than 2^31 elements into their pools."""
+    b = Batch(dtype, 128, [20, 1], [60, 100], page=16, seed=21)
+    ks, vs, tols = b.appended()
+    r = Run(pkg, b)
+    far = 2 ** 31 // (2 * 16 * 128)
+    pools = []
+    for x in (r.kp, r.vp):
+        w = cuda.empty(far + b.n_pages, 2, 16, 128, dtype=b.td, device="cuda")
+        w[far:] = x
+        pools.append(w)
+    table = r.table + far
+    r.kv = pkg.paged_kv_of(*pools, table)
+    with make_ctx(pkg, 128) as ctx:
+        r.append(ctx)
+        out = r.attend(ctx)
+        # entry -7 of Batch became a page of the pool; no row of the sequences is in it
+        assert ctx.device_status() == 0
+    kp, vp = (w[far:].cpu() for w in pools)
+    for s in range(2):
+        assert (np.abs(b.unpool(kp, s) - ks[s]) <= tols[s]).all()
+        np.testing.assert_array_equal(b.unpool(vp, s), vs[s])
+    b.set_appended()
+    check_attention(b, out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_overlapped_launches(pkg, cuda, dtype):
+    """GQA_OPT_PDL off and on: a chain of calls, each of which needs the one before it."""
+    b = Batch(dtype, 128, [40, 1, 1], [90, 500, 40], page=16, seed=22)
+    outs = []
+    for pdl in (0, 1):
+        r = Run(pkg, b)
+        with make_ctx(pkg, 128) as ctx:
+            ctx.set_option(pkg.gqa.GQA_OPT_PDL, pdl)
+            for _ in range(20):
+                # the output is the next call's qkv (q | the same k and v)
+                r.append(ctx)
+                r.attend(ctx, out=r.qkv)
+            tok = cuda.empty(b.n_tokens, dtype=cuda.int32, device="cuda")
+            u = cuda.full((b.n_tokens,), 0.5, device="cuda")
+            ctx.sample(b.n_tokens, b.n_q * 128, r.qkv, None, None, None, None, u, tok)
+            assert ctx.device_status() == 0
+        outs.append((r.kp, r.vp, r.qkv, tok))
+    for x, y in zip(*outs):
+        assert cuda.equal(cuda.nan_to_num(x.float(), 9.0), cuda.nan_to_num(y.float(), 9.0))
+
+
+def test_two_contexts_at_once(pkg, cuda):
+    """Two contexts on two streams do not share a workspace."""
+    bs = [Batch("bf16", 128, [60, 1, 1], [800, 3000, 40], page=16, seed=23 + i) for i in (0, 1)]
+    runs = []
+    for b in bs:
+        b.set_appended()
+        runs.append(Run(pkg, b))
+    streams = [cuda.cuda.Stream() for _ in bs]
+    ctxs = [make_ctx(pkg, 128) for _ in bs]
+    outs = [cuda.zeros(b.n_tokens, b.n_q * 128, dtype=b.td, device="cuda") for b in bs]
+    cuda.cuda.synchronize()
+    for _ in range(20):
+        for r, st, ctx, out in zip(runs, streams, ctxs, outs):
+            r.attend(ctx, out=out, stream=st)
+    cuda.cuda.synchronize()
+    for b, ctx, out in zip(bs, ctxs, outs):
+        assert ctx.device_status() == 0
+        check_attention(b, out)
+        ctx.close()

@@ -253,3 +253,15 @@ def test_refusals(pkg, cuda):
             ctx.sample(4, 100, x.data_ptr() + 2, *none, u, tok, logits_stride=100,
                        dtype=pkg.gqa.F32)
         ctx.sample(0, 100, x, *none, u, tok)                           # nothing to do
+
+
+@pytest.mark.parametrize("rows,vocab", [(1100, 501), (513, 30000)])
+def test_rows_that_take_turns(pkg, cuda, rows, vocab):
+    """More rows than run at once, of every kind of settings: each is written once, by itself."""
+    g = np.random.default_rng(rows)
+    x = cuda.from_numpy(g.standard_normal((rows, vocab)) * 2).float()
+    st = settings(rows, vocab, 30)
+    st[1][1::7] = [vocab // 2] * len(st[1][1::7])
+    run(pkg, cuda, x, *st)
+    alike = [[1.0] * rows, [0] * rows, [1.0] * rows, [0.0] * rows, g.random(rows).tolist()]
+    run(pkg, cuda, x, *alike)
