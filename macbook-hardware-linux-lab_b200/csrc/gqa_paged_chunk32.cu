@@ -46,7 +46,9 @@ struct alignas(1024) Smem {
   uint8_t bad[4][4];  // per key tile: its 16-row parts without a page
   uint64_t item_full[4], item_empty[4];
   uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty;
-  uint64_t s_full[2], p_full, o_full, o_empty, drain;
+  // (P of the next tile can be ready before the MMA warp looks for this one's, which waits for V
+  // first: a barrier for each of the two places)
+  uint64_t s_full[2], p_full[2], o_full, o_empty, drain;
   long long scan[kThreads / 32];
   WalkStart start;
   Walk<tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
@@ -135,7 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&sm.q_full, kOperandWarps);
     mbar_init(&sm.k_full, kOperandWarps);
     mbar_init(&sm.v_full, kOperandWarps);
-    mbar_init(&sm.p_full, 4);
+    mbar_init(&sm.p_full[0], 4);
+    mbar_init(&sm.p_full[1], 4);
     mbar_init(&sm.o_empty, 4);
     mbar_init(&sm.q_empty, 1);
     mbar_init(&sm.k_empty, 1);
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (j > 0) {
             ok = all_wait(&sm.v_full, t & 1) && (t == 0 || all_wait(&sm.o_empty, (t - 1) & 1)) &&
-                 all_wait(&sm.p_full, t & 1);
+                 all_wait(&sm.p_full[t & 1], (t >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
             issue_pv(t);
@@ -495,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l = l * alpha + (sum0 + sum1);
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.p_full);
+          if (lane == 0) mbar_arrive(&sm.p_full[t & 1]);
           ++t;
         }
         if (j > 0) {

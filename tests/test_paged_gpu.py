@@ -542,3 +542,24 @@ def test_two_contexts_at_once(pkg, cuda):
         assert ctx.device_status() == 0
         check_attention(b, out)
         ctx.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [128, 64])
+def test_units_of_one_and_two_tiles(pkg, cuda, dtype, d):
+    """Chunks that end in one tile or in two, in a mixed order, many of them per CTA; every run
+    gives the same bits."""
+    g = np.random.default_rng(24)
+    tok = 128 // {128: 6, 64: 7}[d]
+    news = g.choice([2, 5, tok, tok + 1, 2 * tok - 1, 2 * tok, 2 * tok + 1, 3 * tok, 4 * tok + 1],
+                    120).tolist()
+    lens = [n + int(t) for n, t in zip(news, g.choice([0, 0, 3, 90, 128, 300, 700], 120))]
+    b = Batch(dtype, d, news, lens, page=64, n_kv=4, seed=25)
+    b.set_appended()
+    r = Run(pkg, b)
+    with make_ctx(pkg, d, 4) as ctx:
+        out = r.attend(ctx)
+        for _ in range(10):
+            assert cuda.equal(r.attend(ctx), out)
+        assert ctx.device_status() == 0
+    check_attention(b, out)
