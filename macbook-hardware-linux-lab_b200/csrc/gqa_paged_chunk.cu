@@ -25,10 +25,14 @@
 //
 // Warps 0-7 / 8-15: softmax of tile A / B, two threads per row (64 keys each: with one thread a
 // row, two warps a scheduler waited for their own instructions, 1800 clocks a tile against 1024
-// of the exponential unit); 16: loader (TMA of the pages); 17: MMA.  Tensor memory: S_A | S_B |
-// O_A | O_B, the P of each half of the keys over the first half of its scores.  (One MMA warp
-// per tile measured slower, 64 against 58 us for 512 tokens over 8192 rows: the products of the
-// two interleave and both finish late.)
+// of the exponential unit); 16: loader of K and V (TMA of the pages); 17: MMA; 18: loader of Q.
+// Tensor memory: two buffers of scores (three at head_dim 64) and O_A | O_B; the P of each half of
+// the keys goes over the first half of its scores.  With three buffers a tile's next scores are
+// ready when its softmax is done with these, and the stream of products runs on from one unit to
+// the next (four whole prompts of 1500 to 2500 tokens, f16: 96 -> 88 us; with two buffers, at
+// head_dim 128, a tile's scores, softmax and product follow one another, some 4000 clocks for the
+// two tiles where the tensor cores need 2048).  (One MMA warp per tile measured slower, 64 against
+// 58 us for 512 tokens over 8192 rows: the products of the two interleave and both finish late.)
 // Every wait is bounded; a wait that runs out sets the status bit, and the CTA drains
 // what it issued and returns its tensor memory.
 #include <cuda.h>
@@ -42,24 +46,36 @@ namespace gqa {
 namespace {
 
 constexpr int kKeys = 128;
-constexpr int kSoftmaxWarps = 16, kLoader = 16, kMma = 17;
-constexpr int kThreads = 18 * 32;
+constexpr int kSoftmaxWarps = 16, kLoader = 16, kMma = 17, kQLoader = 18;
+constexpr int kThreads = 19 * 32;
 constexpr int kRowsTile = kChunkRows;
+// Buffers of scores: what tensor memory holds beside the two outputs.
+template <int D>
+constexpr int kScores = D == 64 ? 3 : 2;
+// Stages of K and of V, and units of which Q is held: what shared memory has room for.
+template <int D>
+constexpr int kStages = D == 64 ? 4 : 2;
+template <int D>
+constexpr int kUnitsQ = D == 64 ? 2 : 1;
 
 template <int D, int G>
 struct alignas(1024) Smem {
-  uint16_t q[2][kRowsTile * D];
-  uint16_t k[2][kKeys * D];
-  uint16_t v[2][kKeys * D];
+  uint16_t q[2 * kUnitsQ<D>][kRowsTile * D];  // [unit][tile A, B]
+  uint16_t k[kStages<D>][kKeys * D];
+  uint16_t v[kStages<D>][kKeys * D];
   float xch[2][2][2][kRowsTile];  // [turn][tile A, B][half of the keys][row]: maxima, sums
   Piece ring[4];
   int poison[4];         // number of the last piece of this ring place with a non-finite V
-  // per key tile: its 16-row parts without a page (four tiles: the softmax of a tile may
-  // still be due when the second tile after it is loaded)
-  unsigned bad_rows[4];
+  // per key tile: its 16-row parts without a page (the softmax of a tile may still be due when
+  // one of the second turn of stages after it is loaded)
+  unsigned bad_rows[2 * kStages<D>];
   uint64_t item_full[4], item_empty[4];
-  uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_final[2], drain;
+  uint64_t q_full[2 * kUnitsQ<D>], q_empty[2 * kUnitsQ<D>];
+  uint64_t k_full[kStages<D>], k_empty[kStages<D>], v_full[kStages<D>], v_empty[kStages<D>];
+  // [tile][its even, odd steps]: a tile's next scores can be ready before it has looked at these
+  // (never those after the next)
+  uint64_t s_full[4], o_done[4], o_final[2];
+  uint64_t p_full[kScores<D>], drain;  // [buffer of scores]
   long long scan[kThreads / 32];
   WalkStart start;
   Walk<2 * tile_tokens<G>(), kKeys> walk;  // (one thread's; no registers for it)
@@ -118,9 +134,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Whether key tile kt holds rows past the piece's first token, which not all its rows see.
-__device__ __forceinline__ bool clears_v(const Piece& pc, int kt) {
-  return (kt + 1) * kKeys > pc.pos + 1;
+// Whether key tile kt holds rows past the piece's first token (at pos), which not all its rows see.
+__device__ __forceinline__ bool clears_v(int pos, int kt) {
+  return (kt + 1) * kKeys > pos + 1;
 }
 
 // Scores whose bit is set become -inf.
@@ -184,6 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 ~static_cast<uintptr_t>(1023));
   constexpr int kTok = tile_tokens<G>();
   constexpr int kBlocks = D / 64;               // 64-column blocks of a row
+  constexpr bool kPrefetch = kScores<D> > 2;   // of a tile's next scores before its P is ready
+  constexpr int kS = kScores<D>, kSt = kStages<D>, kQ = kUnitsQ<D>;
   constexpr uint32_t kTileBytes = kKeys * D * 2;
   constexpr uint32_t kQBytes = kTok * G * D * 2;
   constexpr uint32_t kIdS = idesc<T>(128, false), kIdO = idesc<T>(D, true);
@@ -193,20 +211,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < 4; ++s) {
       mbar_init(&sm.item_full[s], 1);
-      mbar_init(&sm.item_empty[s], 1 + kSoftmaxWarps);  // the MMA and the softmax warps
+      mbar_init(&sm.item_empty[s], 2 + kSoftmaxWarps);  // Q's loader, MMA and softmax warps
+      mbar_init(&sm.s_full[s], 1);
+      mbar_init(&sm.o_done[s], 1);
       sm.poison[s] = -1;
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 2; ++s) mbar_init(&sm.o_final[s], 1);
+    for (int s = 0; s < 2 * kQ; ++s) {
       mbar_init(&sm.q_full[s], 1);
       mbar_init(&sm.q_empty[s], 1);
+    }
+    for (int s = 0; s < kSt; ++s) {
       mbar_init(&sm.k_full[s], 1);
       mbar_init(&sm.k_empty[s], 1);
       mbar_init(&sm.v_full[s], 1);
       mbar_init(&sm.v_empty[s], 1);
-      mbar_init(&sm.s_full[s], 1);
-      mbar_init(&sm.p_full[s], kSoftmaxWarps / 2);
-      mbar_init(&sm.o_final[s], 1);
     }
+    for (int s = 0; s < kS; ++s) mbar_init(&sm.p_full[s], kSoftmaxWarps / 2);
     mbar_init(&sm.drain, 1);
     sm.err = 0;
     fence_barrier_init();
@@ -217,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // the two rows of a Q tile that no copy fills
-  for (int i = tid; i < 2 * kBlocks * (kRowsTile - kTok * G) * 64; i += kThreads) {
+  for (int i = tid; i < 2 * kQ * kBlocks * (kRowsTile - kTok * G) * 64; i += kThreads) {
     const int x = i % 64, r = i / 64 % (kRowsTile - kTok * G), b = i / 64 / (kRowsTile - kTok * G);
     sm.q[b / kBlocks][(b % kBlocks) * kRowsTile * 64 + (kTok * G + r) * 64 + x] = 0;
   }
@@ -236,9 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kLoader) {
     // ---- loader ----
-    bool waited = false;  // for q
     Piece pc{};
-    int kv = 0, rd = 0, nq[2] = {0, 0};
+    int kv = 0, rd = 0;
     bool ok = true;
     const CUtensorMap *km = &maps.k, *vm = &maps.v;
     for (;; ++rd) {
@@ -257,30 +277,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!more) break;
       const int seq = __shfl_sync(0xffffffffu, pc.seq, 0);
       const int head = __shfl_sync(0xffffffffu, pc.head, 0);
-      const int tok = __shfl_sync(0xffffffffu, pc.tok, 0);
-      const int n_tok = __shfl_sync(0xffffffffu, pc.n_tok, 0);
       const int len = __shfl_sync(0xffffffffu, pc.len, 0);
       const int kt0 = __shfl_sync(0xffffffffu, pc.kt0, 0);
       const int kt1 = __shfl_sync(0xffffffffu, pc.kt1, 0);
-      if (!waited) pdl_wait();
-      waited = true;
-      for (int g = 0; g < (n_tok > kTok ? 2 : 1) && ok; ++g, __syncwarp()) {
-        if (nq[g] > 0) ok = wait_or_abort(&sm.q_empty[g], (nq[g] - 1) & 1, err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&sm.q_full[g], kQBytes);
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b)
-            tma_load3(sm.q[g] + b * kRowsTile * 64, &maps.q, b * 64, head * G, tok + g * kTok,
-                      &sm.q_full[g]);
-        }
-        ++nq[g];
-      }
-      if (!ok) break;
       const int boxes = kKeys / box_rows;
       for (int kt = kt0; kt < kt1; ++kt, ++kv) {
-        const int st = kv & 1;
+        const int st = kv % kSt;
         // the pages of the tile: one per lane
         int row = kt * kKeys + lane * box_rows, page = p.kv.n_pages;  // (no such page: zeros)
         bool bad = false;
@@ -295,15 +297,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const unsigned bad_boxes = __ballot_sync(0xffffffffu, bad);
         row &= (1 << p.kv.page_shift) - 1;
         const int c1 = hnd ? row : head, c2 = hnd ? head : row;
-        const uint32_t reuse = ((kv >> 1) - 1) & 1;
-        if (kv >= 2) ok = wait_or_abort(&sm.k_empty[st], reuse, err);
+        const uint32_t reuse = (kv / kSt - 1) & 1;
+        if (kv >= kSt) ok = wait_or_abort(&sm.k_empty[st], reuse, err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
           unsigned rows16 = 0;  // 16-row parts without a page
           for (int i = 0; i < 8; ++i)
             if (bad_boxes >> (i * 16 / box_rows) & 1) rows16 |= 1u << i;
-          sm.bad_rows[kv & 3] = rows16;
+          sm.bad_rows[kv % (2 * kSt)] = rows16;
           mbar_arrive_expect_tx(&sm.k_full[st], kTileBytes);
         }
         __syncwarp();
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load4(sm.k[st] + b * kKeys * 64 + lane * box_rows * 64, km, b * 64, c1, c2, page,
                       &sm.k_full[st]);
         __syncwarp();
-        if (kv >= 2) ok = wait_or_abort(&sm.v_empty[st], reuse, err);
+        if (kv >= kSt) ok = wait_or_abort(&sm.v_empty[st], reuse, err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sm.v_full[st], kTileBytes);
@@ -327,19 +329,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
     }
-    if (!waited) pdl_wait();  // (the grid must not end before the one whose q it stands for)
     if (*err && lane == 0) {
       // Let the copies already issued land before the CTA's shared memory is handed on
       // (a phase that was never armed runs into the wait's bound).
-      for (int s = 0; s < 2; ++s) {
-        if (nq[s] > 0) mbar_wait_bounded(&sm.q_full[s], (nq[s] - 1) & 1, kWaitBudget);
-        for (int i = max(0, kv - 1); i <= kv; ++i)
-          if ((i & 1) == s) {
-            mbar_wait_bounded(&sm.k_full[s], (i >> 1) & 1, kWaitBudget / 16);
-            mbar_wait_bounded(&sm.v_full[s], (i >> 1) & 1, kWaitBudget / 16);
-          }
+      for (int i = max(0, kv - kSt + 1); i <= kv; ++i) {
+        mbar_wait_bounded(&sm.k_full[i % kSt], (i / kSt) & 1, kWaitBudget / 16);
+        mbar_wait_bounded(&sm.v_full[i % kSt], (i / kSt) & 1, kWaitBudget / 16);
       }
     }
+    __syncwarp();
+  } else if (warp == kQLoader) {
+    // ---- loader of Q (its own warp, so that K and V of the next unit need not wait for it) ----
+    int nq[2] = {0, 0};
+    bool waited = false, ok = true;
+    for (int rd = 0; ok; ++rd) {
+      ok = __all_sync(0xffffffffu, wait_or_abort(&sm.item_full[rd & 3], (rd >> 2) & 1, err));
+      if (!ok) break;
+      const int n_tok = sm.ring[rd & 3].n_tok, head = sm.ring[rd & 3].head;
+      const int tok = sm.ring[rd & 3].tok;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[rd & 3]);
+      if (n_tok == 0) break;
+      if (!waited) pdl_wait();
+      waited = true;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (!ok || (g == 1 && n_tok <= kTok)) break;
+        const int at = nq[g] % kQ * 2 + g;
+        if (nq[g] >= kQ) ok = wait_or_abort(&sm.q_empty[at], (nq[g] / kQ - 1) & 1, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sm.q_full[at], kQBytes);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b)
+            tma_load3(sm.q[at] + b * kRowsTile * 64, &maps.q, b * 64, head * G, tok + g * kTok,
+                      &sm.q_full[at]);
+        }
+        __syncwarp();
+        ++nq[g];
+      }
+    }
+    if (!waited) pdl_wait();  // (the grid must not end before the one whose q it stands for)
+    if (*err && lane == 0)    // (as above)
+      for (int g = 0; g < 2; ++g)
+        for (int i = max(0, nq[g] - kQ); i < nq[g]; ++i)
+          mbar_wait_bounded(&sm.q_full[i % kQ * 2 + g], (i / kQ) & 1, kWaitBudget / 16);
     __syncwarp();
   } else if (warp == kMma) {
     // ---- MMA issuer (the whole warp, one lane issues) ----
@@ -351,13 +386,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
-    const auto take = [&](int n, Piece& pc) {
-      if (!all_wait(&sm.item_full[n & 3], (n >> 2) & 1)) return false;
-      pc = sm.ring[n & 3];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.item_empty[n & 3]);
-      return true;
-    };
     // Descriptors differ in their low words alone.
     const uint32_t q_low = (uint32_t)desc_k_major(smem_addr(sm.q[0]));
     const uint32_t k_low = (uint32_t)desc_k_major(smem_addr(sm.k[0]));
@@ -368,56 +396,98 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
       return d;
     };
-    Piece pc{};
-    int rd = 0, kv = 0;              // pieces; key tiles whose P V is issued
-    uint32_t q_turn = 0, p_turn = 0; // parities of Q and P, a bit for each of A and B
-    bool ok = take(0, pc);
-    while (ok && pc.n_tok > 0) {
-      const int tiles = pc.kt1 - pc.kt0, both = pc.n_tok > kTok;
-      // Turn j: P V of tile j - 1 and S of tile j, of A, then of B.  Written once and looped
-      // over, as the loops of all roles have to fit the instruction cache together.
-      for (int j = 0; j <= tiles && ok; ++j) {
-        // What the loader brings is waited for first, while the softmax is still at work: the
-        // products then follow the weights at once.
-        const int kn = kv + (j > 0);
-        ok = (j == 0 || all_wait(&sm.v_full[kv & 1], (kv >> 1) & 1)) &&
-             (j == tiles || all_wait(&sm.k_full[kn & 1], (kn >> 1) & 1));
-#pragma unroll 1
-        for (int g = 0; g <= both && ok; ++g) {
-          uint32_t& turn = j == 0 ? q_turn : p_turn;
-          ok = all_wait(j == 0 ? &sm.q_full[g] : &sm.p_full[g], turn >> g & 1);
-          if (!ok) break;
-          turn ^= 1u << g;
-          tc_fence_after();
-          if (elect_one()) {
-            if (j > 0) {
-              const uint32_t v = v_low + (kv & 1) * (kKeys * D * 2 / 16);
-              const uint32_t at = tmem + 128 * g;
-#pragma unroll
-              for (int ks = 0; ks < kKeys / 16; ++ks)
-                umma_ts(tmem + 256 + 128 * g, at + (ks & 3) * 8 + (ks >> 2) * 64,
-                        desc(v + ks * 2048 / 16), kIdO, j > 1 || ks > 0);
-            }
-            if (j < tiles) {
-              const uint32_t q = q_low + g * (kRowsTile * D * 2 / 16);
-              const uint32_t k = k_low + (kn & 1) * (kKeys * D * 2 / 16);
-#pragma unroll
-              for (int ks = 0; ks < D / 16; ++ks) {
-                const uint32_t off = ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32) / 16;
-                umma_ss(tmem + 128 * g, desc(q + off), desc(k + off), kIdS, ks > 0);
-              }
-              umma_commit(&sm.s_full[g]);
-            }
-            if (j == tiles) umma_commit(&sm.o_final[g]);
-            if (j + 1 == tiles) umma_commit(&sm.q_empty[g]);
-          }
-          __syncwarp();
-        }
-        if (ok && j > 0) commit(&sm.v_empty[kv & 1]);
-        if (ok && j < tiles) commit(&sm.k_empty[kn & 1]);
-        kv += j > 0;
+    // Steps are (key tile, A), (key tile, B), the next key tile's and so on, or those of A alone,
+    // of one piece after the other.  A turn issues P V of the step kS before it, then S of its
+    // own, into the buffer of scores that is free by then.  (One call site for each product: the
+    // loops of all roles have to fit the instruction cache together.)
+    int s_rd = 0, s_both = 0, s_steps = 0, s_at = 0, s_kv = 0;  // scores: pieces, the open one's
+    int p_rd = 0, p_both = 0, p_steps = 0, p_at = 0, p_kv = 0;  // steps, key tiles before it
+    int s_buf = 0, p_buf = 0, pending_a = 0, pending_b = 0, nq0 = 0, nq1 = 0;
+    uint32_t p_turn = 0;              // parity of P
+    uint32_t s_turn = 0, o_turn = 0;  // which of a tile's two barriers is next, a bit for each tile
+    bool ok = true, more = true;
+    for (;;) {
+      if (more && s_at == s_steps) {
+        s_kv += s_steps >> s_both;
+        s_at = 0;
+        ok = all_wait(&sm.item_full[s_rd & 3], (s_rd >> 2) & 1);
+        if (!ok) break;
+        const Piece& pc = sm.ring[s_rd & 3];
+        more = pc.n_tok > 0;
+        s_both = pc.n_tok > kTok;
+        s_steps = (pc.kt1 - pc.kt0) << s_both;
+        ++s_rd;
+        ++nq0;
+        nq1 += s_both;
       }
-      if (ok) ok = take(++rd, pc);
+      // Scores wait for a buffer, and for the product of their tile's last scores (of those before
+      // them where scores are prefetched): the barriers of a tile tell two steps apart.
+      const bool full = pending_a + pending_b == kS ||
+                        (s_at & s_both ? pending_b : pending_a) == (kPrefetch ? 2 : 1);
+      if (full || !more) {
+        if (pending_a + pending_b == 0) break;
+        if (p_at == p_steps) {
+          const Piece& pc = sm.ring[p_rd & 3];
+          p_kv += p_steps >> p_both;
+          p_at = 0;
+          p_both = pc.n_tok > kTok;
+          p_steps = (pc.kt1 - pc.kt0) << p_both;
+        }
+        const int g = p_at & p_both, v_at = p_kv + (p_at >> p_both);
+        // (what the loader brings first, while the softmax is still at work)
+        if (g == 0) ok = all_wait(&sm.v_full[v_at % kSt], (v_at / kSt) & 1);
+        if (ok) ok = all_wait(&sm.p_full[p_buf], p_turn);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t v = v_low + (v_at % kSt) * (kKeys * D * 2 / 16);
+          const uint32_t at = tmem + 128 * p_buf;
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            umma_ts(tmem + 128 * kS + D * g, at + (i & 3) * 8 + (i >> 2) * 64,
+                    desc(v + i * 2048 / 16), kIdO, p_at > p_both || i > 0);
+          if (kPrefetch) umma_commit(&sm.o_done[2 * g + (o_turn >> g & 1)]);
+          if (p_at + p_both + 1 >= p_steps) umma_commit(&sm.o_final[g]);
+          if (g == p_both) umma_commit(&sm.v_empty[v_at % kSt]);
+        }
+        __syncwarp();
+        o_turn ^= 1u << g;
+        if (++p_buf == kS) {
+          p_buf = 0;
+          p_turn ^= 1;
+        }
+        --(g ? pending_b : pending_a);
+        if (++p_at == p_steps) {
+          if (lane == 0) mbar_arrive(&sm.item_empty[p_rd & 3]);
+          ++p_rd;
+        }
+      }
+      // (one product in a turn may not be enough, where a piece of one tile follows one of two)
+      if (more && (s_at & s_both ? pending_b : pending_a) < (kPrefetch ? 2 : 1)) {
+        const int g = s_at & s_both, k_at = s_kv + (s_at >> s_both);
+        const int nq = (g ? nq1 : nq0) - 1, q_at = nq % kQ * 2 + g;
+        if (g == 0) ok = all_wait(&sm.k_full[k_at % kSt], (k_at / kSt) & 1);
+        if (ok && s_at <= s_both) ok = all_wait(&sm.q_full[q_at], (nq / kQ) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t q = q_low + q_at * (kRowsTile * D * 2 / 16);
+          const uint32_t k = k_low + (k_at % kSt) * (kKeys * D * 2 / 16);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const uint32_t off = ((i >> 2) * (kKeys * 128) + (i & 3) * 32) / 16;
+            umma_ss(tmem + 128 * s_buf, desc(q + off), desc(k + off), kIdS, i > 0);
+          }
+          umma_commit(&sm.s_full[2 * g + (s_turn >> g & 1)]);
+          if (g == s_both) umma_commit(&sm.k_empty[k_at % kSt]);
+          if (s_at + s_both + 1 >= s_steps) umma_commit(&sm.q_empty[q_at]);
+        }
+        __syncwarp();
+        s_turn ^= 1u << g;
+        if (++s_buf == kS) s_buf = 0;
+        ++s_at;
+        ++(g ? pending_b : pending_a);
+      }
     }
     commit(&sm.drain);  // no MMA may be running when tensor memory is freed
     mbar_wait_bounded(&sm.drain, 0, kWaitBudget);
@@ -426,8 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- softmax of tile g: row r (token r / G, head r % G), keys 64 half .. 64 half + 63 ----
     const int g = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_off + 128 * g + 64 * half;
-    const uint32_t t_o = tmem + lane_off + 256 + 128 * g + D / 2 * half;  // its half of O
+    const uint32_t t_o = tmem + lane_off + 128 * kS + D * g + D / 2 * half;  // its half of O
     const float sc = p.scale_log2;
     // The two warps of 32 rows exchange a value per row; the places alternate, so that one
     // meeting a turn is enough.  A warp that gives up arrives once more on its way out: its
@@ -443,31 +512,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (whole 32-byte sectors: with 16-byte stores a row per thread writes each twice)
     const bool wide_out =
         (reinterpret_cast<uintptr_t>(p.out) | (uint64_t)p.out_stride * sizeof(T)) % 32 == 0;
-    int tc = 0;  // S tiles of this tile's so far
-    int kv = 0;  // key tiles so far
-    int done = 0;
+    unsigned step = 0;  // of the MMA's steps, the first of the piece
+    unsigned kv = 0;    // key tiles so far
+    unsigned turns = 0;  // twice this tile's steps so far, and the parity of its pieces
     bool ok = true;
     for (int rd = 0; ok; ++rd) {
       ok = wait_lean(&sm.item_full[rd & 3], (rd >> 2) & 1, &sm.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const Piece pc = sm.ring[rd & 3];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.item_empty[rd & 3]);
-      if (pc.n_tok == 0) break;
-      if (g == 1 && pc.n_tok <= kTok) {  // nothing in tile B
-        kv += pc.kt1 - pc.kt0;
+      const Piece& pc = sm.ring[rd & 3];  // (given back behind the piece; few registers for it)
+      const int n_tok = pc.n_tok, pos = pc.pos, kt0 = pc.kt0, kt1 = pc.kt1;
+      if (n_tok == 0) break;
+      const int both = n_tok > kTok;
+      unsigned at = step + g;
+      step += (unsigned)(kt1 - kt0) << both;
+      if (g > both) {  // nothing in tile B
+        kv += kt1 - kt0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[rd & 3]);
         continue;
       }
-      const int limit = pc.pos + min(g * kTok + r / G, pc.n_tok - 1);  // last key of this row
-      const int first_limit = pc.pos + g * kTok;                       // of the tile's first row
+      const int limit = pos + min(g * kTok + r / G, n_tok - 1);  // last key of this row
+      const int first_limit = pos + g * kTok;                       // of the tile's first row
       float m = -CUDART_INF_F, l = 0.f;
-      for (int kt = pc.kt0; kt < pc.kt1; ++kt, ++tc, ++kv) {
-        ok = __all_sync(0xffffffffu, wait_lean(&sm.s_full[g], tc & 1, &sm.err));
+      for (int kt = kt0; kt < kt1; ++kt, ++kv) {
+        ok = __all_sync(0xffffffffu, wait_lean(&sm.s_full[2 * g + (turns >> 1 & 1)], turns >> 2 & 1,
+                                                &sm.err));
         if (!ok) break;
         tc_fence_after();
+        const uint32_t t_s = tmem + lane_off + 128 * (at % kS) + 64 * half;
         const int key0 = kt * kKeys;
-        const unsigned bad = sm.bad_rows[kv & 3];
+        const unsigned bad = sm.bad_rows[kv % (2 * kSt)];
         // Keys of this half that the row does not see: those past its own position, and rows
         // without a page.
         const bool edge = key0 + kKeys - 1 > first_limit || bad;
@@ -521,7 +596,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st16(t_s + 16, pk1);
         tmem_wait_st();
         l = l * alpha + (sum0 + sum1);
-        if (kt != pc.kt0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (kt != kt0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // (the scores may be ahead of the product that still adds to O)
+          if (kPrefetch)
+            ok = __all_sync(0xffffffffu, wait_lean(&sm.o_done[2 * g + ((turns >> 1) + 1 & 1)],
+                                                   (turns >> 1) - 1 >> 1 & 1, &sm.err));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
             float v[32];
@@ -535,12 +616,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // unit's last token are cleared; in those of its own tokens, which only some of its
         // rows see, what is not finite is cleared here and added to the rows that do see it
         // at the end.
-        if (g == 0 && clears_v(pc, kt)) {
-          ok = __all_sync(0xffffffffu, wait_lean(&sm.v_full[kv & 1], (kv >> 1) & 1, &sm.err));
+        if (g == 0 && clears_v(pos, kt)) {
+          ok = __all_sync(0xffffffffu, wait_lean(&sm.v_full[kv % kSt], (kv / kSt) & 1, &sm.err));
           if (!ok) break;
-          const int own0 = max(pc.pos + 1 - key0, 0);
-          const int end = pc.pos + pc.n_tok - key0;
-          uint4* v = reinterpret_cast<uint4*>(sm.v[kv & 1]);
+          const int own0 = max(pos + 1 - key0, 0);
+          const int end = pos + n_tok - key0;
+          uint4* v = reinterpret_cast<uint4*>(sm.v[kv % kSt]);
           // (chunks of the rows from own0 on)
           const int rows = kKeys - own0;
           for (int i = half * 128 + r; i < kBlocks * 8 * rows; i += 256) {
@@ -564,11 +645,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[g]);
+        if (lane == 0) mbar_arrive(&sm.p_full[at % kS]);
+        turns += 2;
+        at += 1 + both;
       }
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, wait_lean(&sm.o_final[g], done & 1, &sm.err));
-      ++done;
+      ok = __all_sync(0xffffffffu, wait_lean(&sm.o_final[g], turns & 1, &sm.err));
+      turns ^= 1;
       if (!ok) break;
       tc_fence_after();
       l += other(l);
@@ -578,9 +661,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool whole = pc.slot < 0, mine = r < kTok * G && t < pc.n_tok;
       T* dst = static_cast<T*>(p.out) + (long long)(pc.tok + t) * p.out_stride +
                (long long)(pc.head * G + r % G) * D + D / 2 * half;
-      const long long at = ((long long)pc.slot * 2 + g) * kRowsTile + r;
-      if (!whole && half == 0) part.chunk_ml[at] = make_float2(m, l);
-      float* part_dst = part.chunk_o + at * D + D / 2 * half;
+      const long long part_at = ((long long)pc.slot * 2 + g) * kRowsTile + r;
+      if (!whole && half == 0) part.chunk_ml[part_at] = make_float2(m, l);
+      float* part_dst = part.chunk_o + part_at * D + D / 2 * half;
 #pragma unroll 1
       for (int c = 0; c < D / 2; c += 32) {
         float o[32];
@@ -621,6 +704,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[rd & 3]);
     }
     if (!ok) {
       atomicOr(&sm.err, 1);
