@@ -85,21 +85,26 @@ __device__ void rotate_q(const PagedAttnParams& p) {
     const int pos = len - n_new + tok - first;
     const int rem = (int)(item - (long long)tok * per_token);
     const int h = rem / kChunks, c = rem % kChunks;
-    float co[V::n], si[V::n];
-#pragma unroll
-    for (int e = 0; e < V::n; ++e) rope_cos_sin(pos, p.turns[c * V::n + e], co[e], si[e]);
     const T* src = static_cast<const T*>(p.qkv) + (long long)tok * p.qkv_stride +
                    (long long)h * G * D + c * V::n;
     T* dst = static_cast<T*>(p.out) + (long long)tok * p.out_stride + (long long)h * G * D +
              c * V::n;
+    // (all loads before the first store: out may be where q is, so no compiler reorders them)
+    V lo[G], hi[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const V a = *reinterpret_cast<const V*>(src + g * D);
-      const V b = *reinterpret_cast<const V*>(src + g * D + D / 2);
+      lo[g] = *reinterpret_cast<const V*>(src + g * D);
+      hi[g] = *reinterpret_cast<const V*>(src + g * D + D / 2);
+    }
+    float co[V::n], si[V::n];
+#pragma unroll
+    for (int e = 0; e < V::n; ++e) rope_cos_sin(pos, p.turns[c * V::n + e], co[e], si[e]);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
       V y0, y1;
 #pragma unroll
       for (int e = 0; e < V::n; ++e) {
-        const float x = Elem<T>::get(a.e[e]), y = Elem<T>::get(b.e[e]);
+        const float x = Elem<T>::get(lo[g].e[e]), y = Elem<T>::get(hi[g].e[e]);
         y0.e[e] = Elem<T>::put(x * co[e] - y * si[e]);
         y1.e[e] = Elem<T>::put(x * si[e] + y * co[e]);
       }
