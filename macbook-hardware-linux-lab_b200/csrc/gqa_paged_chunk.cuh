@@ -230,7 +230,7 @@ struct Walk {
       }
     }
     __syncthreads();
-    if (tid != walker) return;
+    if (warp != walker >> 5) return;  // (all lanes of the walker's warp find the same)
     tile = first;
     seq = start->seq;
     tok = start->tok;
@@ -243,11 +243,25 @@ struct Walk {
     }
     head = (int)Shares::divide(tile - at, start->per_head);
     at += head * start->per_head;
-    unit = 0;
-    tiles = unit_tiles<U, KEYS>(n_new, len, 0);
-    while (tile >= at + tiles) {
-      at += tiles;
-      tiles = unit_tiles<U, KEYS>(n_new, len, ++unit);
+    // the unit, 32 at a time
+    for (unit = 0;; unit += 32) {
+      const int mine = unit_tiles<U, KEYS>(n_new, len, unit + lane);
+      long long upto = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, tile < at + upto);
+      const int i = past ? __ffs(past) - 1 : 31;
+      const long long all = __shfl_sync(0xffffffffu, upto, i);
+      tiles = __shfl_sync(0xffffffffu, mine, i);
+      if (past) {
+        at += all - tiles;
+        unit += i;
+        break;
+      }
+      at += all;
     }
   }
 
