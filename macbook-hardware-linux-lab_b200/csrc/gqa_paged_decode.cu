@@ -374,17 +374,24 @@ struct WarpState<float, D, G> {
   }
 };
 
-// Sum over the block of one value a thread.
-__device__ __forceinline__ long long block_sum(long long x, long long (&part)[kWarps]) {
+// Inclusive sum over the block's threads of one value each, and the sum of all.
+__device__ __forceinline__ long long block_scan(long long x, long long (&part)[kWarps],
+                                                long long& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) part[warp] = x;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
-  __syncthreads();
-  long long sum = 0;
+  all = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += part[w];
-  return sum;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) x += all;
+    all += part[w];
+  }
+  return x;
 }
 
 template <typename T, int D, int G>
@@ -401,50 +408,34 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_launch_dependents();
   if (rotate) rotate_q<T, D, G>(p);
 
-  // Tiles of all pairs, and this CTA's share [first, last) of them.
-  long long mine = 0;
+  // Tiles of all pairs: a thread adds up a run of sequences, a scan over the block gives the
+  // thread that holds the first tile of this CTA's share [first, last).
+  const int run = (p.plan.n_seq + kThreads - 1) / kThreads;
+  const int s0 = min(tid * run, p.plan.n_seq), s1 = min(s0 + run, p.plan.n_seq);
   int bad = 0;
-  for (int s = tid; s < p.plan.n_seq; s += kThreads) {
+  const auto tiles_of = [&](int s) {
     int tok;
-    mine += (single_rows(p, s, tok, &bad) + kTile - 1) / kTile;
-  }
+    return (long long)((single_rows(p, s, tok, &bad) + kTile - 1) / kTile) * p.n_kv;
+  };
+  long long mine = 0;
+#pragma unroll 4
+  for (int s = s0; s < s1; ++s) mine += tiles_of(s);
   if (bad && blockIdx.x == 0) atomicOr(p.status, bad);
-  const long long total = block_sum(mine, sm.scan) * p.n_kv;
+  long long total;
+  long long before = block_scan(mine, sm.scan, total) - mine;
   const long long n = min((long long)gridDim.x, total);
-  if (tid == 0) part.jobs[blockIdx.x].n_parts = 0;
+  if (tid == 0) {
+    part.jobs[blockIdx.x].n_parts = 0;
+    sm.found_seq = p.plan.n_seq;
+  }
   if (blockIdx.x >= n) return;
   const long long first = blockIdx.x * total / n, last = (blockIdx.x + 1) * total / n;
-
-  // The sequence of the first tile.
-  long long before = 0;  // tiles of the sequences before the block's current 128
-  if (tid == 0) sm.found_seq = p.plan.n_seq;
-  for (int s0 = 0; s0 < p.plan.n_seq; s0 += kThreads) {
-    int tok;
-    const int s = s0 + tid;
-    const long long x =
-        s < p.plan.n_seq ? (long long)((single_rows(p, s, tok, &bad) + kTile - 1) / kTile) * p.n_kv
-                         : 0;
-    long long incl = x;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) sm.scan[warp] = incl;
-    __syncthreads();
-    long long sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) incl += before + sum;
-      sum += sm.scan[w];
-    }
-    if (incl - x <= first && first < incl) {
-      sm.found_seq = s;
-      sm.found_before = incl - x;
-    }
-    before += sum;
-    if (first < before) break;
+  __syncthreads();
+  if (before <= first && first < before + mine) {
+    int s = s0;
+    for (long long x; s < s1 - 1 && before + (x = tiles_of(s)) <= first; ++s) before += x;
+    sm.found_seq = s;
+    sm.found_before = before;
   }
   __syncthreads();
   int seq = sm.found_seq;
