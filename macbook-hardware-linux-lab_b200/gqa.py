@@ -254,6 +254,18 @@ def _stream(s) -> int | None:
     return s.cuda_stream
 
 
+_RAW_STREAM = []
+
+
+def _current_stream(device: int) -> int:
+    """torch's current stream on a device, without a Stream object where torch can do that (2 us)."""
+    if not _RAW_STREAM:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _RAW_STREAM.append(raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
+    return _RAW_STREAM[0](device)
+
+
 def kv_of(k_cache, v_cache) -> LayerKV:
     return LayerKV(_ptr(k_cache), _ptr(v_cache))
 
@@ -321,9 +333,20 @@ def _matrix(x, what: str, device: int, dtype: int, rows: int, width: int,
                            f"{width} are needed")
         if stride is None:
             stride = own[0] if n > 1 else w
-    elif x.dim() and x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} is not dense in its last dimension")
-    return x.data_ptr(), width if stride is None else stride
+        else:
+            _room(x, what, (rows - 1) * stride + width)
+        return x.data_ptr(), stride
+    if stride is None:
+        stride = width
+    if not x.is_contiguous() or x.numel() < (rows - 1) * stride + width:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} {tuple(x.shape)} is not {rows} rows of {width}")
+    return x.data_ptr(), stride
+
+
+def _room(x, what: str, need: int) -> None:
+    """Refuses a tensor whose storage does not hold `need` elements from its first one on."""
+    if (x.untyped_storage().nbytes() // x.element_size()) - x.storage_offset() < need:
+        raise GqaError(GQA_ERR_INVALID_ARG, f"{what} {tuple(x.shape)} does not hold {need} elements")
 
 
 def paged_kv_of(k_pages, v_pages, page_table, layout: str = "hnd") -> PagedKV:
@@ -801,8 +824,7 @@ class Context:
 
     def _stream_of(self, stream) -> int | None:
         if stream is None:  # torch's current stream on this context's device
-            import torch
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return _current_stream(self.device)
         return _stream(stream)
 
     def _paged_args(self, kv: PagedKV, n_seq, n_tokens, q_starts, seq_lens, qkv, qkv_stride):

@@ -563,3 +563,38 @@ def test_units_of_one_and_two_tiles(pkg, cuda, dtype, d):
             assert cuda.equal(r.attend(ctx), out)
         assert ctx.device_status() == 0
     check_attention(b, out)
+
+
+def test_tensors_too_small_for_their_stride(pkg, cuda):
+    """Rows that would lie past a tensor's end are refused; tensors of other shapes that hold them
+    are taken."""
+    b = Batch("f32", 128, [1, 1, 1], [20, 30, 40], page=16, seed=26)
+    b.set_appended()
+    r = Run(pkg, b)
+    out = cuda.zeros(3, 12 * 128, device="cuda")
+    logits = cuda.zeros(3, 100, device="cuda")
+    u = cuda.zeros(3, device="cuda")
+    tok = cuda.zeros(3, dtype=cuda.int32, device="cuda")
+    with make_ctx(pkg, 128) as ctx:
+        args = (r.kv, 3, 3, None, r.lens)
+        bad = pytest.raises(pkg.GqaError)
+        with bad:
+            ctx.paged_append(*args, r.qkv, qkv_stride=4096)
+        with bad:
+            ctx.paged_append(*args, r.qkv[:2].reshape(-1))
+        with bad:
+            ctx.paged_attention(*args, 1, 40, r.qkv, out[:2].reshape(-1))
+        with bad:
+            ctx.paged_attention(*args, 1, 40, r.qkv, out, out_stride=2048)
+        with bad:
+            ctx.sample(3, 100, logits, None, None, None, None, u, tok, logits_stride=128)
+        with bad:
+            ctx.sample(3, 100, logits, None, None, None, None, u[:2], tok)
+        want = r.attend(ctx)
+        heads = cuda.zeros(3, 12, 128, device="cuda")
+        ctx.paged_attention(*args, 1, 40, r.qkv.reshape(-1), heads)
+        assert cuda.equal(heads.reshape(3, -1), want)
+        wide = cuda.zeros(3, 2048, device="cuda")
+        ctx.paged_attention(*args, 1, 40, r.qkv, wide[:, :1536], out_stride=2048)
+        assert cuda.equal(wide[:, :1536], want)
+        assert ctx.device_status() == 0
