@@ -324,6 +324,8 @@ def _matrix(x, what: str, device: int, dtype: int, rows: int, width: int,
         raise GqaError(GQA_ERR_INVALID_ARG,
                        f"{what} is {x.dtype} on {x.device}: the call's type (GQA dtype {dtype}) on "
                        f"cuda:{device} is needed")
+    if rows == 0:  # (torch gives an empty tensor strides of its own)
+        return x.data_ptr(), width if stride is None else stride
     if x.dim() == 2:
         n, w = x.shape
         own = x.stride()

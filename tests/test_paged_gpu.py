@@ -598,3 +598,22 @@ def test_tensors_too_small_for_their_stride(pkg, cuda):
         ctx.paged_attention(*args, 1, 40, r.qkv, wide[:, :1536], out_stride=2048)
         assert cuda.equal(wide[:, :1536], want)
         assert ctx.device_status() == 0
+
+
+def test_empty_batches(pkg, cuda):
+    """Steps in which no sequence brings a token, as tensors of no rows."""
+    b = Batch("bf16", 128, [1, 1], [20, 30], page=16, seed=27)
+    r = Run(pkg, b)
+    before = r.kp.clone()
+    starts = cuda.zeros(3, dtype=cuda.int32, device="cuda")
+    none = r.qkv[:0]
+    out = cuda.empty(0, 12 * 128, dtype=b.td, device="cuda")
+    with make_ctx(pkg, 128) as ctx:
+        ctx.paged_append(r.kv, 2, 0, starts, r.lens, none)
+        ctx.paged_attention(r.kv, 2, 0, starts, r.lens, 1, 30, none, out)
+        ctx.paged_append(r.kv, 0, 0, None, r.lens[:0], none)
+        empty = cuda.empty(0, device="cuda")
+        ctx.sample(0, 100, cuda.empty(0, 100, device="cuda"), empty, None, None, None, empty,
+                   r.lens[:0])
+        assert ctx.device_status() == 0
+    assert cuda.equal(r.kp.isnan(), before.isnan())
