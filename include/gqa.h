@@ -575,7 +575,10 @@ GQA_API int gqa_paged_append(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_
  * were).  Results go to out + row * out_stride (n_heads_q * head_dim
  * elements); out may equal qkv with the same stride.  A token with no
  * readable row gets zeros.  Rows of the cache past a token's position, and
- * whatever stands in a page past the sequence's end, do not reach its output. */
+ * whatever stands in a page past the sequence's end, do not reach its output;
+ * an infinity or a NaN in a row that it attends may make it NaN.  Sums are
+ * fp32; in 16 bits a sequence with two or more new tokens has its rotated q and
+ * the weights rounded to the type, single tokens only their output. */
 GQA_API int gqa_paged_attention(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_kv *kv,
                                 int n_seq, int n_tokens, const int *q_starts,
                                 const int *seq_lens, int max_new, int max_len, const void *qkv,

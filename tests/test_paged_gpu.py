@@ -617,3 +617,47 @@ def test_empty_batches(pkg, cuda):
                    r.lens[:0])
         assert ctx.device_status() == 0
     assert cuda.equal(r.kp.isnan(), before.isnan())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_graphs_replayed_with_other_lengths(pkg, cuda, dtype):
+    """Two captured graphs of one context, replayed in turn while the plan in device memory (which
+    sequences bring how many tokens, lengths, pages) changes under them."""
+    plans = [([30, 1, 1, 0], [90, 500, 40, 0]), ([1, 1, 28, 2], [1, 900, 700, 2]),
+             ([8, 8, 8, 8], [8, 8, 300, 1000]), ([1, 1, 1, 1], [64, 1, 1024, 17])]
+    batches = [Batch(dtype, 128, *p, page=16, seed=30 + i) for i, p in enumerate(plans)]
+    for b in batches:
+        b.set_appended()
+    runs = [Run(pkg, b, one=False) for b in batches]
+    n_pages = max(b.n_pages for b in batches)
+    cols = max(b.table.shape[1] for b in batches)
+    kp, vp = (cuda.zeros(n_pages, 2, 16, 128, dtype=batches[0].td, device="cuda") for _ in "kv")
+    table = cuda.zeros(4, cols, dtype=cuda.int32, device="cuda")
+    lens = cuda.zeros(4, dtype=cuda.int32, device="cuda")
+    starts = cuda.zeros(5, dtype=cuda.int32, device="cuda")
+    qkv = cuda.zeros(32, batches[0].qkv.shape[1], dtype=batches[0].td, device="cuda")
+    outs = [cuda.zeros(32, 12 * 128, dtype=batches[0].td, device="cuda") for _ in range(2)]
+    kv = pkg.paged_kv_of(kp, vp, table)
+    with make_ctx(pkg, 128) as ctx:
+        graphs = []
+        for out in outs:
+            g = cuda.cuda.CUDAGraph()
+            with cuda.cuda.graph(g):
+                ctx.paged_append(kv, 4, 32, starts, lens, qkv)
+                ctx.paged_attention(kv, 4, 32, starts, lens, 32, 1024, qkv, out)
+            graphs.append(g)
+        for turn in range(8):
+            b, r = batches[turn % 4], runs[turn % 4]
+            kp[:b.n_pages], vp[:b.n_pages] = r.kp, r.vp
+            table[:, :b.table.shape[1]] = r.table
+            lens.copy_(r.lens)
+            starts.copy_(r.starts)
+            qkv[:b.n_tokens] = r.qkv
+            out = outs[turn % 2]
+            out.fill_(7.0)
+            graphs[turn % 2].replay()
+            cuda.cuda.synchronize()
+            assert ctx.device_status() == 0
+            check_attention(b, out)
+            assert (out[b.n_tokens:] == 7).all()
+        del graphs
