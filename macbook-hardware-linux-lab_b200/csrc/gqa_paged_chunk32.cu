@@ -234,7 +234,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
           put4(sm.k, kKeys, w * kRowsWarp + i * kSide + sub, col, x[i]);
-        if (lane == 0) sm.bad[n & 3][w * kRowsWarp / 16] = page < 0;  // (alike in two warps)
+        // (two warps share a 16-row part; the first half's knows its page wherever a row of the
+        // part is in use, the second half's does not where the unit ends before its rows)
+        static_assert(kRowsWarp == 8, "two operand warps to a 16-row part");
+        if (lane == 0 && w % 2 == 0) sm.bad[n & 3][w / 2] = page < 0;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.k_full);
