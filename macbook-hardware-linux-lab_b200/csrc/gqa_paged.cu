@@ -24,8 +24,10 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppendParams p) {
   using V = Vec16<T>;
   constexpr int kChunks = D / 2 / V::n;
-  pdl_launch_dependents();
+  // (in this order: the next kernel may read cache rows ahead of its own wait, and relies on all
+  // before this one being done when it starts)
   pdl_wait();
+  pdl_launch_dependents();
   const int per_token = p.n_kv * kChunks;
   const long long item = (long long)blockIdx.x * kAppendThreads + threadIdx.x;
   const long long last = (long long)p.plan.n_tokens * per_token - 1;
