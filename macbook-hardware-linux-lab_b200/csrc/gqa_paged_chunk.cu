@@ -135,6 +135,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// Weights are taken relative to m, which is held kLift below the row's reference, and the reference
+// moves to the row's maximum when the weights of a tile add up to more than kMost.  fp16 ends at 2^-24
+// and 2^16: with m at the reference itself, a weight below 2^-25 of it would be lost from the product
+// and stay in the sum; lifted by 2^8 what is lost lies below 2^-33, and 128 keys as large as the
+// reference still add up to kMost.  (Bounded by their sum, no weight passes 2^15.)  bf16 has fp32's
+// range.
+template <typename T>
+constexpr float kLift = __is_same(T, __half) ? 8.f : 0.f;
+template <typename T>
+constexpr float kMost = __is_same(T, __half) ? 32768.f : 1024.f;
+
 // Whether key tile kt holds rows past the piece's first token (at pos), which not all its rows see.
 __device__ __forceinline__ bool clears_v(int pos, int kt) {
   return (kt + 1) * kKeys > pos + 1;
@@ -555,9 +566,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i)
             if (bad >> (4 * half + i) & 1) hidden |= 0xffffull << (16 * i);
         }
-        // Weights against the running reference m, which is moved to the row's maximum (in a
+        // Weights against the running reference, which is moved to the row's maximum (in a
         // second pass over the scores) only on the piece's first tile, or when the weights of
-        // the tile add up to more than 2^10 in some row; the two halves of a row agree on it by
+        // the tile add up to more than kMost in some row; the two halves of a row agree on it by
         // their sums.  No P is stored before that, as it goes over the scores.
         uint32_t pk0[16], pk1[16];
         float alpha = 1.f, sum0, sum1;
@@ -580,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int pass = 0; pass < 2; ++pass) {
           if (move) {
             const float top = max64(t_s, hidden);
-            const float mn = fmaxf(m, fmaxf(top, other(top)) * sc);
+            const float mn = fmaxf(m, fmaxf(top, other(top)) * sc - kLift<T>);
             alpha = mn == m ? 1.f : fast_exp2(m - mn);
             m = mn;
           }
@@ -589,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           weights(32, pk1);
           if (move) break;
           const float sum = sum0 + sum1;
-          move = __any_sync(0xffffffffu, !(sum + other(sum) <= 1024.f));
+          move = __any_sync(0xffffffffu, !(sum + other(sum) <= kMost<T>));
           if (!move) break;
         }
         __syncwarp();

@@ -139,10 +139,16 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t& hi, uin
        (uint32_t)reinterpret_cast<const uint16_t&>(l1) << 16;
 }
 
-// The running reference m of a softmax moves only when a score passes it by more than
-// this (weights then stay below 2^8), which saves the reduction and the rescale in almost
+// The running reference of a softmax moves only when a score passes it by more than
+// this (weights then stay below 2^8 of it), which saves the reduction and the rescale in almost
 // every group.
 constexpr float kSlack = 8.f;
+
+// m is held kLift below the reference.  fp16 ends at 2^-24 and 2^16: with m at the reference itself, a
+// weight below 2^-25 of it would be lost from the product and stay in the sum l; lifted by 2^7 (the
+// largest weight is then 2^15), what is lost lies below 2^-32.  bf16 has fp32's range.
+template <typename T>
+constexpr float kLift = __is_same(T, __half) ? 7.f : 0.f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -199,13 +205,14 @@ struct WarpState {
     if (r >= valid) c[0] = c[1] = -CUDART_INF_F;
     if (r + 8 >= valid) c[2] = c[3] = -CUDART_INF_F;
     float mx0 = fmaxf(c[0], c[2]), mx1 = fmaxf(c[1], c[3]);
-    if (__any_sync(0xffffffffu, mx0 > m[0] + kSlack || mx1 > m[1] + kSlack)) {
+    if (__any_sync(0xffffffffu, mx0 > m[0] + (kSlack + kLift<T>) ||
+                                      mx1 > m[1] + (kSlack + kLift<T>))) {
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
       }
-      const float n0 = fmaxf(m[0], mx0), n1 = fmaxf(m[1], mx1);
+      const float n0 = fmaxf(m[0], mx0 - kLift<T>), n1 = fmaxf(m[1], mx1 - kLift<T>);
       const float a0 = n0 == m[0] ? 1.f : exp2_fast(m[0] - n0);
       const float a1 = n1 == m[1] ? 1.f : exp2_fast(m[1] - n1);
       m[0] = n0;
