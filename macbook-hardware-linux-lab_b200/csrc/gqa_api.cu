@@ -1722,10 +1722,10 @@ int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv,
   if (max_new < 1 || (!q_starts && max_new != 1))
     return fail(GQA_ERR_INVALID_ARG, "max_new %d below 1, or not 1 without q_starts", max_new);
   max_new = std::min(max_new, std::min(max_len, n_tokens));
-  const char* q0 = static_cast<const char*>(qkv);
-  const char* o0 = static_cast<const char*>(out);
-  if ((o0 != q0 || out_stride != qkv_stride) && o0 < q0 + qkv_stride * size * n_tokens &&
-      q0 < o0 + out_stride * size * n_tokens)
+  const long long row_o = nq * hd * size, row_q = row_o + 2 * c->cfg.n_heads_kv * hd * size;
+  if ((out != qkv || out_stride != qkv_stride) &&
+      !rows_apart((uintptr_t)qkv, qkv_stride * size, row_q, (uintptr_t)out, out_stride * size, row_o,
+                  n_tokens))
     return fail(GQA_ERR_INVALID_ARG, "out overlaps qkv without being equal to it");
   DeviceGuard g(c->device);
   PagedAttnParams p{};

@@ -39,6 +39,21 @@ struct PagedPartials {
   int n_chunk_ctas;
 };
 
+// Whether no byte of n rows of a_width bytes, a_stride apart, is one of n rows of b_width, b_stride
+// apart.  Rows that interleave are told apart where the strides are equal; otherwise whole extents
+// are (each from its first row's start to its last row's end).
+inline bool rows_apart(unsigned long long a, long long a_stride, long long a_width,
+                       unsigned long long b, long long b_stride, long long b_width, int n) {
+  using Wide = __int128;  // (n rows of the largest stride pass 64 bits)
+  const Wide a_end = (Wide)a + (Wide)(n - 1) * a_stride + a_width;
+  const Wide b_end = (Wide)b + (Wide)(n - 1) * b_stride + b_width;
+  if (b >= a_end || a >= b_end) return true;
+  if (a_stride != b_stride) return false;
+  Wide at = ((Wide)b - (Wide)a) % a_stride;  // where b's rows start in a's
+  if (at < 0) at += a_stride;
+  return at >= a_width && at + b_width <= a_stride;
+}
+
 template <typename... P, typename... A>
 cudaError_t launch_with_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
                             cudaStream_t st, bool pdl, const A&... args) {
