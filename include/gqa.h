@@ -545,7 +545,8 @@ typedef struct {
     int n_pages;    /* pages in each pool */
     int max_pages;  /* entries of a sequence's page table row */
     void *k_pages, *v_pages;                       /* 16-byte aligned */
-    long long page_stride, head_stride, row_stride; /* elements, multiples of 16 bytes */
+    /* elements; multiples of 16 bytes, below 2^40 bytes (as the calls' row strides) */
+    long long page_stride, head_stride, row_stride;
     const int *page_table;                         /* [n_seq][max_pages] */
     long long table_stride;                        /* elements, >= max_pages */
 } gqa_paged_kv;

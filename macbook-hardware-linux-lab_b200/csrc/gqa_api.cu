@@ -613,7 +613,8 @@ int shard_partials(gqa_ctx* c, cudaStream_t st, const gqa_layer_kv* kv, const fl
 
 // ---- paged operators: argument checks ----
 
-constexpr long long kPagedMaxStride = 1LL << 40;  // elements
+// Largest stride in bytes, a multiple of 16 (a tensor map takes none of 2^40 or more).
+constexpr long long kPagedMaxStride = (1LL << 40) - 16;
 
 int dtype_size(int dtype) {
   return dtype == GQA_F32 ? 4 : dtype == GQA_BF16 || dtype == GQA_F16 ? 2 : 0;
@@ -631,13 +632,14 @@ int check_paged(const gqa_ctx* c, const gqa_paged_kv* kv, int n_seq, int n_token
   if (kv->n_pages < 1 || kv->max_pages < 1 || kv->max_pages > (1 << 30) / ps)
     return fail(GQA_ERR_INVALID_ARG, "n_pages %d or max_pages %d out of range", kv->n_pages,
                 kv->max_pages);
-  if (kv->table_stride < kv->max_pages || kv->table_stride > kPagedMaxStride)
-    return fail(GQA_ERR_INVALID_ARG, "table_stride smaller than max_pages");
+  if (kv->table_stride < kv->max_pages || kv->table_stride > kPagedMaxStride / 4)
+    return fail(GQA_ERR_INVALID_ARG, "table_stride outside [max_pages, %lld]", kPagedMaxStride / 4);
   const int hd = c->cfg.head_dim, nkv = c->cfg.n_heads_kv;
-  const auto bad = [&](long long s) { return s < hd || s > kPagedMaxStride || (s * size & 15); };
+  const long long most = kPagedMaxStride / size;
+  const auto bad = [&](long long s) { return s < hd || s > most || (s * size & 15); };
   if (bad(kv->page_stride) || bad(kv->head_stride) || bad(kv->row_stride))
-    return fail(GQA_ERR_INVALID_ARG, "page, head and row strides must be multiples of 16 bytes of "
-                "at least head_dim elements");
+    return fail(GQA_ERR_INVALID_ARG, "page, head and row strides must be multiples of 16 bytes, "
+                "of [head_dim, %lld] elements", most);
   if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
     return fail(GQA_ERR_INVALID_ARG, "pages must be 16-byte aligned");
   if (n_seq < 0 || n_seq > 65535 || n_tokens < 0 || n_tokens > (1 << 24))
@@ -648,10 +650,11 @@ int check_paged(const gqa_ctx* c, const gqa_paged_kv* kv, int n_seq, int n_token
     return fail(GQA_ERR_INVALID_ARG, "without q_starts every sequence has one token (%d of %d)",
                 n_tokens, n_seq);
   if (!seq_lens || !qkv) return fail(GQA_ERR_INVALID_ARG, "null seq_lens or qkv");
+  const long long row = (long long)(c->cfg.n_heads_q + 2 * nkv) * hd;
+  if (qkv_stride < row || qkv_stride > most)
+    return fail(GQA_ERR_INVALID_ARG, "qkv stride outside [%lld, %lld]", row, most);
   if (!aligned16(qkv) || (qkv_stride * size & 15))
     return fail(GQA_ERR_INVALID_ARG, "qkv and its stride must be 16-byte aligned");
-  if (qkv_stride < (long long)(c->cfg.n_heads_q + 2 * nkv) * hd || qkv_stride > kPagedMaxStride)
-    return fail(GQA_ERR_INVALID_ARG, "qkv stride smaller than one token's row");
   return GQA_OK;
 }
 
@@ -1712,10 +1715,11 @@ int gqa_paged_attention(gqa_ctx* c, gqa_stream_t stream, const gqa_paged_kv* kv,
   if (rc != GQA_OK || n_tokens == 0) return rc;
   const int nq = c->cfg.n_heads_q, hd = c->cfg.head_dim;
   const long long size = dtype_size(kv->dtype);
+  if (out_stride < (long long)nq * hd || out_stride > kPagedMaxStride / size)
+    return fail(GQA_ERR_INVALID_ARG, "out stride outside [%d, %lld]", nq * hd,
+                kPagedMaxStride / size);
   if (!out || !aligned16(out) || (out_stride * size & 15))
     return fail(GQA_ERR_INVALID_ARG, "out and its stride must be 16-byte aligned");
-  if (out_stride < (long long)nq * hd || out_stride > kPagedMaxStride)
-    return fail(GQA_ERR_INVALID_ARG, "out stride outside [%d, %lld]", nq * hd, kPagedMaxStride);
   if (max_len < 1) return fail(GQA_ERR_INVALID_ARG, "max_len %d below 1", max_len);
   // (no length beyond the table's rows is accepted by the kernels)
   max_len = std::min(max_len, kv->max_pages * kv->page_size);
@@ -1770,8 +1774,9 @@ int gqa_sample(gqa_ctx* c, gqa_stream_t stream, int n_rows, int vocab, int dtype
     return fail(GQA_ERR_INVALID_ARG, "gqa_sample: null logits, uniform or tokens");
   if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype))
     return fail(GQA_ERR_INVALID_ARG, "logits not aligned to their type");
-  if (logits_stride < vocab || logits_stride > kPagedMaxStride)
-    return fail(GQA_ERR_INVALID_ARG, "logits stride outside [vocab, %lld]", kPagedMaxStride);
+  if (logits_stride < vocab || logits_stride > kPagedMaxStride / dtype_size(dtype))
+    return fail(GQA_ERR_INVALID_ARG, "logits stride outside [vocab, %lld]",
+                kPagedMaxStride / dtype_size(dtype));
   DeviceGuard g(c->device);
   SampleParams p{};
   p.logits = logits;
