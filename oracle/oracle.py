@@ -52,10 +52,16 @@ def build() -> None:
     subprocess.run(["make", "-s", "-C", HERE], check=True)
 
 
+class ReferenceMissing(FileNotFoundError):
+    """A library compiled from the reference's sources is not there: they were absent at build
+    time."""
+
+
 def _load(path: str) -> ctypes.CDLL:
     if path not in _libs:
         if not os.path.exists(path):
-            raise FileNotFoundError(f"{path} not built (run make -C oracle)")
+            kind = FileNotFoundError if path == ORACLE_SO else ReferenceMissing
+            raise kind(f"{path} not built (run make -C oracle)")
         _libs[path] = ctypes.CDLL(path)
     return _libs[path]
 
