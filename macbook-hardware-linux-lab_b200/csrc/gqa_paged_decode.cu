@@ -150,12 +150,6 @@ constexpr float kSlack = 8.f;
 template <typename T>
 constexpr float kLift = __is_same(T, __half) ? 7.f : 0.f;
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // One warp's softmax state over the groups it has seen, for the 16-bit types: scores and
 // outputs transposed (S^T = K Q^T with 16 rows by 8 heads, O^T = V^T P^T), so that the
 // instruction's eight columns are the heads of a KV head.  q and the weights enter as two
@@ -213,8 +207,8 @@ struct WarpState {
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
       }
       const float n0 = fmaxf(m[0], mx0 - kLift<T>), n1 = fmaxf(m[1], mx1 - kLift<T>);
-      const float a0 = n0 == m[0] ? 1.f : exp2_fast(m[0] - n0);
-      const float a1 = n1 == m[1] ? 1.f : exp2_fast(m[1] - n1);
+      const float a0 = n0 == m[0] ? 1.f : fast_exp2(m[0] - n0);
+      const float a1 = n1 == m[1] ? 1.f : fast_exp2(m[1] - n1);
       m[0] = n0;
       m[1] = n1;
       l[0] *= a0;
@@ -227,8 +221,8 @@ struct WarpState {
         o[s][3] *= a1;
       }
     }
-    const float p0 = exp2_fast(c[0] - m[0]), p1 = exp2_fast(c[1] - m[1]);
-    const float p2 = exp2_fast(c[2] - m[0]), p3 = exp2_fast(c[3] - m[1]);
+    const float p0 = fast_exp2(c[0] - m[0]), p1 = fast_exp2(c[1] - m[1]);
+    const float p2 = fast_exp2(c[2] - m[0]), p3 = fast_exp2(c[3] - m[1]);
     l[0] += p0 + p2;
     l[1] += p1 + p3;
     uint32_t h0, h1, l0, l1;
