@@ -68,8 +68,11 @@ typedef struct {
  * built: head_dim 128 with 6 q heads per KV head (Qwen2.5-1.5B, every entry
  * point) and head_dim 64 with 7 (Qwen2.5-0.5B, generate_stream_05b.c:19-31:
  * gqa_kv_alloc/free, gqa_reserve, gqa_layer_attention(_out),
- * gqa_decode_layers and the layer graphs, on shape-generic kernels; the other
- * entry points return GQA_ERR_UNSUPPORTED for it). */
+ * gqa_decode_layers and the layer graphs, on shape-generic kernels, the paged
+ * cache and sampling; the other entry points return GQA_ERR_UNSUPPORTED for
+ * it).  A context holds the paged attention's partial results from its start
+ * (41 MB for head_dim 128, 20 for 64), so that captured graphs never see them
+ * move. */
 GQA_API int gqa_create(const gqa_config *cfg, int device, gqa_ctx **out);
 GQA_API int gqa_destroy(gqa_ctx *ctx);
 
@@ -562,7 +565,8 @@ typedef struct {
  * sequence.  The angle pos * theta^(-2i/d) is formed in 64 bits (the decode
  * calls above form it in fp32, as the reference does), so that far positions
  * keep their place; q is not touched.  Two tokens of one call must not be
- * given the same cache row.  Both shapes of gqa_create. */
+ * given the same cache row.  n_seq up to 65535, n_tokens up to 2^24.  Both
+ * shapes of gqa_create. */
 GQA_API int gqa_paged_append(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_kv *kv, int n_seq,
                              int n_tokens, const int *q_starts, const int *seq_lens,
                              const void *qkv, long long qkv_stride);
@@ -574,12 +578,14 @@ GQA_API int gqa_paged_append(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_
  * the rows of every sequence (a sequence beyond either sets
  * GQA_STATUS_BAD_LENGTH and is skipped: its rows of out are left as they
  * were).  Results go to out + row * out_stride (n_heads_q * head_dim
- * elements); out may equal qkv with the same stride.  A token with no
+ * elements); out may equal qkv with the same stride, and must not touch its
+ * rows otherwise (both may be columns of one buffer).  A token with no
  * readable row gets zeros.  Rows of the cache past a token's position, and
  * whatever stands in a page past the sequence's end, do not reach its output;
  * an infinity or a NaN in a row that it attends may make it NaN.  Sums are
  * fp32; in 16 bits a sequence with two or more new tokens has its rotated q and
- * the weights rounded to the type, single tokens only their output. */
+ * the weights rounded to the type, single tokens only their output.  In fp16
+ * weights below 2^-32 of a row's largest may be lost. */
 GQA_API int gqa_paged_attention(gqa_ctx *ctx, gqa_stream_t stream, const gqa_paged_kv *kv,
                                 int n_seq, int n_tokens, const int *q_starts,
                                 const int *seq_lens, int max_new, int max_len, const void *qkv,
@@ -598,7 +604,10 @@ GQA_API int gqa_paged_attention(gqa_ctx *ctx, gqa_stream_t stream, const gqa_pag
  * always stays).  tokens[row] is the first id, in ascending order of id, at
  * which the cumulative kept weight exceeds uniform[row] (in [0, 1)) times the
  * kept total.  Weights are added as 62-bit integers, exact in any order: equal
- * inputs give equal tokens.  All arrays are device arrays of n_rows;
+ * inputs give equal tokens.  Their unit is the larger of 2^-50 and vocab' *
+ * 2^-62 of the largest weight, vocab' the next power of two (2^-44 for 151936):
+ * a weight below half of it counts as zero and is never drawn.  n_rows up to
+ * 2^20.  All arrays are device arrays of n_rows;
  * temperature NULL means 1, top_k / top_p / min_p NULL leave that filter out.
  * In a row, top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 leave it out
  * too, and temperature <= 0 takes the first largest logit.  A NaN logit counts

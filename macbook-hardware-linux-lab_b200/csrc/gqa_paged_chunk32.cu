@@ -3,11 +3,12 @@
 //
 // Each fp32 number enters as three bf16 terms (x = h + m + l, 8 significant bits each,
 // exactly), and a product of two as the six products of terms that matter (hh, hm, mh, mm,
-// hl, lh; the rest is below 2^-22, and some 2^-25 on average): six bf16 matrix products in place of one, 279 TFLOP/s at
-// the measured bf16 rate against some 70 of the fp32 units, with fp32's accuracy.  bf16 terms
-// rather than fp16 ones (which would do with three products) because they have fp32's range:
-// no scales, and columns of V of very different size keep their digits.  The products of
-// small terms are added first.  Sums of many tiles are kept in registers: the tensor cores
+// hl, lh).  Terms are cut off, not rounded, so they have the number's sign and what is left out
+// makes a product smaller: by less than 2^-21 of it, 2^-24.5 on average.  Six bf16 matrix
+// products in place of one, 279 TFLOP/s at the measured bf16 rate against some 70 of the fp32
+// units.  bf16 terms rather than fp16 ones (which would do with three products) because they
+// have fp32's range: no scales, and columns of V of very different size keep their digits.  The
+// products of small terms are added first.  Sums of many tiles are kept in registers: the tensor cores
 // add within a tile only (24 steps of 16 keys), so that how they round an addition cannot
 // build up over a long cache.
 //
@@ -284,9 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&sm.q_full);
           continue;
         }
-        // A weight of zero does not cancel an infinity or a NaN (and the terms of a weight
-        // have signs): what is not finite stays out of the product, and is added at the end to
-        // the rows that see it.
+        // A weight of zero does not cancel an infinity or a NaN: what is not finite stays out of
+        // the product, and is added at the end to the rows that see it.
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {

@@ -27,10 +27,10 @@
 // the step is cut again by the pair's 64 bits.  For top-p the histogram holds weights
 // rounded to 14 bits; they only propose the step, which the exact sums confirm or move.
 //
-// Measured: one row of 151936 in fp32 with top-k, top-p and min-p 12.2 us (latency: the load, two
-// exchanges over the cluster, the ranks); 64 rows with a setting each of their own 70 us, where
-// the instructions of two to four passes over the row bound it (80 a logit, half of them for the
-// 64-bit weights), not the 39 MB, which take 6.
+// Measured: one row of 151936 in fp32 with top-k, top-p and min-p 11.9 us (latency: the load, three
+// exchanges over the cluster and the barrier at its end, the ranks); 64 rows with a setting each of
+// their own 60 us for two to four passes over the row (the 39 MB take 6).  What bounds the passes is
+// not settled: issue slots are 30 % busy, and weights in fp32 took 2 % off.
 #include <algorithm>
 
 #include <math_constants.h>
